@@ -42,7 +42,8 @@ typedef enum tp_status {
   TP_ERR_CUDA = 3         /* launch / runtime failure (RuntimeError) */
 } tp_status;
 
-typedef enum tp_dtype { TP_F16 = 0, TP_F32 = 1 } tp_dtype;
+/* TP_BF16 is taken by tp_norm_rope and tp_prompt_attention only: caches hold float16 or float32. */
+typedef enum tp_dtype { TP_F16 = 0, TP_F32 = 1, TP_BF16 = 2 } tp_dtype;
 
 /* Key format: the fields of TurboPolarConfig that shape a PolarKeyBlock
  * (rfsn_v11/candidates/turbo_polar_config.py:11-21, rfsn_v11/quant/polar/encoder.py:24-98). */
@@ -302,6 +303,37 @@ int tp_export_pages(const tp_page_pool* pool, int32_t first_page, int32_t n_page
  * rfsn_v11/kernels/turbo_polar/metal.py:651-792). */
 int tp_import_pages(const tp_page_pool* pool, int32_t first_page, int32_t n_pages, const tp_block_store* ref,
                     void* stream);
+
+/* ---- Prompt chunks and drafted tokens: the step that makes queries and keys, and attention with
+ * more than one query token.  The reference leaves these to MLX (benchmarks/
+ * turbopolar_fast_attention.py:56-86 and :247-278: rotation, then dense attention). */
+
+/* Layout of a tp_norm_rope call.  Row (b, t, h) of 128 contiguous channels of the queries is
+ * q_in[0] * b + q_in[1] * t + q_in[2] * h elements into q, and alike for the keys and the outputs
+ * (an axis of one entry may have any stride; rows start on boundaries of four elements).  The
+ * angle tables have table_rows rows of 64 values, row_stride elements apart.  Token (b, t) uses row
+ * positions[b * pos_strides[0] + t * pos_strides[1]] (int32, or int64 with pos64), or row
+ * b * batch_rows + t without positions. */
+typedef struct tp_rope_layout {
+  int32_t batch, tokens, q_heads, k_heads;
+  int32_t dtype;          /* of q, k and the outputs */
+  int32_t weight_dtype;   /* of both weights */
+  int32_t table_dtype;    /* of cos and sin */
+  int32_t interleaved;    /* pairs (2d, 2d + 1) instead of (d, d + 64) */
+  int64_t q_in[3], k_in[3], q_out[3], k_out[3];
+  int64_t row_stride, pos_strides[2];
+  int32_t table_rows, batch_rows, pos64;
+  float eps;
+} tp_rope_layout;
+
+/* Norm of each query and key head and the position rotation, in one pass:
+ *   y = x * rsqrt(mean(x^2) + eps) * weight      (y = x where the weight [128] is NULL)
+ *   (a, b) -> (a cos - b sin, b cos + a sin) for the pairs (y[d], y[d + 64]) or (y[2d], y[2d + 1])
+ * in float32, rounded once.  A position outside the table gives NaN rows.  An output may be its
+ * own input with the same strides, and otherwise shares no element with an input. */
+int tp_norm_rope(const tp_rope_layout* layout, const void* q, const void* k, const void* q_weight,
+                 const void* k_weight, const void* cos, const void* sin, const void* positions,
+                 void* q_out, void* k_out, void* stream);
 
 /* Message of the last failed call on this thread ("" if none). */
 const char* tp_last_error(void);

@@ -9,6 +9,7 @@ Public API (names of dawsonblock/Turbopolar):
 * :class:`PolarQuantEncoder`, :class:`PolarQuantDecoder`, :class:`GroupedVQuantizer`
 * :mod:`turbopolar_b200.llama` -- PyTorch Llama adapter (``TurboPolarFastCache``,
   ``make_turbo_caches``, ``patch_llama_attention``)
+* :func:`norm_rope` -- norms of the query and key heads with the position rotation, in one pass
 * :mod:`turbopolar_b200.sharded` -- sequence-sharded multi-GPU attention
 
 All compute runs in ``libturbopolar.so`` (``include/turbopolar.h``), built by
@@ -20,8 +21,9 @@ from .payload import PolarKeyBlock, QuantizedVBlock
 from .cache import TurboPolarKVCacheRuntime
 from .codec import GroupedVQuantizer, PolarQuantDecoder, PolarQuantEncoder
 from .bridge import CudaKernelBridge
+from .rotary import norm_rope
 
 __all__ = [
     "TurboPolarConfig", "TurboPolarKVCacheRuntime", "CudaKernelBridge", "PolarKeyBlock", "QuantizedVBlock",
-    "PolarQuantEncoder", "PolarQuantDecoder", "GroupedVQuantizer",
+    "PolarQuantEncoder", "PolarQuantDecoder", "GroupedVQuantizer", "norm_rope",
 ]

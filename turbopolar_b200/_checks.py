@@ -1,0 +1,64 @@
+"""Argument checks shared by the prompt and draft operators."""
+
+from __future__ import annotations
+
+from typing import Tuple
+
+import torch
+
+HEAD_DIM = 128
+
+
+def refuse_gradients(*tensors) -> None:
+    """The kernels have no backward pass: say so rather than return outputs without a gradient."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise NotImplementedError("TurboPolar kernels have no backward pass; call them under torch.no_grad()")
+
+
+def launch(device: torch.device, fn, *args) -> int:
+    """``fn(*args, stream)`` on ``device`` and its current stream."""
+    i = device.index
+    stream = torch._C._cuda_getCurrentRawStream(i)
+    if i == torch.cuda.current_device():
+        return fn(*args, stream)
+    with torch.cuda.device(device):
+        return fn(*args, stream)
+
+
+def extent(x: torch.Tensor) -> Tuple[int, int]:
+    """The byte range [lo, hi) that a non-empty tensor touches (strides are never negative)."""
+    last = sum((n - 1) * s for n, s in zip(x.shape, x.stride()))
+    return x.data_ptr(), x.data_ptr() + (last + 1) * x.element_size()
+
+
+def _share_rows(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """True when ``a`` and ``b`` ``(..., T, H, 128)`` are slices of the same token rows with no common
+    element: equal strides and, within a row, disjoint runs of heads (a fused projection's q and k)."""
+    if a.dim() != b.dim() or a.stride() != b.stride() or a.shape[:-2] != b.shape[:-2]:
+        return False
+    row = a.stride(-3)
+    off = (b.data_ptr() - a.data_ptr()) // a.element_size()
+    run_a, run_b = (a.shape[-2] - 1) * a.stride(-2) + HEAD_DIM, (b.shape[-2] - 1) * b.stride(-2) + HEAD_DIM
+    return (run_a <= off and off + run_b <= row) or (run_b <= -off and -off + run_a <= row)
+
+
+def disjoint(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """False when two tensors of rows may have an element in common."""
+    if not a.numel() or not b.numel():
+        return True
+    (a0, a1), (b0, b1) = extent(a), extent(b)
+    return a1 <= b0 or b1 <= a0 or _share_rows(a, b)
+
+
+def check_out(out: torch.Tensor, shape, dtype, device, what: str) -> None:
+    """``out`` is a tensor of this shape, type and device whose elements are all different places."""
+    if not isinstance(out, torch.Tensor) or tuple(out.shape) != tuple(shape) or out.dtype != dtype or out.device != device:
+        raise ValueError(f"{what} must be a {tuple(shape)} tensor of {dtype} on {device}")
+    axes = sorted((s, n) for s, n in zip(out.stride(), out.shape) if n > 1)
+    reach = 0
+    for s, n in axes:
+        if s <= reach:
+            raise ValueError(f"{what} must not overlap itself")
+        reach += s * (n - 1)

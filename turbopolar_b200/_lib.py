@@ -14,7 +14,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libturbopolar.so")
 
 TP_OK, TP_ERR_INVALID, TP_ERR_UNSUPPORTED, TP_ERR_CUDA = 0, 1, 2, 3
-TP_F16, TP_F32 = 0, 1
+TP_F16, TP_F32, TP_BF16 = 0, 1, 2
 PARTIAL_FLOATS = 130
 STATE_WORDS = 6
 
@@ -24,6 +24,7 @@ EXPORTED = (
     "tp_export_pages", "tp_import_pages", "tp_last_error", "tp_version",
     "tp_exchange_bytes", "tp_ipc_alloc", "tp_ipc_open", "tp_ipc_close", "tp_ipc_free",
     "tp_decode_attention_sharded", "tp_decode_step_sharded",
+    "tp_norm_rope",
 )
 MAX_RANKS = 8
 
@@ -71,6 +72,16 @@ class Exchange(ctypes.Structure):
     _fields_ = [("world", ctypes.c_int32), ("rank", ctypes.c_int32), ("buffers", ctypes.c_void_p * 8)]
 
 
+class RopeLayout(ctypes.Structure):
+    """tp_rope_layout: sizes, types and strides of a tp_norm_rope call."""
+    _fields_ = [("batch", ctypes.c_int32), ("tokens", ctypes.c_int32), ("q_heads", ctypes.c_int32),
+                ("k_heads", ctypes.c_int32), ("dtype", ctypes.c_int32), ("weight_dtype", ctypes.c_int32),
+                ("table_dtype", ctypes.c_int32), ("interleaved", ctypes.c_int32), ("q_in", ctypes.c_int64 * 3),
+                ("k_in", ctypes.c_int64 * 3), ("q_out", ctypes.c_int64 * 3), ("k_out", ctypes.c_int64 * 3),
+                ("row_stride", ctypes.c_int64), ("pos_strides", ctypes.c_int64 * 2), ("table_rows", ctypes.c_int32),
+                ("batch_rows", ctypes.c_int32), ("pos64", ctypes.c_int32), ("eps", ctypes.c_float)]
+
+
 _lib = None
 _lock = threading.Lock()
 
@@ -106,6 +117,7 @@ def _declare(lib):
                                                        I32, I32, F, P, ctypes.POINTER(Exchange), P, SZ, P]),
         "tp_decode_step_sharded": (ctypes.c_int, [ctypes.POINTER(PagePool), ctypes.POINTER(Tail), P, P, P, I32, I64, P,
                                                   I32, I32, F, P, ctypes.POINTER(Exchange), P, SZ, P]),
+        "tp_norm_rope": (ctypes.c_int, [ctypes.POINTER(RopeLayout), P, P, P, P, P, P, P, P, P, P]),
         "tp_last_error": (ctypes.c_char_p, []),
         "tp_version": (ctypes.c_int, []),
     }

@@ -1,0 +1,258 @@
+// Norm of each query and key head and the position rotation, in one pass over the rows.
+//
+// For one row x of 128 channels (one token of one head) at angle rows c, s of its position:
+//   y = x * rsqrt(mean(x^2) + eps) * w            (y = x without weights)
+//   pairs (a, b) = (y[d], y[d + 64]), or (y[2d], y[2d + 1]) when interleaved, d = 0..63
+//   out_a = a c[d] - b s[d],   out_b = b c[d] + a s[d]
+// The row is read once, the sum of squares and the rotation are float32, and the result is rounded
+// once to the output type.
+//
+// Bound: memory (read + write of q and k; 8,192 bfloat16 tokens of 32 + 8 heads move 172 MB).  A
+// group of 16 lanes owns a row: lane i holds channels [4i, 4i+4) and [64+4i, 64+4i+4), so both
+// pairings are inside one lane and only the sum of squares crosses lanes (four shuffles).
+#include <cuda_bf16.h>
+
+#include "tp_common.cuh"
+
+namespace tp {
+
+struct RopeSide {  // the query or the key heads
+  const void* in;
+  void* out;
+  const void* weight;
+  int64_t in_b, in_t, in_h, out_b, out_t, out_h;  // strides in elements
+};
+
+struct RopeParams {
+  RopeSide q, k;
+  const void *cos, *sin;
+  const void* positions;
+  int64_t table_stride, pos_b, pos_t;
+  int64_t n_units;      // batch * tokens * head groups
+  int batch, tokens, hq, hkv, table_rows, table_b_rows;
+  int pos64, table_dtype, weight_dtype, interleaved;
+  float eps;
+};
+
+template <typename T> struct Pack4;  // four elements of a row, moved as one word
+template <> struct Pack4<float> {
+  float4 v;
+  __device__ __forceinline__ void get(float* f) const { f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w; }
+  __device__ __forceinline__ void set(const float* f) { v = make_float4(f[0], f[1], f[2], f[3]); }
+};
+template <> struct Pack4<__half> {
+  uint2 v;
+  __device__ __forceinline__ void get(float* f) const {
+    const float2 a = __half22float2(u32_as_h2(v.x)), b = __half22float2(u32_as_h2(v.y));
+    f[0] = a.x, f[1] = a.y, f[2] = b.x, f[3] = b.y;
+  }
+  __device__ __forceinline__ void set(const float* f) { v = make_uint2(pack_h2(f[0], f[1]), pack_h2(f[2], f[3])); }
+};
+template <> struct Pack4<__nv_bfloat16> {
+  uint2 v;
+  __device__ __forceinline__ void get(float* f) const {
+    f[0] = __uint_as_float(v.x << 16), f[1] = __uint_as_float(v.x & 0xffff0000u);
+    f[2] = __uint_as_float(v.y << 16), f[3] = __uint_as_float(v.y & 0xffff0000u);
+  }
+  __device__ __forceinline__ void set(const float* f) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(f[0], f[1]), b = __floats2bfloat162_rn(f[2], f[3]);
+    v = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+  }
+};
+
+template <int N>
+__device__ __forceinline__ void load_small(const void* p, int64_t i, int dtype, float* f) {  // weights and angle rows
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    f[j] = dtype == TP_F32   ? static_cast<const float*>(p)[i + j]
+           : dtype == TP_F16 ? __half2float(static_cast<const __half*>(p)[i + j])
+                             : __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i + j]);
+  }
+}
+
+// kRows heads of one token per 16-lane group.
+template <typename T, int kRows>
+__global__ void __launch_bounds__(256) norm_rope_kernel(const __grid_constant__ RopeParams P) {
+  const int lane = threadIdx.x & 15;
+  const unsigned group_mask = 0xffffu << (threadIdx.x & 16);
+  const int64_t unit = (int64_t(blockIdx.x) * blockDim.x + threadIdx.x) >> 4;
+  if (unit >= P.n_units) return;
+  const int heads = P.hq + P.hkv;
+  const int hgroups = (heads + kRows - 1) / kRows;
+  const int64_t row = unit / hgroups;
+  const int h0 = int(unit - row * hgroups) * kRows;
+  const int b = int(row / P.tokens), t = int(row - int64_t(b) * P.tokens);
+
+  Pack4<T> raw[kRows][2];
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    const int h = h0 + r;
+    if (h < heads) {
+      const RopeSide& S = h < P.hq ? P.q : P.k;
+      const int hs = h < P.hq ? h : h - P.hq;
+      const T* in = static_cast<const T*>(S.in) + b * S.in_b + t * S.in_t + hs * S.in_h + 4 * lane;
+      raw[r][0] = *reinterpret_cast<const Pack4<T>*>(in);
+      raw[r][1] = *reinterpret_cast<const Pack4<T>*>(in + 64);
+    }
+  }
+  // The row of the angle table; a position outside the table gives NaN rows.
+  int64_t pos = t + int64_t(b) * P.table_b_rows;
+  if (P.positions) {
+    const int64_t i = b * P.pos_b + t * P.pos_t;
+    pos = P.pos64 ? static_cast<const int64_t*>(P.positions)[i] : static_cast<const int32_t*>(P.positions)[i];
+  }
+  const bool known = pos >= 0 && pos < P.table_rows;
+  // c[i], s[i]: rotation of pair i of this lane (pairs of four channels apart by 64, or adjacent).
+  float c[4], s[4];
+  if (known) {
+    const int64_t base = pos * P.table_stride;
+    if (P.interleaved) {
+      load_small<2>(P.cos, base + 2 * lane, P.table_dtype, c);
+      load_small<2>(P.cos, base + 32 + 2 * lane, P.table_dtype, c + 2);
+      load_small<2>(P.sin, base + 2 * lane, P.table_dtype, s);
+      load_small<2>(P.sin, base + 32 + 2 * lane, P.table_dtype, s + 2);
+    } else {
+      load_small<4>(P.cos, base + 4 * lane, P.table_dtype, c);
+      load_small<4>(P.sin, base + 4 * lane, P.table_dtype, s);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[i] = s[i] = __int_as_float(0x7fc00000);
+  }
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    const int h = h0 + r;
+    if (h >= heads) break;  // uniform in the group
+    const RopeSide& S = h < P.hq ? P.q : P.k;
+    const int hs = h < P.hq ? h : h - P.hq;
+    float lo[4], hi[4];
+    raw[r][0].get(lo);
+    raw[r][1].get(hi);
+    if (S.weight) {
+      float ss = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ss = fmaf(lo[i], lo[i], fmaf(hi[i], hi[i], ss));
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) ss += __shfl_xor_sync(group_mask, ss, o);
+      const float inv = rsqrtf(ss * (1.0f / kD) + P.eps);
+      float wl[4], wh[4];
+      load_small<4>(S.weight, 4 * lane, P.weight_dtype, wl);
+      load_small<4>(S.weight, 64 + 4 * lane, P.weight_dtype, wh);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        lo[i] = lo[i] * inv * wl[i];
+        hi[i] = hi[i] * inv * wh[i];
+      }
+    }
+    float ol[4], oh[4];
+    if (P.interleaved) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        ol[2 * i] = lo[2 * i] * c[i] - lo[2 * i + 1] * s[i];
+        ol[2 * i + 1] = lo[2 * i + 1] * c[i] + lo[2 * i] * s[i];
+        oh[2 * i] = hi[2 * i] * c[2 + i] - hi[2 * i + 1] * s[2 + i];
+        oh[2 * i + 1] = hi[2 * i + 1] * c[2 + i] + hi[2 * i] * s[2 + i];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        ol[i] = lo[i] * c[i] - hi[i] * s[i];
+        oh[i] = hi[i] * c[i] + lo[i] * s[i];
+      }
+    }
+    T* out = static_cast<T*>(S.out) + b * S.out_b + t * S.out_t + hs * S.out_h + 4 * lane;
+    Pack4<T> p;
+    p.set(ol);
+    *reinterpret_cast<Pack4<T>*>(out) = p;
+    p.set(oh);
+    *reinterpret_cast<Pack4<T>*>(out + 64) = p;
+  }
+}
+
+// Heads per 16-lane group: four, so that a group has eight loads in flight and reads its angle row
+// once for four heads; one where four would leave SMs without a CTA (few rows: latency counts).
+constexpr int kRopeRows = 4;
+
+template <typename T>
+static void launch_rope(RopeParams& P, cudaStream_t s) {
+  const int64_t rows = int64_t(P.batch) * P.tokens;
+  const int heads = P.hq + P.hkv;
+  const int64_t wide = rows * ((heads + kRopeRows - 1) / kRopeRows);
+  if (wide >= 148 * 16) {
+    P.n_units = wide;
+    norm_rope_kernel<T, kRopeRows><<<unsigned((wide + 15) / 16), 256, 0, s>>>(P);
+  } else {
+    P.n_units = rows * heads;
+    norm_rope_kernel<T, 1><<<unsigned((P.n_units + 3) / 4), 64, 0, s>>>(P);
+  }
+}
+
+// Rows on boundaries of four elements, as the kernel's words need.
+static int check_rows(const void* p, const int64_t* strides, const tp_rope_layout& L, int heads, const char* what) {
+  const int bytes = L.dtype == TP_F32 ? 16 : 8;
+  if (!p) return fail(TP_ERR_INVALID, std::string("tp_norm_rope: NULL ") + what);
+  const bool odd = (L.batch > 1 && strides[0] % 4) || (L.tokens > 1 && strides[1] % 4) || (heads > 1 && strides[2] % 4);
+  if (uintptr_t(p) % bytes || odd)
+    return fail(TP_ERR_INVALID, std::string("tp_norm_rope: rows of ") + what + " must start on boundaries of 4 elements");
+  return TP_OK;
+}
+
+static RopeSide rope_side(const void* in, void* out, const void* weight, const int64_t* si, const int64_t* so) {
+  return RopeSide{in, out, weight, si[0], si[1], si[2], so[0], so[1], so[2]};
+}
+
+}  // namespace tp
+
+using namespace tp;
+
+extern "C" int tp_norm_rope(const tp_rope_layout* layout, const void* q, const void* k, const void* q_weight,
+                            const void* k_weight, const void* cos, const void* sin, const void* positions, void* q_out,
+                            void* k_out, void* stream) {
+  if (!layout) return fail(TP_ERR_INVALID, "tp_norm_rope: NULL layout");
+  const tp_rope_layout& L = *layout;
+  auto known = [](int d) { return d == TP_F16 || d == TP_F32 || d == TP_BF16; };
+  if (!known(L.dtype) || !known(L.weight_dtype) || !known(L.table_dtype))
+    return fail(TP_ERR_INVALID, "tp_norm_rope: dtype must be float16, bfloat16 or float32");
+  if (L.batch < 0 || L.tokens < 0) return fail(TP_ERR_INVALID, "tp_norm_rope: negative size");
+  if (L.q_heads < 1 || L.k_heads < 1)
+    return fail(TP_ERR_INVALID, "tp_norm_rope: q and k need at least one head each");
+  if (L.batch == 0 || L.tokens == 0) return TP_OK;
+  int st = check_rows(q, L.q_in, L, L.q_heads, "q");
+  if (st == TP_OK) st = check_rows(k, L.k_in, L, L.k_heads, "k");
+  if (st == TP_OK) st = check_rows(q_out, L.q_out, L, L.q_heads, "q_out");
+  if (st == TP_OK) st = check_rows(k_out, L.k_out, L, L.k_heads, "k_out");
+  if (st != TP_OK) return st;
+  if (!cos || !sin) return fail(TP_ERR_INVALID, "tp_norm_rope: NULL angle table");
+  if (L.table_rows < 0 || (L.table_rows > 1 && L.row_stride < 64))
+    return fail(TP_ERR_INVALID, "tp_norm_rope: angle rows must be at least 64 elements apart");
+  if (!positions && int64_t(L.batch_rows) * (L.batch - 1) + L.tokens > L.table_rows)
+    return fail(TP_ERR_INVALID, "tp_norm_rope: the angle table has fewer rows than tokens");
+  const int64_t heads = int64_t(L.q_heads) + L.k_heads, tokens = int64_t(L.batch) * L.tokens;
+  if (heads > (1 << 20) || tokens > (int64_t(1) << 32) / heads)
+    return fail(TP_ERR_INVALID, "tp_norm_rope: more than 2^32 rows");
+  RopeParams P;
+  P.q = rope_side(q, q_out, q_weight, L.q_in, L.q_out);
+  P.k = rope_side(k, k_out, k_weight, L.k_in, L.k_out);
+  P.cos = cos;
+  P.sin = sin;
+  P.positions = positions;
+  P.table_stride = L.row_stride;
+  P.pos_b = L.pos_strides[0];
+  P.pos_t = L.pos_strides[1];
+  P.batch = L.batch;
+  P.tokens = L.tokens;
+  P.hq = L.q_heads;
+  P.hkv = L.k_heads;
+  P.table_rows = L.table_rows;
+  P.table_b_rows = L.batch_rows;
+  P.pos64 = L.pos64;
+  P.table_dtype = L.table_dtype;
+  P.weight_dtype = L.weight_dtype;
+  P.interleaved = L.interleaved;
+  P.eps = L.eps;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (L.dtype == TP_F16) launch_rope<__half>(P, s);
+  else if (L.dtype == TP_BF16) launch_rope<__nv_bfloat16>(P, s);
+  else launch_rope<float>(P, s);
+  return check_launch("tp_norm_rope");
+}
