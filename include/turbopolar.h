@@ -335,6 +335,37 @@ int tp_norm_rope(const tp_rope_layout* layout, const void* q, const void* k, con
                  const void* k_weight, const void* cos, const void* sin, const void* positions,
                  void* q_out, void* k_out, void* stream);
 
+/* Work list of prompt attention over sequences of given lengths, made once on the host and used by
+ * every layer.  tp_prompt_plan_make fills `plan`; with `words` non-NULL it also writes plan->words
+ * 32-bit words, which the caller copies to device memory.  Row a of a sequence of q_len queries and
+ * k_len keys sees keys j <= a + k_len - q_len: with q_len = k_len a prompt, with q_len < k_len the
+ * last rows of a longer history (one row: a decode step); rows with q_len > k_len may see nothing. */
+typedef struct tp_prompt_plan {
+  int32_t num_q_heads, num_kv_heads;
+  int64_t q_tokens, k_tokens;       /* sums of the lengths */
+  int32_t items, merges, block_tokens;
+  size_t words, workspace_bytes;
+} tp_prompt_plan;
+int tp_prompt_plan_make(const int64_t* q_lens, const int64_t* k_lens, int32_t n_seqs, int32_t num_q_heads,
+                        int32_t num_kv_heads, tp_prompt_plan* plan, int32_t* words, size_t n_words);
+
+/* Packed rows: token t, head h at t * x[0] + h * x[1] elements, 128 contiguous channels; 16-byte
+ * aligned rows. */
+typedef struct tp_prompt_rows {
+  int64_t q[2], k[2], v[2];
+  int32_t dtype; /* TP_F16 or TP_BF16 */
+} tp_prompt_rows;
+
+/* Causal attention of packed sequences: out[t][hq][:] = softmax_j(scale * q[t][hq] . k[j][hq / G]) @ v
+ * over the keys that row t sees (a row that sees none gives 0), out [q_tokens][H_q][128] of the
+ * inputs' type.  Replaces the dense attention that the reference's adapter runs for prompts
+ * (benchmarks/turbopolar_fast_attention.py:56-86 feeds it).  A masked key never changes a row,
+ * whatever it holds.  workspace: plan->workspace_bytes, not shared by calls that may overlap; word 0
+ * is set to 1 when a wait ran out (the output is then unusable) and never cleared. */
+int tp_prompt_attention(const tp_prompt_plan* plan, const int32_t* words, const tp_prompt_rows* rows,
+                        const void* q, const void* k, const void* v, float scale, void* out, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
 /* Message of the last failed call on this thread ("" if none). */
 const char* tp_last_error(void);
 

@@ -24,7 +24,7 @@ EXPORTED = (
     "tp_export_pages", "tp_import_pages", "tp_last_error", "tp_version",
     "tp_exchange_bytes", "tp_ipc_alloc", "tp_ipc_open", "tp_ipc_close", "tp_ipc_free",
     "tp_decode_attention_sharded", "tp_decode_step_sharded",
-    "tp_norm_rope",
+    "tp_norm_rope", "tp_prompt_plan_make", "tp_prompt_attention",
 )
 MAX_RANKS = 8
 
@@ -82,6 +82,19 @@ class RopeLayout(ctypes.Structure):
                 ("batch_rows", ctypes.c_int32), ("pos64", ctypes.c_int32), ("eps", ctypes.c_float)]
 
 
+class PromptPlan(ctypes.Structure):
+    """tp_prompt_plan: the sizes of a prompt-attention work list."""
+    _fields_ = [("num_q_heads", ctypes.c_int32), ("num_kv_heads", ctypes.c_int32), ("q_tokens", ctypes.c_int64),
+                ("k_tokens", ctypes.c_int64), ("items", ctypes.c_int32), ("merges", ctypes.c_int32),
+                ("block_tokens", ctypes.c_int32), ("words", ctypes.c_size_t), ("workspace_bytes", ctypes.c_size_t)]
+
+
+class PromptRows(ctypes.Structure):
+    """tp_prompt_rows: token and head strides of packed q, k and v, and their type."""
+    _fields_ = [("q", ctypes.c_int64 * 2), ("k", ctypes.c_int64 * 2), ("v", ctypes.c_int64 * 2),
+                ("dtype", ctypes.c_int32)]
+
+
 _lib = None
 _lock = threading.Lock()
 
@@ -118,6 +131,9 @@ def _declare(lib):
         "tp_decode_step_sharded": (ctypes.c_int, [ctypes.POINTER(PagePool), ctypes.POINTER(Tail), P, P, P, I32, I64, P,
                                                   I32, I32, F, P, ctypes.POINTER(Exchange), P, SZ, P]),
         "tp_norm_rope": (ctypes.c_int, [ctypes.POINTER(RopeLayout), P, P, P, P, P, P, P, P, P, P]),
+        "tp_prompt_plan_make": (ctypes.c_int, [P, P, I32, I32, I32, ctypes.POINTER(PromptPlan), P, SZ]),
+        "tp_prompt_attention": (ctypes.c_int, [ctypes.POINTER(PromptPlan), P, ctypes.POINTER(PromptRows), P, P, P, F,
+                                               P, P, SZ, P]),
         "tp_last_error": (ctypes.c_char_p, []),
         "tp_version": (ctypes.c_int, []),
     }

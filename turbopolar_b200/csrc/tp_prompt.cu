@@ -1,0 +1,575 @@
+// Causal attention of packed sequences with grouped query heads (prompts, prompt chunks over a
+// history, single tokens over a history), dense keys and values.
+//
+//   out[t][h] = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q[t][h] . k_j),  j <= t + k_len - q_len
+//
+// One CTA takes one work item: one KV head, one or two tiles of 128 query rows, a range of keys.  A
+// tile's rows are 128 / G tokens times the G query heads of the KV head, so the group's heads read
+// each key tile once and a single token fills G rows.  Four products per key tile (two tiles, Q K^T and P V)
+// run on the tensor cores while the two softmax warpgroups work on each other's turn: the
+// scores of one tile are being made while the weights of the other are.
+//
+//   warps 0-3, 4-7   softmax of tile 0 / 1, one row per thread; output of the rows
+//   warp 8           issues the products
+//   warp 9           loads tiles (TMA) into a ring of five 32 KB stages: K0 V0 K1 V1 ...
+//   warps 10, 11     complete the warpgroup (registers are moved per warpgroup)
+//
+// Values that no row may see: keys past the item's range in its last tile belong to another
+// sequence, and a masked weight of 0 times an infinity or NaN is NaN.  The loader clears such rows
+// of the last tile, and in tiles that some row sees only part of it also clears rows with
+// non-finite values and lists them; rows that do see a listed key add it at the end.
+//
+// Long key ranges with few query rows are split into several items; their unnormalised rows are merged by
+// merge_items_kernel.
+#include <cuda_bf16.h>
+
+#include <algorithm>
+#include <string>
+#include <vector>
+
+#include "tp_umma.cuh"
+
+namespace tp {
+
+constexpr int kKeys = 128;               // keys per tile
+constexpr int kRing = 5;                 // K and V tiles in flight
+constexpr int kMaxLate = 384;            // keys of the partly visible tiles of one item: 127 + 255 at most
+// Three warpgroups at 168 registers: 504 in all, of which the softmax threads, with a row of scores
+// each, take 208 and the others 88.
+constexpr int kPromptThreads = 384, kSoftmaxRegs = 208, kIssueRegs = 88;
+constexpr int kPromptBars = 2 * kTileBytes + kRing * kTileBytes;  // byte offset of the barriers
+constexpr int kPromptSmem = kPromptBars + 256 + 2 * kMaxLate;
+constexpr int kRecordRows = 2 * kTile;   // rows of an item's partial record
+
+// One work item (eight words, made on the host and copied to the device).
+struct PromptItem {
+  int32_t q_row;     // first token in the packed queries
+  int32_t q_tokens;  // tokens, at most two tiles' worth
+  int32_t sees;      // keys of its sequence that the first token sees (may be <= 0); one more for each next
+  int32_t k_row;     // the sequence's first key in the packed keys
+  int32_t k_begin, k_end;  // this item's keys, relative to k_row
+  int32_t slot;      // record of an item that is merged later, or -1
+  int32_t pad;
+};
+// The records of one token block that was split: `n` of them from `slot`.
+struct PromptMerge {
+  int32_t q_row, q_tokens, slot, n;
+};
+
+struct PromptParams {
+  CUtensorMap qmap, kmap, vmap;
+  const PromptItem* items;
+  const PromptMerge* merges;
+  int hq, hkv, group, tile_tokens;
+  float scale_log2;
+  const uint16_t *q, *k, *v;  // for listed keys
+  int64_t q_t, q_h, k_t, k_h, v_t, v_h;
+  uint16_t* out;              // [tokens][hq][128]
+  float* rec_o;               // [slot][hkv][256][128]
+  float2* rec_ml;             // [slot][hkv][256]
+  int* error;
+};
+
+template <bool kBf16>
+__device__ __forceinline__ float widen(uint16_t u) {
+  return kBf16 ? __uint_as_float(uint32_t(u) << 16) : __half2float(__ushort_as_half(u));
+}
+template <bool kBf16>
+__device__ __forceinline__ bool not_finite(uint32_t w) {  // either 16-bit number of w
+  const uint32_t e = kBf16 ? 0x7f807f80u : 0x7c007c00u, x = w & e;
+  return (x & 0xffff0000u) == (e & 0xffff0000u) || (x & 0xffffu) == (e & 0xffffu);
+}
+
+// Clear rows >= `valid` of a value tile; with `scan` also rows that hold a non-finite value, whose
+// places (first + row) are added to the list.  One warp.
+template <bool kBf16>
+__device__ void clean_values(uint8_t* tile, int valid, bool scan, int first, uint16_t* late, int* n_late) {
+  const int lane = threadIdx.x & 31;
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  uint32_t bad[4] = {0, 0, 0, 0};  // rows, the same in every lane
+#pragma unroll
+  for (int part = 0; part < 8; ++part) {  // 16 KB halves x groups of 32 rows; four rows per step
+#pragma unroll 4
+    for (int it = 0; it < 8; ++it) {
+      uint4* p = reinterpret_cast<uint4*>(tile) + (part * 8 + it) * 32 + lane;
+      const int row = (part & 3) * 32 + it * 4 + (lane >> 3);
+      bool hit = false;
+      if (row >= valid) {
+        *p = zero;
+      } else if (scan) {
+        const uint4 x = *p;
+        hit = not_finite<kBf16>(x.x) || not_finite<kBf16>(x.y) || not_finite<kBf16>(x.z) || not_finite<kBf16>(x.w);
+      }
+      const uint32_t hits = __ballot_sync(0xffffffffu, hit);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (hits >> (8 * i) & 0xffu) bad[part & 3] |= 1u << (it * 4 + i);
+    }
+  }
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    while (bad[w]) {
+      const int row = w * 32 + __ffs(bad[w]) - 1;
+      bad[w] &= bad[w] - 1;
+      if (lane < 16) *reinterpret_cast<uint4*>(tile + (lane >> 3) * kHalfTile + row * 128 + (lane & 7) * 16) = zero;
+      if (lane == 0) late[(*n_late)++] = uint16_t(first + row);
+    }
+  }
+}
+
+template <bool kBf16>
+__global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(const __grid_constant__ PromptParams P) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const PromptItem it = P.items[blockIdx.x / P.hkv];
+  const int kvh = blockIdx.x % P.hkv;
+  uint8_t* ring = smem + 2 * kTileBytes;
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + kPromptBars);
+  uint64_t *full = q_full + 1, *empty = full + kRing, *s_full = empty + kRing, *p_full = s_full + 2,
+           *o_done = p_full + 2, *clean = o_done + 2, *drained = clean + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
+  int* stop_word = reinterpret_cast<int*>(tmem_slot + 1);
+  volatile int* stop = stop_word;
+  int* n_late = stop_word + 1;
+  uint16_t* late = reinterpret_cast<uint16_t*>(smem + kPromptBars + 256);
+
+  const int n_tiles = (it.k_end - it.k_begin + kKeys - 1) / kKeys;
+  const bool two = it.q_tokens > P.tile_tokens;
+  // Tiles from `partial` on are not seen whole by every row (or end after the item's keys).
+  const int whole = min(it.sees, it.k_end) - it.k_begin;
+  const int partial = whole <= 0 ? 0 : whole / kKeys;
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    for (int i = 0; i < kRing; ++i) {
+      mbar_init(full + i, 1);
+      mbar_init(empty + i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(s_full + i, 1);
+      mbar_init(p_full + i, 4);
+      mbar_init(o_done + i, 1);
+    }
+    mbar_init(clean, 1);
+    mbar_init(drained, 1);
+    *stop = 0;
+    *n_late = 0;
+    fence_mbar_init();
+  }
+  if (warp == 8) tmem_alloc(tmem_slot, 512);
+  tmem_fence_before();
+  __syncthreads();
+  tmem_fence_after();
+  const uint32_t tmem = *tmem_slot;  // scores of tile t: columns 128 t; accumulator: 256 + 128 t
+
+  if (warp < 8) {
+    more_registers<kSoftmaxRegs>();
+    const int t = warp >> 2;
+    const int r = (warp & 3) * 32 + lane;
+    const int tok = t * P.tile_tokens + r / P.group, head = kvh * P.group + r % P.group;
+    const bool valid = r < P.tile_tokens * P.group && tok < it.q_tokens;
+    const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
+    const uint32_t s_addr = tmem + 128 * t + lanes, o_addr = tmem + 256 + 128 * t + lanes;
+    // Rows that are not there see everything, so they ask for no masking; they are not written.
+    const int limit = valid ? min(it.sees + tok, it.k_end) : it.k_end;
+    const bool live = __any_sync(0xffffffffu, valid);
+    SoftmaxRow row;
+    bool ok = true;
+    if (t == 0 || two) {
+      for (int j = 0; j < n_tiles && ok; ++j) {
+        ok = __all_sync(0xffffffffu, wait_bar(s_full + t, j & 1, stop));
+        if (ok && live) {
+          tmem_fence_after();
+          ok = softmax_tile<kKeys, kBf16>(row, s_addr, o_addr, limit - (it.k_begin + j * kKeys), P.scale_log2, j == 0,
+                                          [&] { return wait_bar(o_done + t, (j - 1) & 1, stop); });
+          tmem_fence_before();
+        }
+        __syncwarp();
+        if (ok && lane == 0) mbar_arrive(p_full + t);
+      }
+      if (ok && n_tiles) {
+        ok = wait_bar(o_done + t, (n_tiles - 1) & 1, stop);
+        if (partial < n_tiles) ok = ok && wait_bar(clean, (n_tiles - partial - 1) & 1, stop);
+        ok = __all_sync(0xffffffffu, ok);
+        tmem_fence_after();
+      }
+      if (ok && live) {
+        const int listed = n_tiles ? *n_late : 0;
+        const bool merged = it.slot >= 0;
+        const int64_t q_row = int64_t(it.q_row) + tok;
+        const int64_t rec = (int64_t(it.slot) * P.hkv + kvh) * kRecordRows + t * kTile + r;
+        const float inv = merged ? 1.0f : row.sum == 0.0f ? 0.0f : 1.0f / row.sum;
+#pragma unroll
+        for (int c = 0; c < kD; c += 32) {
+          float o[32];
+          if (n_tiles) {
+            tmem_ld32(o_addr + c, o);
+            tmem_wait_ld<32>(o);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = 0.0f;
+          }
+          if (!valid) continue;
+          for (int e = 0; e < listed; ++e) {  // keys with non-finite values that this row sees
+            const int key = it.k_begin + partial * kKeys + late[e];
+            if (key >= limit) continue;
+            const uint16_t* qr = P.q + q_row * P.q_t + head * P.q_h;
+            const uint16_t* kr = P.k + (int64_t(it.k_row) + key) * P.k_t + kvh * P.k_h;
+            const uint16_t* vr = P.v + (int64_t(it.k_row) + key) * P.v_t + kvh * P.v_h;
+            float dot = 0.0f;
+            for (int d = 0; d < kD; ++d) dot = fmaf(widen<kBf16>(qr[d]), widen<kBf16>(kr[d]), dot);
+            const float p = exp2_approx(fmaf(dot, P.scale_log2, -row.ref));
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = fmaf(p, widen<kBf16>(vr[c + i]), o[i]);
+          }
+          if (merged) {
+            float4* dst = reinterpret_cast<float4*>(P.rec_o + rec * kD + c);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          } else {
+            uint4* dst = reinterpret_cast<uint4*>(P.out + (q_row * P.hq + head) * kD + c);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              dst[i] = make_uint4(pack2<kBf16>(o[8 * i] * inv, o[8 * i + 1] * inv),
+                                  pack2<kBf16>(o[8 * i + 2] * inv, o[8 * i + 3] * inv),
+                                  pack2<kBf16>(o[8 * i + 4] * inv, o[8 * i + 5] * inv),
+                                  pack2<kBf16>(o[8 * i + 6] * inv, o[8 * i + 7] * inv));
+          }
+        }
+        if (merged && valid) P.rec_ml[rec] = make_float2(row.ref, row.sum);
+      }
+    }
+    tmem_fence_before();
+  } else if (fewer_registers<kIssueRegs>(); warp == 8) {
+    if (lane == 0 && n_tiles) {
+      constexpr uint32_t kScores = mma_idesc(kBf16, kKeys, false), kOut = mma_idesc(kBf16, kD, true);
+      const uint32_t q_addr = smem_u32(smem), ring_addr = smem_u32(ring);
+      const int nt = two ? 2 : 1;
+      auto scores = [&](int t, int stage) {
+#pragma unroll
+        for (int ks = 0; ks < kD / 16; ++ks) {
+          const uint32_t off = (ks >> 2) * kHalfTile + (ks & 3) * 32;
+          mma_ss(tmem + 128 * t, rows_desc(q_addr + t * kTileBytes + off), rows_desc(ring_addr + stage * kTileBytes + off),
+                 kScores, ks > 0);
+        }
+        mma_commit(s_full + t);
+      };
+      bool ok = wait_bar(q_full, 0, stop) && wait_bar(full, 0, stop);
+      if (ok) {
+        tmem_fence_after();
+        for (int t = 0; t < nt; ++t) scores(t, 0);
+        mma_commit(empty);
+      }
+      for (int j = 0; j < n_tiles && ok; ++j) {
+        const int iv = 2 * j + 1, sv = iv % kRing, ik = iv + 1, sk = ik % kRing;
+        ok = wait_bar(full + sv, (iv / kRing) & 1, stop);
+        if (ok && j >= partial) ok = wait_bar(clean, (j - partial) & 1, stop);
+        if (ok && j + 1 < n_tiles) ok = wait_bar(full + sk, (ik / kRing) & 1, stop);
+        for (int t = 0; t < nt && ok; ++t) {
+          ok = wait_bar(p_full + t, j & 1, stop);
+          if (!ok) break;
+          tmem_fence_after();
+#pragma unroll
+          for (int ks = 0; ks < kKeys / 16; ++ks)
+            mma_ts(tmem + 256 + 128 * t, tmem + 128 * t + ks * 8,
+                   cols_desc(ring_addr + sv * kTileBytes + ks * 2048, kHalfTile), kOut, j > 0 || ks > 0);
+          mma_commit(o_done + t);
+          if (t == nt - 1) mma_commit(empty + sv);
+          if (j + 1 < n_tiles) scores(t, sk);
+        }
+        if (ok && j + 1 < n_tiles) mma_commit(empty + sk);
+      }
+      mma_commit(drained);
+      drain_bar(drained, 0);
+    }
+    __syncwarp();
+  } else if (warp == 9 && n_tiles) {
+    const int nt = two ? 2 : 1;
+    if (lane == 0) {
+      mbar_arrive_expect_tx(q_full, uint32_t(nt * P.tile_tokens * P.group * 256));
+      for (int t = 0; t < nt; ++t)
+        for (int h = 0; h < 2; ++h)
+          tma_tile_3d(smem_u32(smem) + t * kTileBytes + h * kHalfTile, &P.qmap, h * 64, kvh * P.group,
+                      it.q_row + t * P.tile_tokens, q_full);
+    }
+    int issued = 0, wanted = -1;  // wanted: a value tile to be cleaned
+    bool ok = true;
+    auto clean_one = [&](int i) {
+      const int stage = i % kRing, key = (i >> 1) * kKeys;
+      if (!wait_bar(full + stage, (i / kRing) & 1, stop)) return false;
+      clean_values<kBf16>(ring + stage * kTileBytes, it.k_end - it.k_begin - key, it.q_tokens > 1, key - partial * kKeys,
+                          late, n_late);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(clean);
+      return true;
+    };
+    for (int i = 0; i < 2 * n_tiles && ok; ++i) {
+      const int stage = i % kRing, use = i / kRing;
+      ok = use == 0 || wait_bar(empty + stage, (use - 1) & 1, stop);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      if (lane == 0) {
+        const uint32_t dst = smem_u32(ring) + stage * kTileBytes;
+        const CUtensorMap* map = i & 1 ? &P.vmap : &P.kmap;
+        mbar_arrive_expect_tx(full + stage, kTileBytes);
+        for (int h = 0; h < 2; ++h)
+          tma_tile_3d(dst + h * kHalfTile, map, h * 64, kvh, it.k_row + it.k_begin + (i >> 1) * kKeys, full + stage);
+      }
+      issued = i + 1;
+      if (wanted >= 0) {  // after the next tile's load is under way
+        ok = __all_sync(0xffffffffu, clean_one(wanted));
+        wanted = -1;
+      }
+      if ((i & 1) && (i >> 1) >= partial) wanted = i;
+    }
+    if (ok && wanted >= 0) clean_one(wanted);
+    // No copy may be in flight when the CTA ends.
+    drain_bar(q_full, 0);
+    for (int i = max(0, issued - kRing); i < issued; ++i) drain_bar(full + i % kRing, (i / kRing) & 1);
+  }
+  __syncthreads();
+  if (warp == 8) {
+    tmem_fence_after();
+    tmem_free(tmem, 512);
+  }
+  if (threadIdx.x == 0 && *stop) *P.error = 1;
+}
+
+// Rows of a split token block: with records (ref_i, l_i, o_i), M = max ref_i and w_i = 2^(ref_i - M),
+// out = sum w_i o_i / sum w_i l_i (0 where no record has seen a key).  One warp per row.
+template <bool kBf16>
+__global__ void __launch_bounds__(256) merge_items_kernel(const __grid_constant__ PromptParams P) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const PromptMerge m = P.merges[blockIdx.x / P.hkv];
+  const int kvh = blockIdx.x % P.hkv;
+  const int i = blockIdx.y * 8 + warp;
+  if (i >= m.q_tokens * P.group) return;
+  const int tok = i / P.group, g = i % P.group;
+  const int t = tok / P.tile_tokens, r = (tok - t * P.tile_tokens) * P.group + g;
+  const int64_t step = int64_t(P.hkv) * kRecordRows;
+  const int64_t rec0 = (int64_t(m.slot) * P.hkv + kvh) * kRecordRows + t * kTile + r;
+  float top = -INFINITY;
+  for (int k = lane; k < m.n; k += 32) top = fmaxf(top, P.rec_ml[rec0 + k * step].x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float base = top == -INFINITY ? 0.0f : top;
+  float l = 0.0f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k = 0; k < m.n; ++k) {
+    const float2 ml = P.rec_ml[rec0 + k * step];
+    const float4 o = *reinterpret_cast<const float4*>(P.rec_o + (rec0 + k * step) * kD + 4 * lane);
+    const float w = exp2_approx(ml.x - base);
+    l = fmaf(w, ml.y, l);
+    acc.x = fmaf(w, o.x, acc.x);
+    acc.y = fmaf(w, o.y, acc.y);
+    acc.z = fmaf(w, o.z, acc.z);
+    acc.w = fmaf(w, o.w, acc.w);
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  uint2* dst = reinterpret_cast<uint2*>(P.out + ((int64_t(m.q_row) + tok) * P.hq + kvh * P.group + g) * kD + 4 * lane);
+  *dst = make_uint2(pack2<kBf16>(acc.x * inv, acc.y * inv), pack2<kBf16>(acc.z * inv, acc.w * inv));
+}
+
+// ----------------------------------------------------------------------------- host
+static int tile_tokens_of(int group) { return kTile / group; }
+
+// Tensor map of rows [tokens][heads][128] of 16-bit numbers, boxes of 64 channels.
+static int rows_map(CUtensorMap* m, const void* p, int64_t tokens, int heads, int64_t t_stride, int64_t h_stride,
+                    int box_heads, int box_tokens, bool bf16, const char* what) {
+  static PFN_cuTensorMapEncodeTiled_v12000 enc = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult found = cudaDriverEntryPointSymbolNotFound;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &found) == cudaSuccess &&
+        found == cudaDriverEntryPointSuccess)
+      enc = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+    else
+      cudaGetLastError();
+  });
+  if (!enc) return fail(TP_ERR_CUDA, "tp_prompt_attention: the driver has no cuTensorMapEncodeTiled");
+  // The stride of an axis of one entry is not used, but has to be a legal one.
+  if (heads == 1) h_stride = kD;
+  if (tokens == 1) t_stride = int64_t(heads) * kD;
+  if (!p || uintptr_t(p) % 16 || t_stride % 8 || h_stride % 8 || t_stride < kD || h_stride < kD)
+    return fail(TP_ERR_INVALID, std::string("tp_prompt_attention: ") + what +
+                                    " rows must be contiguous and start on 16-byte boundaries");
+  const cuuint64_t dims[3] = {cuuint64_t(kD), cuuint64_t(heads), cuuint64_t(tokens)};
+  const cuuint64_t strides[2] = {cuuint64_t(h_stride * 2), cuuint64_t(t_stride * 2)};
+  const cuuint32_t box[3] = {64, cuuint32_t(box_heads), cuuint32_t(box_tokens)};
+  const cuuint32_t step[3] = {1, 1, 1};
+  const CUresult r = enc(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                         const_cast<void*>(p), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(TP_ERR_INVALID, std::string("tp_prompt_attention: cannot describe ") + what + " (CUresult " +
+                                    std::to_string(int(r)) + ")");
+  return TP_OK;
+}
+
+static size_t record_bytes(int64_t slots, int hkv) {
+  return size_t(slots) * hkv * kRecordRows * (kD * sizeof(float) + sizeof(float2));
+}
+
+template <bool kBf16>
+static int launch_prompt(const PromptParams& P, const tp_prompt_plan& plan, cudaStream_t s) {
+  static bool allowed[64] = {};  // the attribute belongs to a device's copy of the kernel
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev >= 64 || !allowed[dev])) {
+    e = cudaFuncSetAttribute(prompt_attention_kernel<kBf16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPromptSmem);
+    if (e == cudaSuccess && dev < 64) allowed[dev] = true;
+  }
+  if (e != cudaSuccess) return fail(TP_ERR_CUDA, std::string("tp_prompt_attention: ") + cudaGetErrorString(e));
+  if (plan.items)
+    prompt_attention_kernel<kBf16><<<unsigned(plan.items) * plan.num_kv_heads, kPromptThreads, kPromptSmem, s>>>(P);
+  if (plan.merges) {
+    const int rows = plan.block_tokens * P.group;
+    merge_items_kernel<kBf16><<<dim3(unsigned(plan.merges) * plan.num_kv_heads, (rows + 7) / 8), 256, 0, s>>>(P);
+  }
+  return check_launch("tp_prompt_attention");
+}
+
+}  // namespace tp
+
+using namespace tp;
+
+extern "C" {
+
+int tp_prompt_plan_make(const int64_t* q_lens, const int64_t* k_lens, int32_t n_seqs, int32_t num_q_heads,
+                        int32_t num_kv_heads, tp_prompt_plan* plan, int32_t* words, size_t n_words) {
+  if (!plan || n_seqs < 0 || (n_seqs && (!q_lens || !k_lens)))
+    return fail(TP_ERR_INVALID, "tp_prompt_plan_make: NULL argument");
+  if (num_kv_heads < 1 || num_q_heads < 1 || num_q_heads % num_kv_heads)
+    return fail(TP_ERR_INVALID, "num_q_heads must be divisible by num_kv_heads for GQA");
+  const int group = num_q_heads / num_kv_heads;
+  if (group > kTile) return fail(TP_ERR_UNSUPPORTED, "tp_prompt_plan_make: more than 128 query heads per KV head");
+  int64_t tq = 0, tk = 0, pairs = 0;
+  const int tile = tile_tokens_of(group);
+  for (int i = 0; i < n_seqs; ++i) {
+    if (q_lens[i] < 0 || k_lens[i] < 0) return fail(TP_ERR_INVALID, "tp_prompt_plan_make: negative length");
+    tq += q_lens[i];
+    tk += k_lens[i];
+    if (tq > INT32_MAX / 2 || tk > INT32_MAX / 2)
+      return fail(TP_ERR_INVALID, "tp_prompt_plan_make: more than 2^30 tokens");
+    pairs += (q_lens[i] + 2 * tile - 1) / (2 * tile);
+  }
+  const int64_t sms = device_sms();
+  // Two tiles per item, which halves the reads of each key tile, unless that leaves SMs idle.
+  const int block = pairs * num_kv_heads >= sms ? 2 * tile : tile;
+  struct Block {
+    int32_t q_row, q_tokens, sees, k_row, k_end, tiles;
+  };
+  std::vector<Block> blocks;
+  int64_t q_row = 0, k_row = 0, work = 0, longest = 0;
+  for (int i = 0; i < n_seqs; ++i) {
+    for (int64_t a = 0; a < q_lens[i]; a += block) {
+      Block b;
+      b.q_row = int32_t(q_row + a);
+      b.q_tokens = int32_t(std::min<int64_t>(block, q_lens[i] - a));
+      b.sees = int32_t(k_lens[i] - q_lens[i] + a + 1);
+      b.k_row = int32_t(k_row);
+      b.k_end = int32_t(std::max<int64_t>(0, int64_t(b.sees) + b.q_tokens - 1));  // at most k_lens[i]
+      b.tiles = (b.k_end + kKeys - 1) / kKeys;
+      work += b.tiles;
+      longest = std::max<int64_t>(longest, b.tiles);
+      blocks.push_back(b);
+    }
+    q_row += q_lens[i];
+    k_row += k_lens[i];
+  }
+  // Key ranges: an item takes about `chunk` tiles.  Fewer blocks than SMs: as many items as fit one
+  // wave, at least four tiles each (a record of 256 rows is written and read for each item).
+  int64_t chunk = std::max<int64_t>(4, (work * num_kv_heads + sms - 1) / sms);
+  auto parts_of = [&](int64_t tiles) { return 2 * tiles > 3 * chunk ? (tiles + chunk - 1) / chunk : int64_t(1); };
+  if (int64_t(blocks.size()) * num_kv_heads < sms) {
+    for (; chunk < longest; ++chunk) {
+      int64_t n = 0;
+      for (const Block& b : blocks) n += parts_of(b.tiles);
+      if (n * num_kv_heads <= sms) break;
+    }
+  }
+  std::vector<PromptItem> items;
+  std::vector<PromptMerge> merges;
+  int64_t slots = 0;
+  for (const Block& b : blocks) {
+    const int64_t parts = parts_of(b.tiles);
+    const int64_t per = (b.tiles + parts - 1) / parts;
+    int32_t n = 0;
+    for (int64_t j = 0; j < std::max<int64_t>(1, b.tiles); j += std::max<int64_t>(1, per), ++n)
+      items.push_back(PromptItem{b.q_row, b.q_tokens, b.sees, b.k_row, int32_t(j * kKeys),
+                                 int32_t(std::min<int64_t>(b.k_end, (j + per) * kKeys)),
+                                 parts > 1 ? int32_t(slots + n) : -1, 0});
+    if (parts > 1) {
+      merges.push_back(PromptMerge{b.q_row, b.q_tokens, int32_t(slots), n});
+      slots += n;
+    }
+  }
+  // Longest items first: the CTAs are started in this order, so short ones fill the end.
+  std::stable_sort(items.begin(), items.end(), [](const PromptItem& a, const PromptItem& b) {
+    return (a.k_end - a.k_begin + kKeys - 1) / kKeys > (b.k_end - b.k_begin + kKeys - 1) / kKeys;
+  });
+  if (int64_t(items.size()) * num_kv_heads > INT32_MAX || slots > INT32_MAX / 2)
+    return fail(TP_ERR_UNSUPPORTED, "tp_prompt_plan_make: too many work items");
+  plan->num_q_heads = num_q_heads;
+  plan->num_kv_heads = num_kv_heads;
+  plan->q_tokens = tq;
+  plan->k_tokens = tk;
+  plan->items = int32_t(items.size());
+  plan->merges = int32_t(merges.size());
+  plan->block_tokens = block;
+  plan->words = items.size() * (sizeof(PromptItem) / 4) + merges.size() * (sizeof(PromptMerge) / 4);
+  plan->workspace_bytes = 256 + record_bytes(slots, num_kv_heads);
+  if (!words) return TP_OK;
+  if (n_words < plan->words) return fail(TP_ERR_INVALID, "tp_prompt_plan_make: the word buffer is too small");
+  std::copy_n(reinterpret_cast<const int32_t*>(items.data()), items.size() * (sizeof(PromptItem) / 4), words);
+  std::copy_n(reinterpret_cast<const int32_t*>(merges.data()), merges.size() * (sizeof(PromptMerge) / 4),
+              words + items.size() * (sizeof(PromptItem) / 4));
+  return TP_OK;
+}
+
+int tp_prompt_attention(const tp_prompt_plan* plan, const int32_t* words, const tp_prompt_rows* rows, const void* q,
+                        const void* k, const void* v, float scale, void* out, void* workspace, size_t workspace_bytes,
+                        void* stream) {
+  if (!plan || !rows) return fail(TP_ERR_INVALID, "tp_prompt_attention: NULL argument");
+  if (rows->dtype != TP_F16 && rows->dtype != TP_BF16)
+    return fail(TP_ERR_INVALID, "tp_prompt_attention: q, k and v must be float16 or bfloat16");
+  if (!(scale > 0.f) || !(scale < 1e30f)) return fail(TP_ERR_INVALID, "attention scale must be positive");
+  if (plan->q_tokens == 0) return TP_OK;
+  if (!words || !q || !out) return fail(TP_ERR_INVALID, "tp_prompt_attention: NULL argument");
+  if (uintptr_t(out) % 16) return fail(TP_ERR_INVALID, "tp_prompt_attention: out must be 16-byte aligned");
+  if (!workspace || workspace_bytes < plan->workspace_bytes)
+    return fail(TP_ERR_INVALID, "tp_prompt_attention: workspace too small (need " +
+                                    std::to_string(plan->workspace_bytes) + " bytes)");
+  const bool bf16 = rows->dtype == TP_BF16;
+  PromptParams P;
+  P.hq = plan->num_q_heads;
+  P.hkv = plan->num_kv_heads;
+  P.group = P.hq / P.hkv;
+  P.tile_tokens = tile_tokens_of(P.group);
+  int st = rows_map(&P.qmap, q, plan->q_tokens, P.hq, rows->q[0], rows->q[1], P.group, P.tile_tokens, bf16, "q");
+  // Without keys nothing is loaded and the maps are not read.
+  if (st == TP_OK && plan->k_tokens)
+    st = rows_map(&P.kmap, k, plan->k_tokens, P.hkv, rows->k[0], rows->k[1], 1, kKeys, bf16, "k");
+  if (st == TP_OK && plan->k_tokens)
+    st = rows_map(&P.vmap, v, plan->k_tokens, P.hkv, rows->v[0], rows->v[1], 1, kKeys, bf16, "v");
+  if (st != TP_OK) return st;
+  P.items = reinterpret_cast<const PromptItem*>(words);
+  P.merges = reinterpret_cast<const PromptMerge*>(P.items + plan->items);
+  P.scale_log2 = scale * 1.4426950408889634f;
+  P.q = static_cast<const uint16_t*>(q);
+  P.k = static_cast<const uint16_t*>(k);
+  P.v = static_cast<const uint16_t*>(v);
+  P.q_t = rows->q[0], P.q_h = rows->q[1], P.k_t = rows->k[0], P.k_h = rows->k[1], P.v_t = rows->v[0], P.v_h = rows->v[1];
+  P.out = static_cast<uint16_t*>(out);
+  P.error = static_cast<int*>(workspace);
+  P.rec_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + 256);
+  const size_t slots_rows = (plan->workspace_bytes - 256) / (kD * sizeof(float) + sizeof(float2));
+  P.rec_ml = reinterpret_cast<float2*>(P.rec_o + slots_rows * kD);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return bf16 ? launch_prompt<true>(P, *plan, s) : launch_prompt<false>(P, *plan, s);
+}
+
+}  // extern "C"

@@ -1,0 +1,278 @@
+// 5th-generation tensor-core building blocks of the many-query attention kernels: shared-memory
+// and instruction descriptors, tcgen05 products and tensor-memory moves, bounded barrier waits.
+//
+// Both kernels hold 128 query rows per tile.  A row is one tensor-memory lane, so a softmax thread
+// owns a whole row and the running maximum and sum need no exchange between threads.
+//   S = Q K^T   Q, K: [rows][128] 16-bit in shared memory, two halves of 64 channels, each row 128
+//               bytes with the 128-byte XOR swizzle; float32 scores in tensor memory
+//   O += P V    P: 16-bit in tensor memory over the scores it was made from; V: [keys][128] in the
+//               layout of K, read with the channels as the leading axis (no transposed copy)
+#pragma once
+
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <cmath>
+#include <mutex>
+
+#include "tp_common.cuh"
+
+namespace tp {
+
+// ----------------------------------------------------------------------------- host side
+inline int device_sms() {
+  static int sms[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {
+    cudaGetLastError();
+    return 148;
+  }
+  if (!sms[dev]) {
+    int n = 0;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) {
+      cudaGetLastError();
+      return 148;
+    }
+    sms[dev] = n;
+  }
+  return sms[dev];
+}
+
+// ----------------------------------------------------------------------------- descriptors
+constexpr int kTile = 128;               // query rows of a tile
+constexpr int kHalfTile = kTile * 128;   // bytes of 128 rows x 64 channels
+constexpr int kTileBytes = 2 * kHalfTile;
+
+// Byte offset of 16-byte chunk c (0..15) of row r in a tile of `rows` rows.
+__device__ __forceinline__ uint32_t tile_chunk(int r, int c, int rows) {
+  return uint32_t((c >> 3) * rows * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+}
+
+// Shared-memory operand descriptor, 128-byte swizzle: bits 0-13 address / 16, 16-29 leading-axis
+// offset / 16, 32-45 stride offset / 16, 46-47 version 1, 61-63 swizzle 2.
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t leading, uint32_t stride) {
+  return uint64_t((addr >> 4) & 0x3fff) | (uint64_t(leading >> 4) << 16) | (uint64_t(stride >> 4) << 32) |
+         (uint64_t(1) << 46) | (uint64_t(2) << 61);
+}
+// Rows of 64 channels, channels contracted: groups of 8 rows are 1024 bytes apart.
+__device__ __forceinline__ uint64_t rows_desc(uint32_t addr) { return smem_desc(addr, 16, 1024); }
+// Rows contracted, channels the output axis: halves of 64 channels `half` bytes apart.
+__device__ __forceinline__ uint64_t cols_desc(uint32_t addr, uint32_t half) { return smem_desc(addr, half, 1024); }
+
+// kind::f16 instruction descriptor, M = 128: float32 accumulator, both operands bf16 or both f16.
+__host__ __device__ constexpr uint32_t mma_idesc(bool bf16, int n, bool b_cols) {
+  return (1u << 4) | (uint32_t(bf16) << 7) | (uint32_t(bf16) << 10) | (uint32_t(b_cols) << 16) |
+         (uint32_t(n >> 3) << 17) | (uint32_t(kTile >> 4) << 24);
+}
+
+// ----------------------------------------------------------------------------- tcgen05
+__device__ __forceinline__ void tmem_alloc(uint32_t* slot, int cols) {  // one warp
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(cols)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+}
+__device__ __forceinline__ void tmem_free(uint32_t addr, int cols) {  // the same warp
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols));
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(uint32_t(add))
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(uint32_t(add))
+      : "memory");
+}
+// Arrive on `bar` once every product issued by this thread so far has completed.
+__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ void tmem_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// 32 columns of this warp's 32 lanes: thread i holds lane i.
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, float* r) {
+  uint32_t* u = reinterpret_cast<uint32_t*>(r);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
+        "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]),
+        "=r"(u[17]), "=r"(u[18]), "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]),
+        "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
+      : "r"(addr));
+}
+// The registers of the loads above are valid after the wait; naming them as operands keeps the compiler
+// from moving their uses before it.
+__device__ __forceinline__ void after_wait32(float* r) {
+  asm volatile(""
+      : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]),
+        "+f"(r[8]), "+f"(r[9]), "+f"(r[10]), "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15]),
+        "+f"(r[16]), "+f"(r[17]), "+f"(r[18]), "+f"(r[19]), "+f"(r[20]), "+f"(r[21]), "+f"(r[22]), "+f"(r[23]),
+        "+f"(r[24]), "+f"(r[25]), "+f"(r[26]), "+f"(r[27]), "+f"(r[28]), "+f"(r[29]), "+f"(r[30]), "+f"(r[31]));
+}
+template <int kCols>
+__device__ __forceinline__ void tmem_wait_ld(float* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int c = 0; c < kCols; c += 32) after_wait32(r + c);
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* u) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
+      "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(u[0]),
+      "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]), "r"(u[10]),
+      "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15]), "r"(u[16]), "r"(u[17]), "r"(u[18]), "r"(u[19]),
+      "r"(u[20]), "r"(u[21]), "r"(u[22]), "r"(u[23]), "r"(u[24]), "r"(u[25]), "r"(u[26]), "r"(u[27]), "r"(u[28]),
+      "r"(u[29]), "r"(u[30]), "r"(u[31]), "r"(addr)
+      : "memory");
+}
+
+// Tiled 3-D tensor copy global -> shared memory at element coordinates (x, y, z).
+__device__ __forceinline__ void tma_tile_3d(uint32_t dst, const void* tmap, int x, int y, int z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n" ::
+          "r"(dst),
+      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// ----------------------------------------------------------------------------- bounded waits
+constexpr long long kWaitCycles = 2000000000ll;  // about a second
+
+// Wait for phase `parity` of `bar`.  False once the CTA has given up (`stop` set by any thread's
+// wait that ran out): the caller leaves its loop.
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int* stop) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (!mbar_try_wait(bar, parity)) {
+    if (*stop) return false;
+    if (clock64() - t0 > kWaitCycles) {
+      *stop = 1;
+      return false;
+    }
+  }
+  return true;
+}
+// The same without giving up early, to drain copies and products in flight.
+__device__ __forceinline__ void drain_bar(uint64_t* bar, uint32_t parity) {
+  const long long t0 = clock64();
+  while (!mbar_try_wait(bar, parity) && clock64() - t0 < kWaitCycles) {
+  }
+}
+
+__device__ __forceinline__ uint32_t pack_bf2(float a, float b) {
+  uint32_t d;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(b), "f"(a));
+  return d;
+}
+template <bool kBf16>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  return kBf16 ? pack_bf2(a, b) : pack_h2(a, b);
+}
+
+// Registers per thread of this warpgroup from here on (every warp of it executes this).
+template <int kRegs>
+__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs)); }
+template <int kRegs>
+__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs)); }
+
+// ----------------------------------------------------------------------------- softmax of one row
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {  // two float32 each
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ void split_pair(uint64_t p, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
+}
+
+// The running softmax of a row: weights are 2^(s * scale_log2 - ref) with a reference that is at
+// least the row's maximum so far minus 8.  It moves only when a maximum exceeds it by more than 8:
+// weights up to 2^8 lose nothing in 16 bits, and the output accumulator, which lives in tensor
+// memory, is rescaled a few times per row instead of once per tile.
+constexpr float kRefSlack = 8.0f;
+struct SoftmaxRow {
+  float ref = -INFINITY;  // nothing seen yet
+  float sum = 0.0f;
+};
+
+// One tile of kCols scores of this thread's row, in tensor memory at `s_addr` (the warp's lanes):
+// columns >= `visible` are masked (whatever they hold, NaN included).  Writes the 16-bit weights over the
+// scores.  `o_addr`: the row's 128 accumulator columns, rescaled when the reference moves;
+// `before_rescale()` waits until the products issued so far have completed (false: given up) and
+// is not called for the first tile, when the accumulator holds nothing.
+template <int kCols, bool kBf16, class Wait>
+__device__ __forceinline__ bool softmax_tile(SoftmaxRow& row, uint32_t s_addr, uint32_t o_addr, int visible,
+                                             float scale_log2, bool first, Wait before_rescale) {
+  float s[kCols];
+#pragma unroll
+  for (int c = 0; c < kCols; c += 32) tmem_ld32(s_addr + c, s + c);
+  tmem_wait_ld<kCols>(s);
+  if (__any_sync(0xffffffffu, visible < kCols)) {
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) s[c] = c < visible ? s[c] : -INFINITY;
+  }
+  float top[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+  for (int c = 4; c < kCols; c += 8) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top[i] = fmaxf(fmaxf(top[i], s[c + i]), c + 4 + i < kCols ? s[c + 4 + i] : top[i]);
+  }
+  const float m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale_log2;
+  const bool moves = m > row.ref + kRefSlack;
+  if (__any_sync(0xffffffffu, moves)) {
+    const float to = moves ? m : row.ref;
+    const float f = moves ? exp2_approx(row.ref - to) : 1.0f;
+    row.ref = to;
+    row.sum *= f;
+    if (!first) {
+      if (!__all_sync(0xffffffffu, before_rescale())) return false;
+      tmem_fence_after();
+#pragma unroll
+      for (int c = 0; c < 128; c += 32) {
+        float o[32];
+        tmem_ld32(o_addr + c, o);
+        tmem_wait_ld<32>(o);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] *= f;
+        tmem_st32(o_addr + c, reinterpret_cast<const uint32_t*>(o));
+      }
+    }
+  }
+  const float base = row.ref == -INFINITY ? 0.0f : -row.ref;
+  const uint64_t scale2 = pair_of(scale_log2, scale_log2), base2 = pair_of(base, base);
+  float add[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int c = 0; c < kCols; c += 64) {
+    uint32_t w[32];
+#pragma unroll
+    for (int i = 0; i < 64; i += 2) {
+      float x, y;
+      split_pair(fma_pair(pair_of(s[c + i], s[c + i + 1]), scale2, base2), x, y);
+      x = exp2_approx(x);
+      y = exp2_approx(y);
+      add[i & 2] += x;
+      add[(i & 2) + 1] += y;
+      w[i / 2] = pack2<kBf16>(x, y);
+    }
+    tmem_st32(s_addr + c / 2, w);
+  }
+  row.sum += (add[0] + add[1]) + (add[2] + add[3]);
+  tmem_wait_st();
+  return true;
+}
+
+}  // namespace tp
