@@ -366,6 +366,33 @@ int tp_prompt_attention(const tp_prompt_plan* plan, const int32_t* words, const 
                         const void* q, const void* k, const void* v, float scale, void* out, void* workspace,
                         size_t workspace_bytes, void* stream);
 
+/* Layout of a tp_tree_attention call: queries (batch, head, draft) at b * q[0] + h * q[1] + t * q[2]
+ * elements, drafted keys and values alike, 128 contiguous channels, rows on 16-byte boundaries;
+ * mask bytes at b * mask[0] + row * mask[1] + column. */
+typedef struct tp_drafts {
+  int32_t batch, num_q_heads, n_drafts; /* query heads of one sequence; drafts 1..256 */
+  int32_t q_dtype, kv_dtype;            /* TP_F16 or TP_F32; float32 is rounded to float16 */
+  int64_t q[3], k[3], v[3], mask[2];
+} tp_drafts;
+
+/* Workspace bytes of tp_tree_attention; num_q_heads over num_kv_heads as the pool counts them (all
+ * sequences), or 0 for an invalid layout. */
+size_t tp_tree_attention_workspace_size(int32_t num_kv_heads, int32_t num_q_heads, int32_t n_drafts);
+
+/* Attention of drafted tokens over the compressed cache and each other, to verify them in one call:
+ *   out[b][t][hq][:] = softmax(scale * q . K) @ V   (fp16, [batch][n_drafts][H_q][128])
+ * where draft t sees every cached token (pages [0, n_pages) decoded as tp_decode_pages decodes them,
+ * then the tail; positions >= seq_len masked) and the drafts d with mask[t][d] != 0, usually its
+ * ancestors and itself.  A row that sees nothing gives 0, and a masked draft has no influence,
+ * whatever it holds.  Nothing is appended: tp_append takes the accepted drafts.  The reference has
+ * no counterpart (its fused call takes one query token, benchmarks/turbopolar_fast_attention.py:
+ * 106-131).  The pool's heads are batch x KV heads; state.first_page must be 0.  workspace: not
+ * shared by calls that may overlap; word 0 is set to 1 when a wait ran out (the output is then
+ * unusable) and never cleared. */
+int tp_tree_attention(const tp_page_pool* pool, const tp_tail* tail, tp_state state, const tp_drafts* drafts,
+                      const void* q, const void* k, const void* v, const void* mask, float scale, void* out,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
 /* Message of the last failed call on this thread ("" if none). */
 const char* tp_last_error(void);
 

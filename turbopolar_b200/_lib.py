@@ -25,6 +25,7 @@ EXPORTED = (
     "tp_exchange_bytes", "tp_ipc_alloc", "tp_ipc_open", "tp_ipc_close", "tp_ipc_free",
     "tp_decode_attention_sharded", "tp_decode_step_sharded",
     "tp_norm_rope", "tp_prompt_plan_make", "tp_prompt_attention",
+    "tp_tree_attention", "tp_tree_attention_workspace_size",
 )
 MAX_RANKS = 8
 
@@ -95,6 +96,13 @@ class PromptRows(ctypes.Structure):
                 ("dtype", ctypes.c_int32)]
 
 
+class Drafts(ctypes.Structure):
+    """tp_drafts: sizes, types and strides of a tp_tree_attention call."""
+    _fields_ = [("batch", ctypes.c_int32), ("num_q_heads", ctypes.c_int32), ("n_drafts", ctypes.c_int32),
+                ("q_dtype", ctypes.c_int32), ("kv_dtype", ctypes.c_int32), ("q", ctypes.c_int64 * 3),
+                ("k", ctypes.c_int64 * 3), ("v", ctypes.c_int64 * 3), ("mask", ctypes.c_int64 * 2)]
+
+
 _lib = None
 _lock = threading.Lock()
 
@@ -134,6 +142,9 @@ def _declare(lib):
         "tp_prompt_plan_make": (ctypes.c_int, [P, P, I32, I32, I32, ctypes.POINTER(PromptPlan), P, SZ]),
         "tp_prompt_attention": (ctypes.c_int, [ctypes.POINTER(PromptPlan), P, ctypes.POINTER(PromptRows), P, P, P, F,
                                                P, P, SZ, P]),
+        "tp_tree_attention_workspace_size": (SZ, [I32, I32, I32]),
+        "tp_tree_attention": (ctypes.c_int, [ctypes.POINTER(PagePool), ctypes.POINTER(Tail), State,
+                                             ctypes.POINTER(Drafts), P, P, P, P, F, P, P, SZ, P]),
         "tp_last_error": (ctypes.c_char_p, []),
         "tp_version": (ctypes.c_int, []),
     }

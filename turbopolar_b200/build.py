@@ -16,7 +16,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libturbopolar.so")
 STAMP = LIB + ".stamp"
-SOURCES = ["tp_encode.cu", "tp_attention.cu", "tp_misc.cu", "tp_rope.cu", "tp_prompt.cu"]
+SOURCES = ["tp_encode.cu", "tp_attention.cu", "tp_misc.cu", "tp_rope.cu", "tp_prompt.cu",
+           "tp_tree.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",

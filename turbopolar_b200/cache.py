@@ -29,10 +29,18 @@ from typing import Any, Dict, Optional, Tuple
 import torch
 
 from . import _lib, guard
+from ._checks import check_out, disjoint, launch, refuse_gradients
 from .codec import encode_pages, _stream
 from .config import TurboPolarConfig
 from .pages import PAGE, PagePool, page_bytes
 from .payload import PolarKeyBlock, QuantizedVBlock, block_metadata
+
+
+def _row_layout(x: torch.Tensor) -> bool:
+    """Rows of contiguous channels on 16-byte boundaries."""
+    step = 16 // x.element_size()
+    return x.stride(-1) == 1 and not x.data_ptr() & 15 and not any(
+        s % step for s, n in zip(x.stride()[:-1], x.shape) if n > 1)
 
 
 class TurboPolarKVCacheRuntime:
@@ -63,6 +71,8 @@ class TurboPolarKVCacheRuntime:
         self.tail_v: Optional[torch.Tensor] = None
         self.d_state: Optional[torch.Tensor] = None
         self._workspace: Optional[torch.Tensor] = None
+        self._tree_workspace: Optional[torch.Tensor] = None
+        self._tree_layouts: dict = {}  # checked layouts of tree_attention calls, by shapes, strides and types
         self.n_pages = 0
         self.tail_len = 0
         self.qjl_blocks: list = []
@@ -334,6 +344,91 @@ class TurboPolarKVCacheRuntime:
         else:
             self.tail_len += 1
         return out if out is not None else partial_out
+
+    # ------------------------------------------------------------------ drafted tokens
+    def _tree_layout(self, q, k, v, mask) -> Tuple[Optional[_lib.Drafts], int]:
+        """The layout of a tree_attention call and its workspace size, or ``(None, 0)`` where an
+        input has to be copied first.  Raises for everything that does not fit the cache."""
+        B, H, D = self._batch_size, self._num_kv_heads, self._head_dim
+        if q.dim() != 4 or q.shape[0] != B or q.shape[3] != D:
+            raise ValueError(f"query shape {tuple(q.shape)} does not match the cache (B={B}, D=128)")
+        Hq, T = q.shape[1], q.shape[2]
+        if Hq < 1 or Hq % H:
+            raise ValueError(f"tree_attention requires GQA ratio to divide evenly, got {Hq} and {H}")
+        if not 1 <= T <= 256:
+            raise ValueError(f"tree_attention takes 1 to 256 drafted tokens, got {T}")
+        for name, x in (("k_draft", k), ("v_draft", v)):
+            if tuple(x.shape) != (B, H, T, D):
+                raise ValueError(f"{name} must be ({B}, {H}, {T}, {D}), got {tuple(x.shape)}")
+        for name, x in (("q", q), ("k_draft", k), ("v_draft", v)):
+            if x.dtype not in (torch.float16, torch.float32):
+                raise ValueError(f"{name} must be float16 or float32, got {x.dtype}")
+        if k.dtype != v.dtype:
+            raise ValueError(f"k_draft dtype {k.dtype} must match v_draft dtype {v.dtype}")
+        if mask.dtype != torch.bool or tuple(mask.shape) not in ((T, T), (B, T, T)):
+            raise ValueError(f"mask must be a ({T}, {T}) or ({B}, {T}, {T}) bool tensor")
+        if any(x.device != self.device for x in (q, k, v, mask)):
+            raise ValueError("q, k_draft, v_draft and mask must be on the cache's device")
+        if not all(map(_row_layout, (q, k, v))) or (T > 1 and mask.stride(-1) != 1):
+            return None, 0
+        strides = lambda x: (ctypes.c_int64 * 3)(*(s if n > 1 else 0 for s, n in zip(x.stride(), x.shape[:3])))
+        code = lambda x: _lib.TP_F16 if x.dtype == torch.float16 else _lib.TP_F32
+        layout = _lib.Drafts(B, Hq, T, code(q), code(k), strides(q), strides(k), strides(v),
+                             (ctypes.c_int64 * 2)(mask.stride(0) if mask.dim() == 3 else 0, mask.stride(-2)))
+        return layout, _lib.lib().tp_tree_attention_workspace_size(self.heads, B * Hq, T)
+
+    def tree_attention(self, q: torch.Tensor, k_draft: torch.Tensor, v_draft: torch.Tensor, mask: torch.Tensor,
+                       scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Attention of ``T`` drafted tokens over every appended token and each other, for verifying a
+        tree (or a chain) of drafts in one call.  Nothing is appended.
+
+        ``q`` is ``(B, H_q, T, 128)``, ``k_draft`` and ``v_draft`` ``(B, H_kv, T, 128)``, all rotated
+        to the drafts' positions, float16 or float32 (rounded to float16); ``T`` is 1 to 256.
+        ``mask`` is ``(T, T)`` or ``(B, T, T)`` bool: draft ``t`` sees draft ``d`` where
+        ``mask[t, d]``, usually its ancestors and itself.  Every draft sees the whole cache.
+        A draft that is masked has no influence on a row, whatever it holds.
+
+        Returns float16 ``(B, H_q, T, 128)``, a view of a ``(B, T, H_q, 128)`` buffer (``out`` if
+        given), so that ``.transpose(1, 2).reshape(B, T, -1)`` copies nothing.  After verification,
+        ``append(k_draft[:, :, path], v_draft[:, :, path])`` stores the accepted path.
+        """
+        if not self._initialized or (self.n_pages == 0 and self.tail_len == 0):
+            raise RuntimeError("TurboPolar cache returned no blocks after append")
+        if self.first_page or self.later_tokens:
+            raise NotImplementedError("tree_attention works on whole sequences, not on sequence shards")
+        refuse_gradients(q, k_draft, v_draft)
+        key = (q.shape, q.stride(), q.dtype, q.device, k_draft.shape, k_draft.stride(), k_draft.dtype, k_draft.device,
+               v_draft.shape, v_draft.stride(), v_draft.dtype, v_draft.device, mask.shape, mask.stride(), mask.dtype,
+               mask.device)
+        known = self._tree_layouts.get(key)
+        qp, kp, vp = q.data_ptr(), k_draft.data_ptr(), v_draft.data_ptr()
+        if known is None or (qp | kp | vp) & 15:
+            known = self._tree_layout(q, k_draft, v_draft, mask)
+            if known[0] is None:
+                copies = (x if _row_layout(x) else x.clone(memory_format=torch.contiguous_format)
+                          for x in (q, k_draft, v_draft))
+                return self.tree_attention(*copies, mask.contiguous(), scale, out)
+            if len(self._tree_layouts) >= 256:
+                self._tree_layouts.clear()
+            self._tree_layouts[key] = known
+        layout, need = known
+        B, Hq, T = layout.batch, layout.num_q_heads, layout.n_drafts
+        if out is None:
+            out = torch.empty((B, T, Hq, 128), dtype=torch.float16, device=self.device)
+        else:
+            check_out(out, (B, T, Hq, 128), torch.float16, self.device, "out")
+            if not out.is_contiguous() or out.data_ptr() & 15:
+                raise ValueError("out must be contiguous and 16-byte aligned")
+            if not all(disjoint(out, x) for x in (q, k_draft, v_draft)):
+                raise ValueError("out shares memory with an input")
+        if self._tree_workspace is None or self._tree_workspace.numel() < need:
+            self._tree_workspace = torch.zeros(need, dtype=torch.uint8, device=self.device)
+        status = launch(self.device, _lib.lib().tp_tree_attention, self.pool_struct(), self.tail_struct(), self.state(),
+                        layout, qp, kp, vp, mask.data_ptr(), float(self.config.attention_scale if scale is None else scale),
+                        out.data_ptr(), self._tree_workspace.data_ptr(), self._tree_workspace.numel())
+        if status:
+            _lib.check(status)
+        return out.transpose(1, 2)
 
     # ------------------------------------------------------------------ reference views
     def _views(self, n: int):

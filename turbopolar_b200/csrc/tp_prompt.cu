@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
         ok = __all_sync(0xffffffffu, wait_bar(s_full + t, j & 1, stop));
         if (ok && live) {
           tmem_fence_after();
-          ok = softmax_tile<kKeys, kBf16>(row, s_addr, o_addr, limit - (it.k_begin + j * kKeys), P.scale_log2, j == 0,
+          ok = softmax_tile<kKeys, kBf16>(row, s_addr, o_addr, FirstN{limit - (it.k_begin + j * kKeys)}, P.scale_log2, j == 0,
                                           [&] { return wait_bar(o_done + t, (j - 1) & 1, stop); });
           tmem_fence_before();
         }
@@ -209,32 +209,34 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
 #pragma unroll
             for (int i = 0; i < 32; ++i) o[i] = 0.0f;
           }
-          if (!valid) continue;
-          for (int e = 0; e < listed; ++e) {  // keys with non-finite values that this row sees
-            const int key = it.k_begin + partial * kKeys + late[e];
-            if (key >= limit) continue;
-            const uint16_t* qr = P.q + q_row * P.q_t + head * P.q_h;
-            const uint16_t* kr = P.k + (int64_t(it.k_row) + key) * P.k_t + kvh * P.k_h;
-            const uint16_t* vr = P.v + (int64_t(it.k_row) + key) * P.v_t + kvh * P.v_h;
-            float dot = 0.0f;
-            for (int d = 0; d < kD; ++d) dot = fmaf(widen<kBf16>(qr[d]), widen<kBf16>(kr[d]), dot);
-            const float p = exp2_approx(fmaf(dot, P.scale_log2, -row.ref));
-#pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = fmaf(p, widen<kBf16>(vr[c + i]), o[i]);
+          if (valid) {
+            for (int e = 0; e < listed; ++e) {  // keys with non-finite values that this row sees
+              const int key = it.k_begin + partial * kKeys + late[e];
+              if (key >= limit) continue;
+              const uint16_t* qr = P.q + q_row * P.q_t + head * P.q_h;
+              const uint16_t* kr = P.k + (int64_t(it.k_row) + key) * P.k_t + kvh * P.k_h;
+              const uint16_t* vr = P.v + (int64_t(it.k_row) + key) * P.v_t + kvh * P.v_h;
+              float dot = 0.0f;
+              for (int d = 0; d < kD; ++d) dot = fmaf(widen<kBf16>(qr[d]), widen<kBf16>(kr[d]), dot);
+              const float p = exp2_approx(fmaf(dot, P.scale_log2, -row.ref));
+  #pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = fmaf(p, widen<kBf16>(vr[c + i]), o[i]);
+            }
+            if (merged) {
+              float4* dst = reinterpret_cast<float4*>(P.rec_o + rec * kD + c);
+  #pragma unroll
+              for (int i = 0; i < 8; ++i) dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            } else {
+              uint4* dst = reinterpret_cast<uint4*>(P.out + (q_row * P.hq + head) * kD + c);
+  #pragma unroll
+              for (int i = 0; i < 4; ++i)
+                dst[i] = make_uint4(pack2<kBf16>(o[8 * i] * inv, o[8 * i + 1] * inv),
+                                    pack2<kBf16>(o[8 * i + 2] * inv, o[8 * i + 3] * inv),
+                                    pack2<kBf16>(o[8 * i + 4] * inv, o[8 * i + 5] * inv),
+                                    pack2<kBf16>(o[8 * i + 6] * inv, o[8 * i + 7] * inv));
+            }
           }
-          if (merged) {
-            float4* dst = reinterpret_cast<float4*>(P.rec_o + rec * kD + c);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-          } else {
-            uint4* dst = reinterpret_cast<uint4*>(P.out + (q_row * P.hq + head) * kD + c);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              dst[i] = make_uint4(pack2<kBf16>(o[8 * i] * inv, o[8 * i + 1] * inv),
-                                  pack2<kBf16>(o[8 * i + 2] * inv, o[8 * i + 3] * inv),
-                                  pack2<kBf16>(o[8 * i + 4] * inv, o[8 * i + 5] * inv),
-                                  pack2<kBf16>(o[8 * i + 6] * inv, o[8 * i + 7] * inv));
-          }
+          __syncwarp();
         }
         if (merged && valid) P.rec_ml[rec] = make_float2(row.ref, row.sum);
       }
@@ -419,8 +421,10 @@ static int launch_prompt(const PromptParams& P, const tp_prompt_plan& plan, cuda
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess && (dev >= 64 || !allowed[dev])) {
-    e = cudaFuncSetAttribute(prompt_attention_kernel<kBf16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPromptSmem);
-    if (e == cudaSuccess && dev < 64) allowed[dev] = true;
+    const int st = allow_kernel(reinterpret_cast<const void*>(prompt_attention_kernel<kBf16>), kPromptSmem, kPromptThreads,
+                                2 * kSoftmaxRegs + kIssueRegs, "tp_prompt_attention");
+    if (st != TP_OK) return st;
+    if (dev < 64) allowed[dev] = true;
   }
   if (e != cudaSuccess) return fail(TP_ERR_CUDA, std::string("tp_prompt_attention: ") + cudaGetErrorString(e));
   if (plan.items)

@@ -1,0 +1,782 @@
+// Attention of drafted tokens over the compressed cache, the dense tail and each other.
+//
+//   out[t][h] = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q[t][h] . k_j)
+// over every cached token (pages decoded to float16 keys and values as tp_decode_pages decodes
+// them, then the tail) and the drafts d with mask[t][d].
+//
+// The T drafts times the G query heads of a KV head are the rows; up to 256 rows (two tiles of 128)
+// share each decoded page, so a page is read and decoded once per KV head for T * G <= 256, where
+// one single-token call per draft would stream it T times.  The steps of all (KV head, row group)
+// segments -- pages, tail, tiles of 64 drafts -- form one flat list, cut into equal ranges, one per
+// SM; rows of a segment that several CTAs worked on are merged by merge_pieces_kernel.
+//
+//   warps 0-3, 4-7   softmax, one row per thread (queries live in tensor memory as operand A)
+//   warps 8-15       decode: 64 keys and values per step into a ring of 32 KB stages
+//   warp 16          issues the products
+//   warps 17-19      complete the warpgroup (registers are moved per warpgroup)
+// With more than 128 rows the softmax warpgroups have a tile each; with fewer they take
+// alternate steps of the one tile, each with its own running maximum, sum and accumulator, and
+// merge at the segment's end.
+#include <algorithm>
+#include <cmath>
+#include <string>
+
+#include "tp_codec.cuh"
+#include "tp_umma.cuh"
+
+namespace tp {
+
+constexpr int kTreeKeys = 64;                         // keys per step: one page
+constexpr int kKvHalf = kTreeKeys * 128;              // 64 keys x 64 channels
+constexpr int kTreeStage = 4 * kKvHalf;               // K then V
+constexpr int kTreeStages = 5;
+constexpr int kMaxDrafts = 256;
+constexpr int kGroupRows = 2 * kTile;                 // rows that share a decoded page
+constexpr int kLateRing = 16;                         // segments whose lists may be alive
+constexpr int kTreeThreads = 640;
+// Five warpgroups at 96 registers: 480, of which the softmax threads take 128, decode 88, issue 48.
+constexpr int kTreeSoftmaxRegs = 128, kTreeDecodeRegs = 88, kTreeIssueRegs = 48;
+constexpr int kOffBits = kTreeStages * kTreeStage;    // [2][128][4] uint64: drafts that a row sees
+constexpr int kOffTab = kOffBits + 2 * 128 * 4 * 8;   // float2[512]
+constexpr int kOffMl = kOffTab + 512 * 8;             // [2 pieces][2 warpgroups][128] float2
+constexpr int kOffLate = kOffMl + 2 * 2 * 128 * 8;    // [kLateRing][8] words
+constexpr int kOffTreeBars = kOffLate + kLateRing * 32;
+constexpr int kTreeSmem = kOffTreeBars + 256;
+
+enum { kTreeDefault = 0, kTreeAdapter = 1, kTreeGeneral = 2 };
+
+struct TreeParams {
+  PoolArgs pool;
+  const void *tail_k, *tail_v;
+  int tail_f32, q_f32, kv_f32;
+  int heads, hkv, hq, group, drafts, rows;  // heads: batch * hkv; rows: drafts * group
+  int row_groups, n_page_steps, tail_len, n_tail_steps, n_steps, visible;
+  int64_t total;                            // segments * n_steps
+  int grid;
+  float scale_log2;
+  const void *q, *k, *v;
+  int64_t q_b, q_h, q_t, k_b, k_h, k_t, v_b, v_h, v_t;
+  const uint8_t* mask;
+  int64_t mask_b, mask_t;
+  __half* out;                              // [batch][drafts][hq][128]
+  float* rec_o;                             // [piece][record rows][128]
+  float2* rec_ml;
+  int rec_rows;
+  int* error;
+  float2 cs[512];                           // (cos, sin) of the level-1 codes, then of the deep codes
+};
+
+__device__ __forceinline__ int64_t range_begin(const TreeParams& P, int cta) { return P.total * cta / P.grid; }
+
+// A thread's share of one page in flight: two radius chunks (8 pairs of a row each), their codes, two
+// value words and their scales.
+struct PageRegs {
+  uint4 rad[2], v[2];
+  uint2 code[2];
+  uint32_t scale[2][2];
+  float rscale;
+};
+
+__device__ __forceinline__ uint4 ldg16(const void* p) {
+  uint4 r;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "l"(p));
+  return r;
+}
+__device__ __forceinline__ uint2 ldg8(const void* p) {
+  uint2 r;
+  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
+  return r;
+}
+__device__ __forceinline__ uint32_t ldg4(const void* p) {
+  uint32_t r;
+  asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(r) : "l"(p));
+  return r;
+}
+
+template <int kMode>
+__device__ __forceinline__ void load_page(PageRegs& R, const PoolArgs& L, int head, int page, int tid) {
+  const uint8_t* pg = L.pages + (int64_t(head) * L.page_capacity + page) * L.page_bytes;
+  const int warp = tid >> 5, lane = tid & 31, c = tid & 7, l = tid >> 3;
+  if (kMode != kTreeGeneral) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const uint8_t* un = pg + u * L.unit_bytes;
+      if (kMode == kTreeDefault) {
+        R.rad[u] = ldg16(un + radii_f16_offset(l, 8 * c));
+        R.code[u].x = ldg4(un + L.u_codes + l * 32 + 4 * c);
+      } else {
+        const uint2 r8 = ldg8(un + l * 64 + 8 * c);
+        R.rad[u].x = r8.x, R.rad[u].y = r8.y;
+        R.code[u] = ldg8(un + L.u_codes + l * 64 + 8 * c);
+      }
+    }
+  }
+  const uint8_t* un = pg + (warp >> 2) * L.unit_bytes;
+#pragma unroll
+  for (int kk = 0; kk < 2; ++kk) {
+    R.v[kk] = ldg16(un + L.u_vcodes + kk * 2048 + (warp & 3) * 512 + lane * 16);
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+      R.scale[kk][a] = ldg4(un + L.u_vscales + (kk * 64 + (lane & 3) * 16 + a * 8 + (warp & 3) * 2) * 2);
+  }
+  R.rscale = L.int8_radii ? __half2float(L.radii_scales[int64_t(head) * L.page_capacity + page]) : 0.0f;
+}
+
+__device__ __forceinline__ void st16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ void st8(uint32_t addr, uint32_t a, uint32_t b) {
+  asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(addr), "r"(a), "r"(b) : "memory");
+}
+
+// The 16 channels of 8 decoded pairs of row `row`: two 16-byte chunks; the two halves of the warp's
+// chunks are stored in opposite order, so that eight lanes always cover all banks.
+__device__ __forceinline__ void store_pairs(uint32_t k_tile, int row, int c, const uint32_t (&w)[8]) {
+  const uint32_t base = k_tile + (c >> 2) * kKvHalf + row * 128;
+  const int c0 = (2 * c) & 7, odd = c >> 2;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int which = i ^ odd;
+    const uint32_t at = base + (((c0 + which) ^ (row & 7)) << 4);
+    if (which == 0) st16(at, w[0], w[1], w[2], w[3]);
+    else st16(at, w[4], w[5], w[6], w[7]);
+  }
+}
+
+// Decode one page into the stage (K tile, V tile).  `limit`: tokens of the page that are seen;
+// values of the others are cleared (their weights are 0, and 0 times a non-finite value is NaN).
+template <int kMode>
+__device__ __forceinline__ void decode_step(const PageRegs& R, const PoolArgs& L, const float2* tab, uint32_t stage,
+                                            int head, int page, int limit, int tid) {
+  const int warp = tid >> 5, lane = tid & 31, c = tid & 7, l = tid >> 3;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    uint32_t w[8];
+    if (kMode == kTreeDefault) {
+      const uint32_t rr[4] = {R.rad[u].x, R.rad[u].y, R.rad[u].z, R.rad[u].w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float2 cs = tab[(R.code[u].x >> (4 * i)) & 15];
+        const float2 r2 = __half22float2(u32_as_h2(rr[i >> 1]));
+        const float r = i & 1 ? r2.y : r2.x;
+        w[i] = pack_h2(r * cs.x, r * cs.y);
+      }
+    } else if (kMode == kTreeAdapter) {
+      const float s = R.rscale * 1.4426950408889634f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t rw = i < 4 ? R.rad[u].x : R.rad[u].y, cw = i < 4 ? R.code[u].x : R.code[u].y;
+        const float2 cs = tab[256 + ((cw >> (8 * (i & 3))) & 255)];
+        const float r = exp2_approx(float(int8_t(rw >> (8 * (i & 3)))) * s);
+        w[i] = pack_h2(r * cs.x, r * cs.y);
+      }
+    } else {
+      const uint8_t* un = L.pages + (int64_t(head) * L.page_capacity + page) * L.page_bytes + u * L.unit_bytes;
+      const uint8_t* row = un + L.u_codes + l * L.code_row;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int j = 8 * c + i;
+        const bool l1 = j < L.l1_pairs;
+        const int rel = l1 ? j : j - L.l1_pairs, bits = l1 ? L.l1_bits : L.deep_bits;
+        const int at = rel * bits;
+        const uint32_t code = (row[(l1 ? 0 : L.l1_row) + (at >> 3)] >> (at & 7)) & ((1u << bits) - 1);
+        const float r = L.int8_radii
+                            ? exp2_approx(float(reinterpret_cast<const int8_t*>(un)[l * 64 + j]) * R.rscale * 1.4426950408889634f)
+                            : __half2float(*reinterpret_cast<const __half*>(un + radii_f16_offset(l, j)));
+        const float2 cs = tab[(l1 ? 0 : 256) + code];
+        w[i] = pack_h2(r * cs.x, r * cs.y);
+      }
+    }
+    store_pairs(stage, u * 32 + l, c, w);
+  }
+  // Values: byte x of a word is code + 128; 0x6400 | x is the float16 number 1024 + x.
+  const uint32_t v_tile = stage + 2 * kKvHalf;
+  const int u = warp >> 2, G = warp & 3, g = lane >> 2, t = lane & 3;
+  const __half2 bias = __float2half2_rn(1152.0f);
+#pragma unroll
+  for (int kk = 0; kk < 2; ++kk) {
+    const uint32_t words[4] = {R.v[kk].x, R.v[kk].y, R.v[kk].z, R.v[kk].w};
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const __half s = b ? __high2half(u32_as_h2(R.scale[kk][a])) : __low2half(u32_as_h2(R.scale[kk][a]));
+        const __half2 s2 = __half2half2(s);
+        const int in_page = u * 32 + kk * 16 + 8 * a + 2 * t + b;
+        uint32_t o[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          o[e] = h2_as_u32(__hmul2(__hsub2(u32_as_h2(prmt(words[2 * a + e], 0x64646464u, b ? 0x4341u : 0x4240u)), bias), s2));
+        if (in_page >= limit) o[0] = o[1] = 0;
+        const int chunk = (G & 1) * 4 + (g >> 1);
+        st8(v_tile + (G >> 1) * kKvHalf + in_page * 128 + ((chunk ^ (in_page & 7)) << 4) + (g & 1) * 8, o[0], o[1]);
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ uint4 dense_chunk(const void* p, int64_t at, int f32) {  // 8 channels as float16
+  if (!f32) return *reinterpret_cast<const uint4*>(static_cast<const __half*>(p) + at);
+  const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + at);
+  const float4 b = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + at + 4);
+  return make_uint4(pack_h2(a.x, a.y), pack_h2(a.z, a.w), pack_h2(b.x, b.y), pack_h2(b.z, b.w));
+}
+__device__ __forceinline__ bool chunk_not_finite(uint4 x) {
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t e = w[i] & 0x7c007c00u;
+    bad |= (e & 0xffff0000u) == 0x7c000000u || (e & 0xffffu) == 0x7c00u;
+  }
+  return bad;
+}
+
+// Rows [0, valid) of dense keys and values (row strides kt, vt) into the stage, the rest cleared.
+// With `late`, a row with a non-finite value sets its bit there.  All 256 decode threads.
+__device__ __forceinline__ void dense_step(uint32_t stage, const void* k, const void* v, int64_t kt, int64_t vt, int f32,
+                                           int valid, uint32_t* late, int tid) {
+#pragma unroll 2
+  for (int i = 0; i < 4; ++i) {
+    const int row = i * 16 + (tid >> 4), c = tid & 15;
+    uint4 x = make_uint4(0, 0, 0, 0), y = x;
+    if (row < valid) {
+      x = dense_chunk(k, row * kt + 8 * c, f32);
+      y = dense_chunk(v, row * vt + 8 * c, f32);
+      if (late && chunk_not_finite(y)) atomicOr(late + (row >> 5), 1u << (row & 31));
+    }
+    const uint32_t at = stage + tile_chunk(row, c, kTreeKeys);
+    st16(at, x.x, x.y, x.z, x.w);
+    st16(at + 2 * kKvHalf, y.x, y.y, y.z, y.w);
+  }
+}
+
+__device__ __forceinline__ float load_any(const void* p, int64_t i, int f32) {
+  return f32 ? __half2float(__float2half_rn(static_cast<const float*>(p)[i])) : __half2float(static_cast<const __half*>(p)[i]);
+}
+
+// kPair: a tile per softmax warpgroup (more than 128 rows).
+template <int kMode, bool kPair>
+__global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const __grid_constant__ TreeParams P) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float2* tab = reinterpret_cast<float2*>(smem + kOffTab);
+  uint32_t* late_ring = reinterpret_cast<uint32_t*>(smem + kOffLate);
+  uint64_t* kv_full = reinterpret_cast<uint64_t*>(smem + kOffTreeBars);
+  uint64_t *kv_empty = kv_full + kTreeStages, *s_full = kv_empty + kTreeStages, *p_full = s_full + 2,
+           *o_done = p_full + 2, *q_full = o_done + 2, *met = q_full + 1, *scanned = met + 1, *drained = scanned + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
+  volatile int* stop = reinterpret_cast<int*>(tmem_slot + 1);
+
+  for (int i = threadIdx.x; i < 512; i += kTreeThreads) tab[i] = P.cs[i];
+  for (int i = threadIdx.x; i < kLateRing * 8; i += kTreeThreads) late_ring[i] = 0;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kTreeStages; ++i) {
+      mbar_init(kv_full + i, 8);
+      mbar_init(kv_empty + i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(s_full + i, 2);
+      mbar_init(p_full + i, 4);
+      mbar_init(o_done + i, 1);
+    }
+    mbar_init(q_full, 8);
+    mbar_init(met, 8);
+    mbar_init(scanned, 8);
+    mbar_init(drained, 1);
+    *stop = 0;
+    fence_mbar_init();
+  }
+  if (warp == 16) tmem_alloc(tmem_slot, 512);
+  tmem_fence_before();
+  __syncthreads();
+  tmem_fence_after();
+  asm volatile("griddepcontrol.launch_dependents;");  // merge_pieces_kernel waits for this grid itself
+  // Tensor memory: queries of tile t at 64 t, accumulator t at 128 + 128 t, scores t at 384 + 64 t.
+  const uint32_t tmem = *tmem_slot;
+  const int64_t f0 = range_begin(P, blockIdx.x), f1 = range_begin(P, blockIdx.x + 1);
+  const int seg0 = int(f0 / P.n_steps), step0 = int(f0 - int64_t(seg0) * P.n_steps);
+  const int count = int(f1 - f0);
+  const int draft0 = P.n_page_steps + P.n_tail_steps;  // first step of draft tiles
+
+  if (warp < 8) {
+    more_registers<kTreeSoftmaxRegs>();
+    const int w = warp >> 2;
+    const int r0 = (warp & 3) * 32 + lane;          // row in the tile
+    const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
+    const uint32_t s_addr = tmem + 384 + 64 * w + lanes;
+    uint64_t* bits = reinterpret_cast<uint64_t*>(smem + kOffBits) + (w * 128 + r0) * 4;
+    float2* ml = reinterpret_cast<float2*>(smem + kOffMl);
+    int units = 0, piece = 0, draft_pieces = 0;
+    bool ok = true;
+    for (int done = 0, seg = seg0, a = step0; done < count && ok; ++piece, ++seg, a = 0) {
+      const int b = min(P.n_steps, a + count - done);
+      const int head = seg / P.row_groups, rg = seg - head * P.row_groups;
+      const int batch = head / P.hkv, kvh = head - batch * P.hkv;
+      const int r = rg * kGroupRows + (kPair ? w * kTile : 0) + r0;
+      const bool valid = r < P.rows;
+      const int g = valid ? r / P.drafts : 0, t = valid ? r - g * P.drafts : 0;
+      const int64_t q_at = batch * P.q_b + (int64_t(kvh) * P.group + g) * P.q_h + t * P.q_t;
+      if (kPair || w == 0) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint32_t x[32];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint4 v = valid ? dense_chunk(P.q, q_at + half * 64 + 8 * i, P.q_f32) : make_uint4(0, 0, 0, 0);
+            x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
+          }
+          tmem_st32(tmem + 64 * w + lanes + 32 * half, x);
+        }
+        tmem_wait_st();
+      }
+      if (b > draft0) {  // which drafts this row sees
+        const uint8_t* m = P.mask + batch * P.mask_b + t * P.mask_t;
+        for (int d0 = 0; d0 < P.drafts; d0 += 64) {
+          uint64_t x = 0;
+          const int n = min(64, P.drafts - d0);
+#pragma unroll 16
+          for (int d = 0; d < n; ++d) x |= uint64_t(m[d0 + d] != 0) << d;
+          bits[d0 >> 6] = x;
+        }
+      }
+      tmem_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+      const bool live = __any_sync(0xffffffffu, valid);
+      SoftmaxRow row;
+      bool any = false;
+      for (int s = a; s < b && ok; ++s) {
+        if (!kPair && ((done + s - a) & 1) != w) continue;
+        ok = __all_sync(0xffffffffu, wait_bar(s_full + w, units & 1, stop));
+        if (ok && live) {
+          tmem_fence_after();
+          uint64_t sees = ~uint64_t(0);
+          if (s >= draft0) {
+            sees = bits[s - draft0];
+          } else {
+            const int n = s < P.n_page_steps ? P.visible - s * kTreeKeys : P.tail_len;
+            if (n < kTreeKeys) sees = (uint64_t(1) << n) - 1;
+          }
+          ok = softmax_tile<kTreeKeys, false>(row, s_addr, tmem + 128 + 128 * w + lanes, Bits64{sees}, P.scale_log2, !any,
+                                              [&] { return wait_bar(o_done + w, (units - 1) & 1, stop); });
+          tmem_fence_before();
+        }
+        __syncwarp();
+        if (ok && lane == 0) mbar_arrive(p_full + w);
+        any = true;
+        ++units;
+      }
+      if (ok && any) ok = __all_sync(0xffffffffu, wait_bar(o_done + w, (units - 1) & 1, stop));
+      bool any0 = any, any1 = false;
+      float2 other = make_float2(-INFINITY, 0.0f);
+      if (!kPair && ok) {
+        // Both warpgroups hold parts of the same rows: exchange maxima and sums, then each writes
+        // half of the channels of both accumulators' weighted sum.
+        float2* mine = ml + (piece & 1) * 256;
+        mine[w * 128 + r0] = make_float2(row.ref, row.sum);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(met);
+        ok = __all_sync(0xffffffffu, wait_bar(met, piece & 1, stop));
+        if (ok) other = mine[(w ^ 1) * 128 + r0];
+        const int n = b - a, first = done & 1;  // warpgroup of the piece's first step
+        any0 = n > 1 || first == 0;
+        any1 = n > 1 || first == 1;
+      }
+      if (ok && live) {
+        tmem_fence_after();
+        const float ref0 = kPair || w == 0 ? row.ref : other.x, ref1 = kPair || w == 0 ? other.x : row.ref;
+        const float top = fmaxf(row.ref, other.x);
+        const float base = top == -INFINITY ? 0.0f : top;
+        const float w0 = exp2_approx(ref0 - base), w1 = kPair ? 0.0f : exp2_approx(ref1 - base);
+        const float sum = kPair ? row.sum
+                                : w0 * (w == 0 ? row.sum : other.y) + w1 * (w == 0 ? other.y : row.sum);
+        const bool whole = a == 0 && b == P.n_steps;
+        const float inv = !whole ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
+        const int64_t rec = (int64_t(blockIdx.x) + seg) * P.rec_rows + (r - rg * kGroupRows);
+        const int64_t out_at = ((int64_t(batch) * P.drafts + t) * P.hq + int64_t(kvh) * P.group + g) * kD;
+        const uint32_t* late = late_ring + (draft_pieces & (kLateRing - 1)) * 8;
+        const int c_begin = kPair ? 0 : 64 * w, c_end = kPair ? kD : 64 * w + 64;
+        const uint32_t o0 = tmem + 128 + (kPair ? 128 * w : 0) + lanes, o1 = tmem + 256 + lanes;
+        for (int c = c_begin; c < c_end; c += 32) {
+          float o[32], x[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0.0f;
+          if (any0) {
+            tmem_ld32(o0 + c, o);
+            tmem_wait_ld<32>(o);
+            if (!kPair) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] *= w0;
+            }
+          }
+          if (!kPair && any1) {
+            tmem_ld32(o1 + c, x);
+            tmem_wait_ld<32>(x);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = fmaf(w1, x[i], o[i]);
+          }
+          if (valid) {
+            if (b > draft0) {  // drafts with non-finite values that this row sees
+              for (int d = 0; d < P.drafts; ++d) {
+                if (!(late[d >> 5] >> (d & 31) & 1) || !(bits[d >> 6] >> (d & 63) & 1)) continue;
+                const int64_t k_at = batch * P.k_b + kvh * P.k_h + d * P.k_t, v_at = batch * P.v_b + kvh * P.v_h + d * P.v_t;
+                float dot = 0.0f;
+                for (int i = 0; i < kD; ++i) dot = fmaf(load_any(P.q, q_at + i, P.q_f32), load_any(P.k, k_at + i, P.kv_f32), dot);
+                const float p = exp2_approx(fmaf(dot, P.scale_log2, -base));
+  #pragma unroll 4
+                for (int i = 0; i < 32; ++i) o[i] = fmaf(p, load_any(P.v, v_at + c + i, P.kv_f32), o[i]);
+              }
+            }
+            if (whole) {
+              uint4* dst = reinterpret_cast<uint4*>(P.out + out_at + c);
+  #pragma unroll
+              for (int i = 0; i < 4; ++i)
+                dst[i] = make_uint4(pack_h2(o[8 * i] * inv, o[8 * i + 1] * inv), pack_h2(o[8 * i + 2] * inv, o[8 * i + 3] * inv),
+                                    pack_h2(o[8 * i + 4] * inv, o[8 * i + 5] * inv),
+                                    pack_h2(o[8 * i + 6] * inv, o[8 * i + 7] * inv));
+            } else {
+              float4* dst = reinterpret_cast<float4*>(P.rec_o + rec * kD + c);
+  #pragma unroll
+              for (int i = 0; i < 8; ++i) dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            }
+          }
+          __syncwarp();
+        }
+        if (!whole && valid && (kPair || w == 0)) P.rec_ml[rec] = make_float2(kPair ? row.ref : top, sum);
+      }
+      tmem_fence_before();
+      if (b > draft0) ++draft_pieces;
+      done += b - a;
+    }
+  } else if (warp < 16) {
+    fewer_registers<kTreeDecodeRegs>();
+    const int tid = threadIdx.x - 256;
+    const uint32_t stages = smem_u32(smem);
+    PageRegs next;
+    int seg = seg0, s = step0, scans = 0, draft_pieces = 0;
+    bool ok = true;
+    auto prefetch = [&](int ahead) {  // page of the step `ahead` steps on, into L2
+      int ps = s + ahead, pseg = seg;
+      if (ps >= P.n_steps) ps -= P.n_steps, ++pseg;
+      if (ps < P.n_page_steps) {
+        const uint8_t* pg = P.pool.pages + (int64_t(pseg / P.row_groups) * P.pool.page_capacity + ps) * P.pool.page_bytes;
+        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(pg), "r"(P.pool.page_bytes) : "memory");
+      }
+    };
+    constexpr int kAhead = 6;
+    if (tid == 0)
+      for (int i = 1; i < min(kAhead, count); ++i)
+        if (i < P.n_steps) prefetch(i);
+    if (count && s < P.n_page_steps) load_page<kMode>(next, P.pool, seg / P.row_groups, s, tid);
+    for (int i = 0; i < count && ok; ++i) {
+      const int st = i % kTreeStages, use = i / kTreeStages;
+      const uint32_t stage = stages + st * kTreeStage;
+      const int head = seg / P.row_groups;
+      const PageRegs now = next;
+      int ns = s + 1, nseg = seg;
+      if (ns == P.n_steps) ns = 0, ++nseg;
+      if (tid == 0 && i + kAhead < count && kAhead < P.n_steps) prefetch(kAhead);
+      if (i + 1 < count && ns < P.n_page_steps) load_page<kMode>(next, P.pool, nseg / P.row_groups, ns, tid);
+      ok = use == 0 || wait_bar(kv_empty + st, (use - 1) & 1, stop);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      if (s < P.n_page_steps) {
+        decode_step<kMode>(now, P.pool, tab, stage, head, s, P.visible - s * kTreeKeys, tid);
+      } else if (s < draft0) {
+        const int64_t at = int64_t(head) * kPage * kD * (P.tail_f32 ? 4 : 2);
+        dense_step(stage, static_cast<const uint8_t*>(P.tail_k) + at, static_cast<const uint8_t*>(P.tail_v) + at, kD, kD,
+                   P.tail_f32, P.tail_len, nullptr, tid);
+      } else {
+        const int batch = head / P.hkv, kvh = head - batch * P.hkv, d0 = (s - draft0) * kTreeKeys;
+        const int size = P.kv_f32 ? 4 : 2;
+        uint32_t* late = late_ring + (draft_pieces & (kLateRing - 1)) * 8;
+        if (tid < 8 && (s == draft0 || i == 0)) late_ring[((draft_pieces + kLateRing / 2) & (kLateRing - 1)) * 8 + tid] = 0;
+        const int n = min(kTreeKeys, P.drafts - d0);
+        dense_step(stage, static_cast<const uint8_t*>(P.k) + (batch * P.k_b + kvh * P.k_h + d0 * P.k_t) * size,
+                   static_cast<const uint8_t*>(P.v) + (batch * P.v_b + kvh * P.v_h + d0 * P.v_t) * size, P.k_t, P.v_t,
+                   P.kv_f32, n, late + (d0 >> 5), tid);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(scanned);
+        ok = __all_sync(0xffffffffu, wait_bar(scanned, scans & 1, stop));
+        if (!ok) break;
+        ++scans;
+        for (int q = 0; q < 4; ++q) {
+          const int row = q * 16 + (tid >> 4);
+          if (late[(d0 >> 5) + (row >> 5)] >> (row & 31) & 1)
+            st16(stage + 2 * kKvHalf + tile_chunk(row, tid & 15, kTreeKeys), 0, 0, 0, 0);
+        }
+        if (s == P.n_steps - 1) ++draft_pieces;
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(kv_full + st);
+      s = ns;
+      seg = nseg;
+    }
+  } else if (fewer_registers<kTreeIssueRegs>(); warp == 16) {
+    if (lane == 0) {
+      constexpr uint32_t kScores = mma_idesc(false, kTreeKeys, false), kOut = mma_idesc(false, kD, true);
+      const uint32_t stages = smem_u32(smem);
+      int n[2] = {0, 0};
+      bool ok = true;
+      int a = step0;
+      for (int done = 0, piece = 0; done < count && ok; ++piece, a = 0) {
+        const int b = min(P.n_steps, a + count - done);
+        const int n_units = (b - a) * (kPair ? 2 : 1);
+        bool acc[2] = {false, false};
+        ok = wait_bar(q_full, piece & 1, stop);
+        auto scores = [&](int u) {
+          const int i = done + (kPair ? u >> 1 : u), t = kPair ? u & 1 : i & 1, st = i % kTreeStages;
+          if ((!kPair || t == 0) && !wait_bar(kv_full + st, (i / kTreeStages) & 1, stop)) return false;
+          tmem_fence_after();
+#pragma unroll
+          for (int ks = 0; ks < kD / 16; ++ks)
+            mma_ts(tmem + 384 + 64 * t, tmem + (kPair ? 64 * t : 0) + ks * 8,
+                   rows_desc(stages + st * kTreeStage + (ks >> 2) * kKvHalf + (ks & 3) * 32), kScores, ks > 0);
+          mbar_arrive(s_full + t);  // makes what this thread has acquired from the decode warps visible
+          mma_commit(s_full + t);
+          return true;
+        };
+        auto values = [&](int u) {
+          const int i = done + (kPair ? u >> 1 : u), t = kPair ? u & 1 : i & 1, st = i % kTreeStages;
+          if (!wait_bar(p_full + t, n[t] & 1, stop)) return false;
+          tmem_fence_after();
+#pragma unroll
+          for (int ks = 0; ks < kTreeKeys / 16; ++ks)
+            mma_ts(tmem + 128 + 128 * t, tmem + 384 + 64 * t + ks * 8,
+                   cols_desc(stages + st * kTreeStage + 2 * kKvHalf + ks * 2048, kKvHalf), kOut, acc[t] || ks > 0);
+          acc[t] = true;
+          ++n[t];
+          mma_commit(o_done + t);
+          if (!kPair || t == 1) mma_commit(kv_empty + st);
+          return true;
+        };
+        if (ok) ok = scores(0) && (n_units < 2 || scores(1));
+        for (int u = 0; u < n_units && ok; ++u) {
+          ok = values(u);
+          if (ok && u + 2 < n_units) ok = scores(u + 2);
+        }
+        done += b - a;
+      }
+      mma_commit(drained);
+      drain_bar(drained, 0);
+    }
+    __syncwarp();
+  }
+  __syncthreads();
+  if (warp == 16) {
+    tmem_fence_after();
+    tmem_free(tmem, 512);
+  }
+  if (threadIdx.x == 0 && *stop) *P.error = 1;
+}
+
+// Rows of segments that several CTAs worked on: M = max ref_i, w_i = 2^(ref_i - M),
+// out = sum w_i o_i / sum w_i l_i (0 where nothing was seen).  One warp per row.
+__global__ void __launch_bounds__(256) merge_pieces_kernel(const __grid_constant__ TreeParams P) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int seg = blockIdx.x, head = seg / P.row_groups, rg = seg - head * P.row_groups;
+  const int i = blockIdx.y * 8 + warp, r = rg * kGroupRows + i;
+  if (i >= kGroupRows || r >= P.rows) return;
+  // CTAs whose ranges meet the segment's steps [f0, f1).
+  const int64_t f0 = int64_t(seg) * P.n_steps, f1 = f0 + P.n_steps;
+  int first = int(f0 * P.grid / P.total);
+  while (range_begin(P, first + 1) <= f0) ++first;
+  int last = first;
+  while (range_begin(P, last + 1) < f1) ++last;
+  if (first == last) return;  // written by that CTA
+  float top = -INFINITY;
+  for (int c = first + lane; c <= last; c += 32) top = fmaxf(top, P.rec_ml[(int64_t(c) + seg) * P.rec_rows + i].x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float base = top == -INFINITY ? 0.0f : top;
+  float l = 0.0f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int c = first; c <= last; ++c) {
+    const int64_t rec = (int64_t(c) + seg) * P.rec_rows + i;
+    const float2 ml = P.rec_ml[rec];
+    const float4 o = *reinterpret_cast<const float4*>(P.rec_o + rec * kD + 4 * lane);
+    const float w = exp2_approx(ml.x - base);
+    l = fmaf(w, ml.y, l);
+    acc.x = fmaf(w, o.x, acc.x);
+    acc.y = fmaf(w, o.y, acc.y);
+    acc.z = fmaf(w, o.z, acc.z);
+    acc.w = fmaf(w, o.w, acc.w);
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const int batch = head / P.hkv, kvh = head - batch * P.hkv, g = r / P.drafts, t = r - g * P.drafts;
+  uint2* dst = reinterpret_cast<uint2*>(P.out + ((int64_t(batch) * P.drafts + t) * P.hq + int64_t(kvh) * P.group + g) * kD +
+                                        4 * lane);
+  *dst = make_uint2(pack_h2(acc.x * inv, acc.y * inv), pack_h2(acc.z * inv, acc.w * inv));
+}
+
+// ----------------------------------------------------------------------------- host
+template <int kMode, bool kPair>
+static int launch_tree(const TreeParams& P, int segments, cudaStream_t s) {
+  static bool allowed[64] = {};  // the attribute belongs to a device's copy of the kernel
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev >= 64 || !allowed[dev])) {
+    const int st = allow_kernel(reinterpret_cast<const void*>(tree_attention_kernel<kMode, kPair>), kTreeSmem, kTreeThreads,
+                                2 * kTreeSoftmaxRegs + 2 * kTreeDecodeRegs + kTreeIssueRegs, "tp_tree_attention");
+    if (st != TP_OK) return st;
+    if (dev < 64) allowed[dev] = true;
+  }
+  if (e != cudaSuccess) return fail(TP_ERR_CUDA, std::string("tp_tree_attention: ") + cudaGetErrorString(e));
+  tree_attention_kernel<kMode, kPair><<<P.grid, kTreeThreads, kTreeSmem, s>>>(P);
+  if (P.grid > 1) {
+    // A programmatic dependent of the first grid: its CTAs are launched while that one ends.
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(segments, (P.rec_rows + 7) / 8);
+    cfg.blockDim = dim3(256);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, merge_pieces_kernel, P);
+    if (e != cudaSuccess) return fail(TP_ERR_CUDA, std::string("tp_tree_attention: ") + cudaGetErrorString(e));
+  }
+  return check_launch("tp_tree_attention");
+}
+
+template <int kMode>
+static int launch_tree_rows(const TreeParams& P, int segments, cudaStream_t s) {
+  return P.rows > kTile ? launch_tree<kMode, true>(P, segments, s) : launch_tree<kMode, false>(P, segments, s);
+}
+
+// (cos, sin) of every code of 2, 4 or 8 bits, the decoder's angle formula in float32 (rfsn_v11/quant/
+// polar/decoder.py:36-56), cosine and sine rounded to float32; computed once.
+static void copy_angles(float2* cs, int bits) {
+  static float2 table[9][256];
+  static std::once_flag once;
+  std::call_once(once, [] {
+    for (int b : {2, 4, 8}) {
+      const int n = 1 << b;
+      for (int code = 0; code < n; ++code) {
+        const float norm = float(code) / float(n - 1);
+        volatile float turned = norm * 6.28318530717958647692f;  // rounded before the subtraction
+        const float angle = turned - 3.14159265358979323846f;
+        table[b][code] = make_float2(float(std::cos(double(angle))), float(std::sin(double(angle))));
+      }
+    }
+  });
+  std::copy_n(table[bits], 1 << bits, cs);
+}
+
+static int row_groups_of(int64_t rows) { return int((rows + kGroupRows - 1) / kGroupRows); }
+
+static size_t tree_workspace(int64_t heads, int64_t rows) {
+  const int64_t slots = heads * row_groups_of(rows) + device_sms();
+  return 256 + size_t(slots) * std::min<int64_t>(rows, kGroupRows) * (kD * sizeof(float) + sizeof(float2));
+}
+
+static bool rows_ok(const void* p, const int64_t* st, const int* n, int f32) {
+  const int step = f32 ? 4 : 8;
+  if (uintptr_t(p) % 16) return false;
+  for (int i = 0; i < 3; ++i)
+    if (n[i] > 1 && st[i] % step) return false;
+  return true;
+}
+
+}  // namespace tp
+
+using namespace tp;
+
+extern "C" {
+
+size_t tp_tree_attention_workspace_size(int32_t num_kv_heads, int32_t num_q_heads, int32_t n_drafts) {
+  if (num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads || n_drafts < 1 || n_drafts > kMaxDrafts) return 0;
+  return tree_workspace(num_kv_heads, int64_t(n_drafts) * (num_q_heads / num_kv_heads));
+}
+
+int tp_tree_attention(const tp_page_pool* pool, const tp_tail* tail, tp_state state, const tp_drafts* drafts,
+                      const void* q, const void* k, const void* v, const void* mask, float scale, void* out,
+                      void* workspace, size_t workspace_bytes, void* stream) {
+  Layout L;
+  int st = validate_pool(pool, &L);
+  if (st != TP_OK) return st;
+  if (!drafts || !q || !k || !v || !mask || !out) return fail(TP_ERR_INVALID, "tp_tree_attention: NULL argument");
+  const tp_drafts& D = *drafts;
+  const int heads = pool->num_kv_heads;
+  if (D.batch < 1 || heads % D.batch) return fail(TP_ERR_INVALID, "tp_tree_attention: batch does not divide the pool's heads");
+  const int hkv = heads / D.batch;
+  if (D.num_q_heads < 1 || D.num_q_heads % hkv)
+    return fail(TP_ERR_INVALID, "num_q_heads must be divisible by num_kv_heads for GQA");
+  if (D.n_drafts < 1 || D.n_drafts > kMaxDrafts)
+    return fail(TP_ERR_INVALID, "tp_tree_attention: n_drafts must be in [1, 256]");
+  if ((D.q_dtype != TP_F16 && D.q_dtype != TP_F32) || (D.kv_dtype != TP_F16 && D.kv_dtype != TP_F32))
+    return fail(TP_ERR_INVALID, "tp_tree_attention: q, k and v must be float16 or float32");
+  if (!(scale > 0.f) || !(scale < 1e30f)) return fail(TP_ERR_INVALID, "attention scale must be positive");
+  if (state.n_pages < 0 || state.n_pages > pool->page_capacity || state.tail_len < 0 || state.tail_len >= kPage ||
+      state.first_page != 0)
+    return fail(TP_ERR_INVALID, "tp_tree_attention: cache state outside the pool, or a sequence shard");
+  const int64_t cached = int64_t(state.n_pages) * kPage + state.tail_len;
+  if (state.seq_len < 0 || state.seq_len > cached)
+    return fail(TP_ERR_INVALID, "tp_tree_attention: seq_len outside the cached tokens");
+  if (state.tail_len > 0 && (!tail || !tail->k || !tail->v || (uintptr_t(tail->k) | uintptr_t(tail->v)) % 16))
+    return fail(TP_ERR_INVALID, "tp_tree_attention: tail buffers missing");
+  if (state.tail_len > 0 && tail->dtype != TP_F16 && tail->dtype != TP_F32)
+    return fail(TP_ERR_INVALID, "tp_tree_attention: tail dtype must be float16 or float32");
+  const int q_n[3] = {D.batch, D.num_q_heads, D.n_drafts}, kv_n[3] = {D.batch, hkv, D.n_drafts};
+  if (!rows_ok(q, D.q, q_n, D.q_dtype == TP_F32) || !rows_ok(k, D.k, kv_n, D.kv_dtype == TP_F32) ||
+      !rows_ok(v, D.v, kv_n, D.kv_dtype == TP_F32) || uintptr_t(out) % 16)
+    return fail(TP_ERR_INVALID, "tp_tree_attention: rows must start on 16-byte boundaries");
+  const int group = D.num_q_heads / hkv;
+  const int64_t rows = int64_t(group) * D.n_drafts;
+  const size_t need = tree_workspace(heads, rows);
+  if (!workspace || workspace_bytes < need)
+    return fail(TP_ERR_INVALID, "tp_tree_attention: workspace too small (need " + std::to_string(need) + " bytes)");
+
+  static thread_local TreeParams P;  // 4.6 KB, filled anew by each call
+  P.pool = pool_args(*pool, L);
+  P.tail_k = tail ? tail->k : nullptr;
+  P.tail_v = tail ? tail->v : nullptr;
+  P.tail_f32 = tail && tail->dtype == TP_F32;
+  P.q_f32 = D.q_dtype == TP_F32;
+  P.kv_f32 = D.kv_dtype == TP_F32;
+  P.heads = heads;
+  P.hkv = hkv;
+  P.hq = D.num_q_heads;
+  P.group = group;
+  P.drafts = D.n_drafts;
+  P.rows = int(rows);
+  P.row_groups = row_groups_of(rows);
+  P.visible = int(std::min<int64_t>(state.seq_len, int64_t(state.n_pages) * kPage));
+  P.n_page_steps = (P.visible + kPage - 1) / kPage;
+  P.tail_len = int(std::max<int64_t>(0, state.seq_len - int64_t(state.n_pages) * kPage));
+  P.n_tail_steps = P.tail_len > 0;
+  P.n_steps = P.n_page_steps + P.n_tail_steps + (D.n_drafts + kTreeKeys - 1) / kTreeKeys;
+  const int64_t segments = int64_t(heads) * P.row_groups;
+  P.total = segments * P.n_steps;
+  if (segments > (1 << 24) || P.total > (int64_t(1) << 31))
+    return fail(TP_ERR_UNSUPPORTED, "tp_tree_attention: too many heads, drafts or pages");
+  P.grid = int(std::min<int64_t>(device_sms(), P.total));
+  P.scale_log2 = scale * 1.4426950408889634f;
+  P.q = q, P.k = k, P.v = v;
+  P.q_b = D.q[0], P.q_h = D.q[1], P.q_t = D.q[2];
+  P.k_b = D.k[0], P.k_h = D.k[1], P.k_t = D.k[2];
+  P.v_b = D.v[0], P.v_h = D.v[1], P.v_t = D.v[2];
+  P.mask = static_cast<const uint8_t*>(mask);
+  P.mask_b = D.mask[0], P.mask_t = D.mask[1];
+  P.out = static_cast<__half*>(out);
+  P.error = static_cast<int*>(workspace);
+  P.rec_rows = int(std::min<int64_t>(rows, kGroupRows));
+  P.rec_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + 256);
+  P.rec_ml = reinterpret_cast<float2*>(P.rec_o + (segments + device_sms()) * P.rec_rows * kD);
+  copy_angles(P.cs, pool->fmt.l1_bits);
+  copy_angles(P.cs + 256, pool->fmt.deep_bits);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const tp_format& F = pool->fmt;
+  if (F.l1_bits == 4 && F.deep_bits == 4 && F.split_dim == 64 && !F.int8_radii)
+    return launch_tree_rows<kTreeDefault>(P, int(segments), s);
+  if (F.int8_radii && F.split_dim == 0 && F.deep_bits == 8) return launch_tree_rows<kTreeAdapter>(P, int(segments), s);
+  return launch_tree_rows<kTreeGeneral>(P, int(segments), s);
+}
+
+}  // extern "C"

@@ -38,6 +38,22 @@ inline int device_sms() {
   return sms[dev];
 }
 
+// Allow a kernel its dynamic shared memory on the current device.  `wg_regs`: the registers per
+// thread that its warpgroups ask for, summed over the warpgroups; a warpgroup that asked for more than the block
+// was launched with would wait for good, so a build whose register count differs is refused here.
+inline int allow_kernel(const void* fn, int smem, int threads, int wg_regs, const char* what) {
+  cudaFuncAttributes attr;
+  cudaError_t e = cudaFuncGetAttributes(&attr, fn);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail(TP_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
+  }
+  if (attr.numRegs * (threads / 128) < wg_regs)
+    return fail(TP_ERR_CUDA, std::string(what) + ": built with " + std::to_string(attr.numRegs) + " registers per thread");
+  return TP_OK;
+}
+
 // ----------------------------------------------------------------------------- descriptors
 constexpr int kTile = 128;               // query rows of a tile
 constexpr int kHalfTile = kTile * 128;   // bytes of 128 rows x 64 channels
@@ -209,21 +225,33 @@ struct SoftmaxRow {
   float sum = 0.0f;
 };
 
-// One tile of kCols scores of this thread's row, in tensor memory at `s_addr` (the warp's lanes):
-// columns >= `visible` are masked (whatever they hold, NaN included).  Writes the 16-bit weights over the
+// Which columns of a tile a row sees: the first `n`, or those whose bit is set.
+struct FirstN {
+  int n;
+  template <int kCols> __device__ __forceinline__ bool all() const { return n >= kCols; }
+  __device__ __forceinline__ bool operator()(int c) const { return c < n; }
+};
+struct Bits64 {
+  uint64_t bits;
+  template <int kCols> __device__ __forceinline__ bool all() const { return ~bits == 0; }
+  __device__ __forceinline__ bool operator()(int c) const { return bits >> c & 1; }
+};
+
+// One tile of kCols scores of this thread's row, in tensor memory at `s_addr` (the warp's lanes);
+// columns that the row does not see are masked, whatever they hold.  Writes the 16-bit weights over the
 // scores.  `o_addr`: the row's 128 accumulator columns, rescaled when the reference moves;
 // `before_rescale()` waits until the products issued so far have completed (false: given up) and
 // is not called for the first tile, when the accumulator holds nothing.
-template <int kCols, bool kBf16, class Wait>
-__device__ __forceinline__ bool softmax_tile(SoftmaxRow& row, uint32_t s_addr, uint32_t o_addr, int visible,
+template <int kCols, bool kBf16, class Sees, class Wait>
+__device__ __forceinline__ bool softmax_tile(SoftmaxRow& row, uint32_t s_addr, uint32_t o_addr, Sees sees,
                                              float scale_log2, bool first, Wait before_rescale) {
   float s[kCols];
 #pragma unroll
   for (int c = 0; c < kCols; c += 32) tmem_ld32(s_addr + c, s + c);
   tmem_wait_ld<kCols>(s);
-  if (__any_sync(0xffffffffu, visible < kCols)) {
+  if (!__all_sync(0xffffffffu, sees.template all<kCols>())) {
 #pragma unroll
-    for (int c = 0; c < kCols; ++c) s[c] = c < visible ? s[c] : -INFINITY;
+    for (int c = 0; c < kCols; ++c) s[c] = sees(c) ? s[c] : -INFINITY;
   }
   float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
