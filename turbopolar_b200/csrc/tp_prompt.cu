@@ -40,6 +40,8 @@ constexpr int kPromptThreads = 384, kSoftmaxRegs = 208, kIssueRegs = 88;
 constexpr int kPromptBars = 2 * kTileBytes + kRing * kTileBytes;  // byte offset of the barriers
 constexpr int kPromptSmem = kPromptBars + 256 + 2 * kMaxLate;
 constexpr int kRecordRows = 2 * kTile;   // rows of an item's partial record
+// Tensor memory (a CTA holds all of it, so it starts at column 0): scores of tile t at 128 t.
+constexpr uint32_t kScoreCol = 0, kOutCol = 256;
 
 // One work item (eight words, made on the host and copied to the device).
 struct PromptItem {
@@ -160,7 +162,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
   tmem_fence_before();
   __syncthreads();
   tmem_fence_after();
-  const uint32_t tmem = *tmem_slot;  // scores of tile t: columns 128 t; accumulator: 256 + 128 t
+  const uint32_t tmem = *tmem_slot;
+  if (tmem != 0 && threadIdx.x == 0) *stop = 1;  // all 512 columns: always at 0
+  asm volatile("griddepcontrol.launch_dependents;");  // merge_items_kernel waits for this grid itself
 
   if (warp < 8) {
     more_registers<kSoftmaxRegs>();
@@ -169,7 +173,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
     const int tok = t * P.tile_tokens + r / P.group, head = kvh * P.group + r % P.group;
     const bool valid = r < P.tile_tokens * P.group && tok < it.q_tokens;
     const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
-    const uint32_t s_addr = tmem + 128 * t + lanes, o_addr = tmem + 256 + 128 * t + lanes;
+    const uint32_t s_addr = kScoreCol + 128 * t + lanes, o_addr = kOutCol + 128 * t + lanes;
     // Rows that are not there see everything, so they ask for no masking; they are not written.
     const int limit = valid ? min(it.sees + tok, it.k_end) : it.k_end;
     const bool live = __any_sync(0xffffffffu, valid);
@@ -243,45 +247,63 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
     }
     tmem_fence_before();
   } else if (fewer_registers<kIssueRegs>(); warp == 8) {
-    if (lane == 0 && n_tiles) {
+    if (n_tiles) {
       constexpr uint32_t kScores = mma_idesc(kBf16, kKeys, false), kOut = mma_idesc(kBf16, kD, true);
-      const uint32_t q_addr = smem_u32(smem), ring_addr = smem_u32(ring);
+      const uint32_t q_lo = rows_lo(smem_u32(smem)), ring_addr = smem_u32(ring);
       const int nt = two ? 2 : 1;
-      auto scores = [&](int t, int stage) {
+      auto scores = [&](int t, int stage) {  // one thread
+        const uint32_t k_lo = rows_lo(ring_addr) + stage * (kTileBytes >> 4);
 #pragma unroll
         for (int ks = 0; ks < kD / 16; ++ks) {
-          const uint32_t off = (ks >> 2) * kHalfTile + (ks & 3) * 32;
-          mma_ss(tmem + 128 * t, rows_desc(q_addr + t * kTileBytes + off), rows_desc(ring_addr + stage * kTileBytes + off),
-                 kScores, ks > 0);
+          const uint32_t off = ((ks >> 2) * kHalfTile + (ks & 3) * 32) >> 4;
+          mma_ss(kScoreCol + 128 * t, q_lo + t * (kTileBytes >> 4) + off, k_lo + off, kScores, ks > 0);
         }
         mma_commit(s_full + t);
       };
-      bool ok = wait_bar(q_full, 0, stop) && wait_bar(full, 0, stop);
+      int st = 0, ph = 0;  // stage and phase of the next tile in the ring
+      auto advance = [&] { st = st + 1 == kRing ? (ph ^= 1, 0) : st + 1; };
+      bool ok = warp_wait(q_full, 0, stop) && warp_wait(full, 0, stop);
       if (ok) {
         tmem_fence_after();
-        for (int t = 0; t < nt; ++t) scores(t, 0);
-        mma_commit(empty);
+        if (elect_one()) {
+          for (int t = 0; t < nt; ++t) scores(t, 0);
+          mma_commit(empty);
+        }
+        __syncwarp();
+        advance();
       }
       for (int j = 0; j < n_tiles && ok; ++j) {
-        const int iv = 2 * j + 1, sv = iv % kRing, ik = iv + 1, sk = ik % kRing;
-        ok = wait_bar(full + sv, (iv / kRing) & 1, stop);
-        if (ok && j >= partial) ok = wait_bar(clean, (j - partial) & 1, stop);
-        if (ok && j + 1 < n_tiles) ok = wait_bar(full + sk, (ik / kRing) & 1, stop);
+        const int sv = st;
+        ok = warp_wait(full + sv, ph, stop);
+        if (ok && j >= partial) ok = warp_wait(clean, (j - partial) & 1, stop);
+        advance();
+        const int sk = st;
+        const bool more = j + 1 < n_tiles;
+        if (ok && more) {
+          ok = warp_wait(full + sk, ph, stop);
+          advance();
+        }
+        const uint32_t v_lo = cols_lo(ring_addr, kHalfTile) + sv * (kTileBytes >> 4);
         for (int t = 0; t < nt && ok; ++t) {
-          ok = wait_bar(p_full + t, j & 1, stop);
+          ok = warp_wait(p_full + t, j & 1, stop);
           if (!ok) break;
           tmem_fence_after();
+          if (elect_one()) {
 #pragma unroll
-          for (int ks = 0; ks < kKeys / 16; ++ks)
-            mma_ts(tmem + 256 + 128 * t, tmem + 128 * t + ks * 8,
-                   cols_desc(ring_addr + sv * kTileBytes + ks * 2048, kHalfTile), kOut, j > 0 || ks > 0);
-          mma_commit(o_done + t);
-          if (t == nt - 1) mma_commit(empty + sv);
-          if (j + 1 < n_tiles) scores(t, sk);
+            for (int ks = 0; ks < kKeys / 16; ++ks)
+              mma_ts(kOutCol + 128 * t, kScoreCol + 128 * t + ks * 8, v_lo + ks * (2048 >> 4), kOut, j > 0 || ks > 0);
+            mma_commit(o_done + t);
+            if (t == nt - 1) mma_commit(empty + sv);
+            if (more) {
+              scores(t, sk);
+              if (t == nt - 1) mma_commit(empty + sk);
+            }
+          }
+          __syncwarp();
         }
-        if (ok && j + 1 < n_tiles) mma_commit(empty + sk);
       }
-      mma_commit(drained);
+      if (elect_one()) mma_commit(drained);
+      __syncwarp();
       drain_bar(drained, 0);
     }
     __syncwarp();
@@ -338,39 +360,21 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
   if (threadIdx.x == 0 && *stop) *P.error = 1;
 }
 
-// Rows of a split token block: with records (ref_i, l_i, o_i), M = max ref_i and w_i = 2^(ref_i - M),
-// out = sum w_i o_i / sum w_i l_i (0 where no record has seen a key).  One warp per row.
+// Rows of split token blocks, one warp per row.
 template <bool kBf16>
 __global__ void __launch_bounds__(256) merge_items_kernel(const __grid_constant__ PromptParams P) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const PromptMerge m = P.merges[blockIdx.x / P.hkv];
   const int kvh = blockIdx.x % P.hkv;
   const int i = blockIdx.y * 8 + warp;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (i >= m.q_tokens * P.group) return;
   const int tok = i / P.group, g = i % P.group;
   const int t = tok / P.tile_tokens, r = (tok - t * P.tile_tokens) * P.group + g;
-  const int64_t step = int64_t(P.hkv) * kRecordRows;
   const int64_t rec0 = (int64_t(m.slot) * P.hkv + kvh) * kRecordRows + t * kTile + r;
-  float top = -INFINITY;
-  for (int k = lane; k < m.n; k += 32) top = fmaxf(top, P.rec_ml[rec0 + k * step].x);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  const float base = top == -INFINITY ? 0.0f : top;
-  float l = 0.0f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int k = 0; k < m.n; ++k) {
-    const float2 ml = P.rec_ml[rec0 + k * step];
-    const float4 o = *reinterpret_cast<const float4*>(P.rec_o + (rec0 + k * step) * kD + 4 * lane);
-    const float w = exp2_approx(ml.x - base);
-    l = fmaf(w, ml.y, l);
-    acc.x = fmaf(w, o.x, acc.x);
-    acc.y = fmaf(w, o.y, acc.y);
-    acc.z = fmaf(w, o.z, acc.z);
-    acc.w = fmaf(w, o.w, acc.w);
-  }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const float4 o = merge_row(P.rec_ml + rec0, P.rec_o + rec0 * kD, int64_t(P.hkv) * kRecordRows, m.n);
   uint2* dst = reinterpret_cast<uint2*>(P.out + ((int64_t(m.q_row) + tok) * P.hq + kvh * P.group + g) * kD + 4 * lane);
-  *dst = make_uint2(pack2<kBf16>(acc.x * inv, acc.y * inv), pack2<kBf16>(acc.z * inv, acc.w * inv));
+  *dst = make_uint2(pack2<kBf16>(o.x, o.y), pack2<kBf16>(o.z, o.w));
 }
 
 // ----------------------------------------------------------------------------- host
@@ -431,7 +435,8 @@ static int launch_prompt(const PromptParams& P, const tp_prompt_plan& plan, cuda
     prompt_attention_kernel<kBf16><<<unsigned(plan.items) * plan.num_kv_heads, kPromptThreads, kPromptSmem, s>>>(P);
   if (plan.merges) {
     const int rows = plan.block_tokens * P.group;
-    merge_items_kernel<kBf16><<<dim3(unsigned(plan.merges) * plan.num_kv_heads, (rows + 7) / 8), 256, 0, s>>>(P);
+    e = launch_dependent(merge_items_kernel<kBf16>, dim3(unsigned(plan.merges) * plan.num_kv_heads, (rows + 7) / 8), 256, s, P);
+    if (e != cudaSuccess) return fail(TP_ERR_CUDA, std::string("tp_prompt_attention: ") + cudaGetErrorString(e));
   }
   return check_launch("tp_prompt_attention");
 }

@@ -43,6 +43,9 @@ constexpr int kOffLate = kOffMl + 2 * 2 * 128 * 8;    // [kLateRing][8] words
 constexpr int kOffTreeBars = kOffLate + kLateRing * 32;
 constexpr int kTreeSmem = kOffTreeBars + 256;
 
+// Tensor memory (a CTA holds all of it): queries of tile t at 64 t, accumulator and scores t at
+constexpr uint32_t kTreeOutCol = 128, kTreeScoreCol = 384;  // + 128 t and + 64 t
+
 enum { kTreeDefault = 0, kTreeAdapter = 1, kTreeGeneral = 2 };
 
 struct TreeParams {
@@ -294,8 +297,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
   __syncthreads();
   tmem_fence_after();
   asm volatile("griddepcontrol.launch_dependents;");  // merge_pieces_kernel waits for this grid itself
-  // Tensor memory: queries of tile t at 64 t, accumulator t at 128 + 128 t, scores t at 384 + 64 t.
   const uint32_t tmem = *tmem_slot;
+  if (tmem != 0 && threadIdx.x == 0) *stop = 1;  // all 512 columns: always at 0
   const int64_t f0 = range_begin(P, blockIdx.x), f1 = range_begin(P, blockIdx.x + 1);
   const int seg0 = int(f0 / P.n_steps), step0 = int(f0 - int64_t(seg0) * P.n_steps);
   const int count = int(f1 - f0);
@@ -306,7 +309,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
     const int w = warp >> 2;
     const int r0 = (warp & 3) * 32 + lane;          // row in the tile
     const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
-    const uint32_t s_addr = tmem + 384 + 64 * w + lanes;
+    const uint32_t s_addr = kTreeScoreCol + 64 * w + lanes;
     uint64_t* bits = reinterpret_cast<uint64_t*>(smem + kOffBits) + (w * 128 + r0) * 4;
     float2* ml = reinterpret_cast<float2*>(smem + kOffMl);
     int units = 0, piece = 0, draft_pieces = 0;
@@ -328,7 +331,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
             const uint4 v = valid ? dense_chunk(P.q, q_at + half * 64 + 8 * i, P.q_f32) : make_uint4(0, 0, 0, 0);
             x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
           }
-          tmem_st32(tmem + 64 * w + lanes + 32 * half, x);
+          tmem_st32(64 * w + lanes + 32 * half, x);
         }
         tmem_wait_st();
       }
@@ -337,8 +340,19 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
         for (int d0 = 0; d0 < P.drafts; d0 += 64) {
           uint64_t x = 0;
           const int n = min(64, P.drafts - d0);
+          if ((uintptr_t(m) & 3) == 0) {
+            // Four bytes of 0 or 1 at a time: the product moves byte i to bit 28 + i.
+            uint32_t word[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              word[i] = 4 * i + 3 < n ? *reinterpret_cast<const uint32_t*>(m + d0 + 4 * i) : 0;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x |= uint64_t((word[i] & 0x01010101u) * 0x10204080u >> 28) << (4 * i);
+            for (int d = n & ~3; d < n; ++d) x |= uint64_t(m[d0 + d] & 1) << d;
+          } else {
 #pragma unroll 16
-          for (int d = 0; d < n; ++d) x |= uint64_t(m[d0 + d] != 0) << d;
+            for (int d = 0; d < n; ++d) x |= uint64_t(m[d0 + d] & 1) << d;
+          }
           bits[d0 >> 6] = x;
         }
       }
@@ -360,7 +374,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
             const int n = s < P.n_page_steps ? P.visible - s * kTreeKeys : P.tail_len;
             if (n < kTreeKeys) sees = (uint64_t(1) << n) - 1;
           }
-          ok = softmax_tile<kTreeKeys, false>(row, s_addr, tmem + 128 + 128 * w + lanes, Bits64{sees}, P.scale_log2, !any,
+          ok = softmax_tile<kTreeKeys, false>(row, s_addr, kTreeOutCol + 128 * w + lanes, Bits64{sees}, P.scale_log2, !any,
                                               [&] { return wait_bar(o_done + w, (units - 1) & 1, stop); });
           tmem_fence_before();
         }
@@ -398,8 +412,11 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
         const int64_t rec = (int64_t(blockIdx.x) + seg) * P.rec_rows + (r - rg * kGroupRows);
         const int64_t out_at = ((int64_t(batch) * P.drafts + t) * P.hq + int64_t(kvh) * P.group + g) * kD;
         const uint32_t* late = late_ring + (draft_pieces & (kLateRing - 1)) * 8;
+        bool listed = false;
+        if (b > draft0)
+          for (int i = 0; i < (P.drafts + 31) >> 5; ++i) listed |= late[i] != 0;
         const int c_begin = kPair ? 0 : 64 * w, c_end = kPair ? kD : 64 * w + 64;
-        const uint32_t o0 = tmem + 128 + (kPair ? 128 * w : 0) + lanes, o1 = tmem + 256 + lanes;
+        const uint32_t o0 = kTreeOutCol + (kPair ? 128 * w : 0) + lanes, o1 = kTreeOutCol + 128 + lanes;
         for (int c = c_begin; c < c_end; c += 32) {
           float o[32], x[32];
 #pragma unroll
@@ -419,7 +436,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
             for (int i = 0; i < 32; ++i) o[i] = fmaf(w1, x[i], o[i]);
           }
           if (valid) {
-            if (b > draft0) {  // drafts with non-finite values that this row sees
+            if (listed) {  // drafts with non-finite values that this row sees
               for (int d = 0; d < P.drafts; ++d) {
                 if (!(late[d >> 5] >> (d & 31) & 1) || !(bits[d >> 6] >> (d & 63) & 1)) continue;
                 const int64_t k_at = batch * P.k_b + kvh * P.k_h + d * P.k_t, v_at = batch * P.v_b + kvh * P.v_h + d * P.v_t;
@@ -517,53 +534,65 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
       seg = nseg;
     }
   } else if (fewer_registers<kTreeIssueRegs>(); warp == 16) {
-    if (lane == 0) {
-      constexpr uint32_t kScores = mma_idesc(false, kTreeKeys, false), kOut = mma_idesc(false, kD, true);
-      const uint32_t stages = smem_u32(smem);
-      int n[2] = {0, 0};
-      bool ok = true;
-      int a = step0;
-      for (int done = 0, piece = 0; done < count && ok; ++piece, a = 0) {
-        const int b = min(P.n_steps, a + count - done);
-        const int n_units = (b - a) * (kPair ? 2 : 1);
-        bool acc[2] = {false, false};
-        ok = wait_bar(q_full, piece & 1, stop);
-        auto scores = [&](int u) {
-          const int i = done + (kPair ? u >> 1 : u), t = kPair ? u & 1 : i & 1, st = i % kTreeStages;
-          if ((!kPair || t == 0) && !wait_bar(kv_full + st, (i / kTreeStages) & 1, stop)) return false;
-          tmem_fence_after();
+    constexpr uint32_t kScores = mma_idesc(false, kTreeKeys, false), kOut = mma_idesc(false, kD, true);
+    const uint32_t stages = smem_u32(smem);
+    int n[2] = {0, 0};
+    int st_s = 0, ph_s = 0, st_v = 0;  // ring: stage and phase of the next scores, stage of the next values
+    bool ok = true;
+    int a = step0;
+    for (int done = 0, piece = 0; done < count && ok; ++piece, a = 0) {
+      const int b = min(P.n_steps, a + count - done);
+      const int n_units = (b - a) * (kPair ? 2 : 1);
+      uint32_t acc[2] = {0, 0};
+      ok = warp_wait(q_full, piece & 1, stop);
+      // Unit u: (step, tile) pairs with two tiles, steps taking turns at the warpgroups with one.
+      auto tile_of = [&](int u) { return kPair ? u & 1 : (done + u) & 1; };
+      auto scores = [&](int u) {
+        const int t = tile_of(u);
+        if ((!kPair || t == 0) && !warp_wait(kv_full + st_s, ph_s, stop)) return false;
+        tmem_fence_after();
+        if (elect_one()) {
+          const uint32_t k_lo = rows_lo(stages) + st_s * (kTreeStage >> 4);
 #pragma unroll
           for (int ks = 0; ks < kD / 16; ++ks)
-            mma_ts(tmem + 384 + 64 * t, tmem + (kPair ? 64 * t : 0) + ks * 8,
-                   rows_desc(stages + st * kTreeStage + (ks >> 2) * kKvHalf + (ks & 3) * 32), kScores, ks > 0);
-          mbar_arrive(s_full + t);  // makes what this thread has acquired from the decode warps visible
+            mma_ts(kTreeScoreCol + 64 * t, (kPair ? 64 * t : 0) + ks * 8, k_lo + (((ks >> 2) * kKvHalf + (ks & 3) * 32) >> 4),
+                   kScores, ks > 0);
+          mbar_arrive(s_full + t);  // makes what this warp has acquired from the decode warps visible
           mma_commit(s_full + t);
-          return true;
-        };
-        auto values = [&](int u) {
-          const int i = done + (kPair ? u >> 1 : u), t = kPair ? u & 1 : i & 1, st = i % kTreeStages;
-          if (!wait_bar(p_full + t, n[t] & 1, stop)) return false;
-          tmem_fence_after();
+        }
+        __syncwarp();
+        if (!kPair || t == 1) st_s = st_s + 1 == kTreeStages ? (ph_s ^= 1, 0) : st_s + 1;
+        return true;
+      };
+      auto values = [&](int u) {
+        const int t = tile_of(u);
+        if (!warp_wait(p_full + t, (t ? n[1] : n[0]) & 1, stop)) return false;
+        tmem_fence_after();
+        if (elect_one()) {
+          const uint32_t v_lo = cols_lo(stages + 2 * kKvHalf, kKvHalf) + st_v * (kTreeStage >> 4);
 #pragma unroll
           for (int ks = 0; ks < kTreeKeys / 16; ++ks)
-            mma_ts(tmem + 128 + 128 * t, tmem + 384 + 64 * t + ks * 8,
-                   cols_desc(stages + st * kTreeStage + 2 * kKvHalf + ks * 2048, kKvHalf), kOut, acc[t] || ks > 0);
-          acc[t] = true;
-          ++n[t];
+            mma_ts(kTreeOutCol + 128 * t, kTreeScoreCol + 64 * t + ks * 8, v_lo + ks * (2048 >> 4), kOut,
+                   ks > 0 || (t ? acc[1] : acc[0]));
           mma_commit(o_done + t);
-          if (!kPair || t == 1) mma_commit(kv_empty + st);
-          return true;
-        };
-        if (ok) ok = scores(0) && (n_units < 2 || scores(1));
-        for (int u = 0; u < n_units && ok; ++u) {
-          ok = values(u);
-          if (ok && u + 2 < n_units) ok = scores(u + 2);
+          if (!kPair || t == 1) mma_commit(kv_empty + st_v);
         }
-        done += b - a;
+        __syncwarp();
+        if (t) acc[1] = 1, ++n[1];
+        else acc[0] = 1, ++n[0];
+        if (!kPair || t == 1) st_v = st_v + 1 == kTreeStages ? 0 : st_v + 1;
+        return true;
+      };
+      if (ok) ok = scores(0) && (n_units < 2 || scores(1));
+      for (int u = 0; u < n_units && ok; ++u) {
+        ok = values(u);
+        if (ok && u + 2 < n_units) ok = scores(u + 2);
       }
-      mma_commit(drained);
-      drain_bar(drained, 0);
+      done += b - a;
     }
+    if (elect_one()) mma_commit(drained);
+    __syncwarp();
+    drain_bar(drained, 0);
     __syncwarp();
   }
   __syncthreads();
@@ -574,44 +603,25 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
   if (threadIdx.x == 0 && *stop) *P.error = 1;
 }
 
-// Rows of segments that several CTAs worked on: M = max ref_i, w_i = 2^(ref_i - M),
-// out = sum w_i o_i / sum w_i l_i (0 where nothing was seen).  One warp per row.
+// Rows of segments that several CTAs worked on, one warp per row.
 __global__ void __launch_bounds__(256) merge_pieces_kernel(const __grid_constant__ TreeParams P) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int seg = blockIdx.x, head = seg / P.row_groups, rg = seg - head * P.row_groups;
   const int i = blockIdx.y * 8 + warp, r = rg * kGroupRows + i;
-  if (i >= kGroupRows || r >= P.rows) return;
   // CTAs whose ranges meet the segment's steps [f0, f1).
   const int64_t f0 = int64_t(seg) * P.n_steps, f1 = f0 + P.n_steps;
   int first = int(f0 * P.grid / P.total);
   while (range_begin(P, first + 1) <= f0) ++first;
-  int last = first;
+  int last = int((f1 - 1) * P.grid / P.total);
   while (range_begin(P, last + 1) < f1) ++last;
-  if (first == last) return;  // written by that CTA
-  float top = -INFINITY;
-  for (int c = first + lane; c <= last; c += 32) top = fmaxf(top, P.rec_ml[(int64_t(c) + seg) * P.rec_rows + i].x);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  const float base = top == -INFINITY ? 0.0f : top;
-  float l = 0.0f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int c = first; c <= last; ++c) {
-    const int64_t rec = (int64_t(c) + seg) * P.rec_rows + i;
-    const float2 ml = P.rec_ml[rec];
-    const float4 o = *reinterpret_cast<const float4*>(P.rec_o + rec * kD + 4 * lane);
-    const float w = exp2_approx(ml.x - base);
-    l = fmaf(w, ml.y, l);
-    acc.x = fmaf(w, o.x, acc.x);
-    acc.y = fmaf(w, o.y, acc.y);
-    acc.z = fmaf(w, o.z, acc.z);
-    acc.w = fmaf(w, o.w, acc.w);
-  }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (i >= kGroupRows || r >= P.rows || first == last) return;  // one CTA: it has written the rows
+  const int64_t rec0 = (int64_t(first) + seg) * P.rec_rows + i;
+  const float4 o = merge_row(P.rec_ml + rec0, P.rec_o + rec0 * kD, P.rec_rows, last - first + 1);
   const int batch = head / P.hkv, kvh = head - batch * P.hkv, g = r / P.drafts, t = r - g * P.drafts;
   uint2* dst = reinterpret_cast<uint2*>(P.out + ((int64_t(batch) * P.drafts + t) * P.hq + int64_t(kvh) * P.group + g) * kD +
                                         4 * lane);
-  *dst = make_uint2(pack_h2(acc.x * inv, acc.y * inv), pack_h2(acc.z * inv, acc.w * inv));
+  *dst = make_uint2(pack_h2(o.x, o.y), pack_h2(o.z, o.w));
 }
 
 // ----------------------------------------------------------------------------- host
@@ -629,17 +639,7 @@ static int launch_tree(const TreeParams& P, int segments, cudaStream_t s) {
   if (e != cudaSuccess) return fail(TP_ERR_CUDA, std::string("tp_tree_attention: ") + cudaGetErrorString(e));
   tree_attention_kernel<kMode, kPair><<<P.grid, kTreeThreads, kTreeSmem, s>>>(P);
   if (P.grid > 1) {
-    // A programmatic dependent of the first grid: its CTAs are launched while that one ends.
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(segments, (P.rec_rows + 7) / 8);
-    cfg.blockDim = dim3(256);
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, merge_pieces_kernel, P);
+    e = launch_dependent(merge_pieces_kernel, dim3(segments, (P.rec_rows + 7) / 8), 256, s, P);
     if (e != cudaSuccess) return fail(TP_ERR_CUDA, std::string("tp_tree_attention: ") + cudaGetErrorString(e));
   }
   return check_launch("tp_tree_attention");

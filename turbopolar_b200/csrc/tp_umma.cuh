@@ -64,16 +64,15 @@ __device__ __forceinline__ uint32_t tile_chunk(int r, int c, int rows) {
   return uint32_t((c >> 3) * rows * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
 }
 
-// Shared-memory operand descriptor, 128-byte swizzle: bits 0-13 address / 16, 16-29 leading-axis
-// offset / 16, 32-45 stride offset / 16, 46-47 version 1, 61-63 swizzle 2.
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t leading, uint32_t stride) {
-  return uint64_t((addr >> 4) & 0x3fff) | (uint64_t(leading >> 4) << 16) | (uint64_t(stride >> 4) << 32) |
-         (uint64_t(1) << 46) | (uint64_t(2) << 61);
-}
-// Rows of 64 channels, channels contracted: groups of 8 rows are 1024 bytes apart.
-__device__ __forceinline__ uint64_t rows_desc(uint32_t addr) { return smem_desc(addr, 16, 1024); }
+// Shared-memory operand descriptor, 128-byte swizzle.  Low word: bits 0-13 address / 16, 16-29
+// leading-axis offset / 16.  High word, the same for every operand here: bits 0-13 stride between
+// groups of 8 rows (1024) / 16, 14-15 version 1, 29-31 swizzle 2.  Moving along a tile adds to the
+// low word only.
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+// Rows of 64 channels, channels contracted.
+__device__ __forceinline__ uint32_t rows_lo(uint32_t addr) { return (addr >> 4) | (1u << 16); }
 // Rows contracted, channels the output axis: halves of 64 channels `half` bytes apart.
-__device__ __forceinline__ uint64_t cols_desc(uint32_t addr, uint32_t half) { return smem_desc(addr, half, 1024); }
+__device__ __forceinline__ uint32_t cols_lo(uint32_t addr, uint32_t half) { return (addr >> 4) | ((half >> 4) << 16); }
 
 // kind::f16 instruction descriptor, M = 128: float32 accumulator, both operands bf16 or both f16.
 __host__ __device__ constexpr uint32_t mma_idesc(bool bf16, int n, bool b_cols) {
@@ -90,18 +89,26 @@ __device__ __forceinline__ void tmem_alloc(uint32_t* slot, int cols) {  // one w
 __device__ __forceinline__ void tmem_free(uint32_t addr, int cols) {  // the same warp
   asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols));
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+// One thread of a warp, always the same one.  Issuing under this predicate inside code that the whole
+// warp runs keeps descriptors and addresses in uniform registers, which the instruction needs; in
+// code of a single lane each product took about 100 cycles to issue.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t yes;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(yes));
+  return yes != 0;
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, bool add) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(uint32_t(add))
+      "{\n .reg .pred p;\n .reg .b64 da, db;\n setp.ne.u32 p, %4, 0;\n mov.b64 da, {%1, %5};\n mov.b64 db, {%2, %5};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n}\n" ::"r"(d),
+      "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(uint32_t(add)), "n"(kDescHi)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc, bool add) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(uint32_t(add))
+      "{\n .reg .pred p;\n .reg .b64 db;\n setp.ne.u32 p, %4, 0;\n mov.b64 db, {%2, %5};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "r"(b_lo), "r"(idesc), "r"(uint32_t(add)), "n"(kDescHi)
       : "memory");
 }
 // Arrive on `bar` once every product issued by this thread so far has completed.
@@ -125,20 +132,33 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, float* r) {
         "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
       : "r"(addr));
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, float* r) {
+  uint32_t* u = reinterpret_cast<uint32_t*>(r);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
+        "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* u) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(u[0]),
+      "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]), "r"(u[10]),
+      "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15]), "r"(addr)
+      : "memory");
+}
 // The registers of the loads above are valid after the wait; naming them as operands keeps the compiler
 // from moving their uses before it.
-__device__ __forceinline__ void after_wait32(float* r) {
+__device__ __forceinline__ void after_wait16(float* r) {
   asm volatile(""
       : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]),
-        "+f"(r[8]), "+f"(r[9]), "+f"(r[10]), "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15]),
-        "+f"(r[16]), "+f"(r[17]), "+f"(r[18]), "+f"(r[19]), "+f"(r[20]), "+f"(r[21]), "+f"(r[22]), "+f"(r[23]),
-        "+f"(r[24]), "+f"(r[25]), "+f"(r[26]), "+f"(r[27]), "+f"(r[28]), "+f"(r[29]), "+f"(r[30]), "+f"(r[31]));
+        "+f"(r[8]), "+f"(r[9]), "+f"(r[10]), "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15]));
 }
 template <int kCols>
 __device__ __forceinline__ void tmem_wait_ld(float* r) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-  for (int c = 0; c < kCols; c += 32) after_wait32(r + c);
+  for (int c = 0; c < kCols; c += 16) after_wait16(r + c);
 }
 __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* u) {
   asm volatile(
@@ -176,6 +196,9 @@ __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatil
     }
   }
   return true;
+}
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* stop) {
+  return __all_sync(0xffffffffu, wait_bar(bar, parity, stop));
 }
 // The same without giving up early, to drain copies and products in flight.
 __device__ __forceinline__ void drain_bar(uint64_t* bar, uint32_t parity) {
@@ -215,6 +238,43 @@ __device__ __forceinline__ void split_pair(uint64_t p, float& a, float& b) {
   asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
 }
 
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// 2^x of two numbers below +inf on the multiply-add pipe: the special-function unit makes 16
+// exponentials a cycle, as many as a tile's products leave time for, so part of them is made here.
+// x = n + f with f in [-1/2, 1/2]; 2^f by a polynomial of degree 4 whose coefficients minimise the
+// largest relative error, 2.6e-6 (weights are rounded to 2^-12 or 2^-9 afterwards); n goes into the
+// exponent.  Below 2^-125: 0.
+__device__ __forceinline__ void exp2_poly(uint64_t x, float& e0, float& e1) {
+  constexpr float kRound = 12582912.0f;  // 1.5 * 2^23: adding it rounds to an integer in the low bits
+  const uint64_t t = add_pair(x, pair_of(kRound, kRound));
+  const uint64_t n = add_pair(t, pair_of(-kRound, -kRound));
+  const uint64_t f = fma_pair(n, pair_of(-1.0f, -1.0f), x);
+  uint64_t p = pair_of(0.009570102207362652f, 0.009570102207362652f);
+  p = fma_pair(p, f, pair_of(0.05591785907745361f, 0.05591785907745361f));
+  p = fma_pair(p, f, pair_of(0.240247443318367f, 0.240247443318367f));
+  p = fma_pair(p, f, pair_of(0.6931217908859253f, 0.6931217908859253f));
+  p = fma_pair(p, f, pair_of(0.9999992847442627f, 0.9999992847442627f));
+  float x0, x1, t0, t1, p0, p1;
+  split_pair(x, x0, x1);
+  split_pair(t, t0, t1);
+  split_pair(p, p0, p1);
+  e0 = x0 < -125.0f ? 0.0f : __int_as_float(__float_as_int(p0) + (__float_as_int(t0) << 23));
+  e1 = x1 < -125.0f ? 0.0f : __int_as_float(__float_as_int(p1) + (__float_as_int(t1) << 23));
+}
+// Pairs of a tile's columns that take the polynomial.
+constexpr int kPolyPairs = 3;
+__host__ __device__ constexpr bool poly_pair(int i) { return (i & 7) * kPolyPairs % 8 >= 8 - kPolyPairs; }
+
 // The running softmax of a row: weights are 2^(s * scale_log2 - ref) with a reference that is at
 // least the row's maximum so far minus 8.  It moves only when a maximum exceeds it by more than 8:
 // weights up to 2^8 lose nothing in 16 bits, and the output accumulator, which lives in tensor
@@ -253,13 +313,14 @@ __device__ __forceinline__ bool softmax_tile(SoftmaxRow& row, uint32_t s_addr, u
 #pragma unroll
     for (int c = 0; c < kCols; ++c) s[c] = sees(c) ? s[c] : -INFINITY;
   }
+  // NaN wins, so a row with a NaN score is known.
   float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
   for (int c = 4; c < kCols; c += 8) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) top[i] = fmaxf(fmaxf(top[i], s[c + i]), c + 4 + i < kCols ? s[c + 4 + i] : top[i]);
+    for (int i = 0; i < 4; ++i) top[i] = c + 4 < kCols ? max3_nan(top[i], s[c + i], s[c + 4 + i]) : max3_nan(top[i], s[c + i], top[i]);
   }
-  const float m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale_log2;
+  const float m = max3_nan(top[0], top[1], max3_nan(top[2], top[3], top[3])) * scale_log2;
   const bool moves = m > row.ref + kRefSlack;
   if (__any_sync(0xffffffffu, moves)) {
     const float to = moves ? m : row.ref;
@@ -270,37 +331,105 @@ __device__ __forceinline__ bool softmax_tile(SoftmaxRow& row, uint32_t s_addr, u
       if (!__all_sync(0xffffffffu, before_rescale())) return false;
       tmem_fence_after();
 #pragma unroll
-      for (int c = 0; c < 128; c += 32) {
-        float o[32];
-        tmem_ld32(o_addr + c, o);
-        tmem_wait_ld<32>(o);
+      for (int c = 0; c < 128; c += 16) {  // a few times per row: registers count more than speed
+        float o[16];
+        tmem_ld16(o_addr + c, o);
+        tmem_wait_ld<16>(o);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) o[i] *= f;
-        tmem_st32(o_addr + c, reinterpret_cast<const uint32_t*>(o));
+        for (int i = 0; i < 16; ++i) o[i] *= f;
+        tmem_st16(o_addr + c, reinterpret_cast<const uint32_t*>(o));
       }
     }
   }
   const float base = row.ref == -INFINITY ? 0.0f : -row.ref;
   const uint64_t scale2 = pair_of(scale_log2, scale_log2), base2 = pair_of(base, base);
-  float add[4] = {0.f, 0.f, 0.f, 0.f};
+  uint64_t add[2] = {0, 0};
 #pragma unroll
-  for (int c = 0; c < kCols; c += 64) {
-    uint32_t w[32];
+  for (int c = 0; c < kCols; c += 32) {
+    uint32_t w[16];
 #pragma unroll
-    for (int i = 0; i < 64; i += 2) {
-      float x, y;
-      split_pair(fma_pair(pair_of(s[c + i], s[c + i + 1]), scale2, base2), x, y);
-      x = exp2_approx(x);
-      y = exp2_approx(y);
-      add[i & 2] += x;
-      add[(i & 2) + 1] += y;
-      w[i / 2] = pack2<kBf16>(x, y);
+    for (int i = 0; i < 16; ++i) {
+      const uint64_t x = fma_pair(pair_of(s[c + 2 * i], s[c + 2 * i + 1]), scale2, base2);
+      float e0, e1;
+      if (poly_pair(i)) {
+        exp2_poly(x, e0, e1);
+      } else {
+        split_pair(x, e0, e1);
+        e0 = exp2_approx(e0);
+        e1 = exp2_approx(e1);
+      }
+      add[i & 1] = add_pair(add[i & 1], pair_of(e0, e1));
+      w[i] = pack2<kBf16>(e0, e1);
     }
-    tmem_st32(s_addr + c / 2, w);
+    tmem_st16(s_addr + c / 2, w);
   }
-  row.sum += (add[0] + add[1]) + (add[2] + add[3]);
+  float a0, a1;
+  split_pair(add_pair(add[0], add[1]), a0, a1);
+  // A NaN or +inf score makes the whole row NaN, whatever the polynomial made of it.
+  row.sum += m < INFINITY ? a0 + a1 : NAN;
   tmem_wait_st();
   return true;
+}
+
+// ----------------------------------------------------------------------------- merging split rows
+// Four channels (4 * lane ..) of a row whose keys were split: records (ref_k, sum_k) at ml[k * step]
+// and unnormalised outputs at o[k * step * 128 + 4 * lane].  M = max ref_k, w_k = 2^(ref_k - M),
+// sum w_k o_k / sum w_k sum_k; 0 where no record has seen a key.  One warp; each lane makes the
+// weights of every 32nd record, and the outputs of eight records are loaded at a time.
+__device__ __forceinline__ float4 merge_row(const float2* ml, const float* o, int64_t step, int n) {
+  const int lane = threadIdx.x & 31;
+  float top = -INFINITY;
+  for (int k = lane; k < n; k += 32) top = fmaxf(top, ml[k * step].x);
+#pragma unroll
+  for (int i = 16; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
+  const float base = top == -INFINITY ? 0.0f : top;
+  float l = 0.0f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k0 = 0; k0 < n; k0 += 32) {
+    float w = 0.0f;
+    if (k0 + lane < n) {
+      const float2 r = ml[(k0 + lane) * step];
+      w = exp2_approx(r.x - base);
+      l = fmaf(w, r.y, l);
+    }
+    const int m = min(32, n - k0);
+    for (int k = 0; k < m; k += 8) {
+      float4 v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        v[i] = k + i < m ? *reinterpret_cast<const float4*>(o + (k0 + k + i) * step * kD + 4 * lane)
+                         : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float wi = __shfl_sync(0xffffffffu, w, (k + i) & 31);
+        if (k + i >= m) break;
+        acc.x = fmaf(wi, v[i].x, acc.x);
+        acc.y = fmaf(wi, v[i].y, acc.y);
+        acc.z = fmaf(wi, v[i].z, acc.z);
+        acc.w = fmaf(wi, v[i].w, acc.w);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 16; i > 0; i >>= 1) l += __shfl_xor_sync(0xffffffffu, l, i);
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  return make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+}
+
+// Launch a kernel as the programmatic dependent of the previous one in the stream (which lets it
+// start, and which it waits for with griddepcontrol.wait).
+template <class Params>
+inline cudaError_t launch_dependent(void (*kernel)(Params), dim3 grid, int threads, cudaStream_t s, const Params& p) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
 }  // namespace tp
