@@ -67,7 +67,7 @@ struct PromptParams {
   const uint16_t *q, *k, *v;  // for listed keys
   int64_t q_t, q_h, k_t, k_h, v_t, v_h;
   uint16_t* out;              // [tokens][hq][128]
-  float* rec_o;               // [slot][hkv][256][128]
+  float* rec_o;               // [slot][hkv][32][256][4]: channel / 4, row
   float2* rec_ml;             // [slot][hkv][256]
   int* error;
 };
@@ -201,9 +201,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
         const int listed = n_tiles ? *n_late : 0;
         const bool merged = it.slot >= 0;
         const int64_t q_row = int64_t(it.q_row) + tok;
-        const int64_t rec = (int64_t(it.slot) * P.hkv + kvh) * kRecordRows + t * kTile + r;
-        const float inv = merged ? 1.0f : row.sum == 0.0f ? 0.0f : 1.0f / row.sum;
-#pragma unroll
+        const int64_t rec = int64_t(it.slot) * P.hkv + kvh;
+        const float inv = row.sum == 0.0f ? 0.0f : 1.0f / row.sum;
+        uint8_t* dst = valid ? reinterpret_cast<uint8_t*>(P.out + (q_row * P.hq + head) * kD) : nullptr;
+#pragma unroll 1
         for (int c = 0; c < kD; c += 32) {
           float o[32];
           if (n_tiles) {
@@ -223,26 +224,26 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
               float dot = 0.0f;
               for (int d = 0; d < kD; ++d) dot = fmaf(widen<kBf16>(qr[d]), widen<kBf16>(kr[d]), dot);
               const float p = exp2_approx(fmaf(dot, P.scale_log2, -row.ref));
-  #pragma unroll
+#pragma unroll
               for (int i = 0; i < 32; ++i) o[i] = fmaf(p, widen<kBf16>(vr[c + i]), o[i]);
-            }
-            if (merged) {
-              float4* dst = reinterpret_cast<float4*>(P.rec_o + rec * kD + c);
-  #pragma unroll
-              for (int i = 0; i < 8; ++i) dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-            } else {
-              uint4* dst = reinterpret_cast<uint4*>(P.out + (q_row * P.hq + head) * kD + c);
-  #pragma unroll
-              for (int i = 0; i < 4; ++i)
-                dst[i] = make_uint4(pack2<kBf16>(o[8 * i] * inv, o[8 * i + 1] * inv),
-                                    pack2<kBf16>(o[8 * i + 2] * inv, o[8 * i + 3] * inv),
-                                    pack2<kBf16>(o[8 * i + 4] * inv, o[8 * i + 5] * inv),
-                                    pack2<kBf16>(o[8 * i + 6] * inv, o[8 * i + 7] * inv));
             }
           }
           __syncwarp();
+          if (merged) {
+            float4* to = reinterpret_cast<float4*>(P.rec_o) + (rec * 32 + c / 4) * kRecordRows + t * kTile + r;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (valid) to[i * kRecordRows] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          } else {
+            uint32_t w[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) w[i] = pack2<kBf16>(o[2 * i] * inv, o[2 * i + 1] * inv);
+            // The query tile has been read: its memory carries the rows out.
+            store_rows64(smem + t * kTileBytes + (warp & 3) * kStageRows, w, dst ? dst + 2 * c : nullptr);
+          }
+          __syncwarp();
         }
-        if (merged && valid) P.rec_ml[rec] = make_float2(row.ref, row.sum);
+        if (merged && valid) P.rec_ml[rec * kRecordRows + t * kTile + r] = make_float2(row.ref, row.sum);
       }
     }
     tmem_fence_before();
@@ -360,21 +361,26 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
   if (threadIdx.x == 0 && *stop) *P.error = 1;
 }
 
-// Rows of split token blocks, one warp per row.
+// Rows of split token blocks: 32 rows x 8 channels per block.
 template <bool kBf16>
-__global__ void __launch_bounds__(256) merge_items_kernel(const __grid_constant__ PromptParams P) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+__global__ void __launch_bounds__(kMergeThreads) merge_items_kernel(const __grid_constant__ PromptParams P) {
   const PromptMerge m = P.merges[blockIdx.x / P.hkv];
   const int kvh = blockIdx.x % P.hkv;
-  const int i = blockIdx.y * 8 + warp;
+  const int tile_rows = P.tile_tokens * P.group;
+  const int r0 = blockIdx.y * 32, t = r0 >> 7;  // rows of the record: tile t, row r0 & 127
+  const int rows = min(min(32, tile_rows - (r0 & 127)), m.q_tokens * P.group - t * tile_rows - (r0 & 127));
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (i >= m.q_tokens * P.group) return;
-  const int tok = i / P.group, g = i % P.group;
-  const int t = tok / P.tile_tokens, r = (tok - t * P.tile_tokens) * P.group + g;
-  const int64_t rec0 = (int64_t(m.slot) * P.hkv + kvh) * kRecordRows + t * kTile + r;
-  const float4 o = merge_row(P.rec_ml + rec0, P.rec_o + rec0 * kD, int64_t(P.hkv) * kRecordRows, m.n);
-  uint2* dst = reinterpret_cast<uint2*>(P.out + ((int64_t(m.q_row) + tok) * P.hq + kvh * P.group + g) * kD + 4 * lane);
-  *dst = make_uint2(pack2<kBf16>(o.x, o.y), pack2<kBf16>(o.z, o.w));
+  if (rows <= 0) return;
+  const int64_t rec = int64_t(m.slot) * P.hkv + kvh;
+  const float v = merge_block(P.rec_ml + rec * kRecordRows + r0,
+                              reinterpret_cast<const float4*>(P.rec_o) + (rec * 32 + 2 * blockIdx.z) * kRecordRows + r0,
+                              int64_t(P.hkv) * kRecordRows, int64_t(P.hkv) * 32 * kRecordRows, kRecordRows, m.n, rows);
+  const int row = threadIdx.x >> 3;
+  if (row >= rows) return;
+  const int i = t * tile_rows + (r0 & 127) + row;
+  const int64_t at = ((int64_t(m.q_row) + i / P.group) * P.hq + kvh * P.group + i % P.group) * kD + 8 * blockIdx.z +
+                     (threadIdx.x & 7);
+  P.out[at] = uint16_t(pack2<kBf16>(v, 0.0f));
 }
 
 // ----------------------------------------------------------------------------- host
@@ -434,8 +440,9 @@ static int launch_prompt(const PromptParams& P, const tp_prompt_plan& plan, cuda
   if (plan.items)
     prompt_attention_kernel<kBf16><<<unsigned(plan.items) * plan.num_kv_heads, kPromptThreads, kPromptSmem, s>>>(P);
   if (plan.merges) {
-    const int rows = plan.block_tokens * P.group;
-    e = launch_dependent(merge_items_kernel<kBf16>, dim3(unsigned(plan.merges) * plan.num_kv_heads, (rows + 7) / 8), 256, s, P);
+    const int rows = plan.block_tokens > P.tile_tokens ? kRecordRows : plan.block_tokens * P.group;
+    e = launch_dependent(merge_items_kernel<kBf16>, dim3(unsigned(plan.merges) * plan.num_kv_heads, (rows + 31) / 32, kD / 8),
+                         kMergeThreads, s, P);
     if (e != cudaSuccess) return fail(TP_ERR_CUDA, std::string("tp_prompt_attention: ") + cudaGetErrorString(e));
   }
   return check_launch("tp_prompt_attention");

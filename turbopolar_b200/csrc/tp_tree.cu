@@ -39,7 +39,8 @@ constexpr int kTreeSoftmaxRegs = 128, kTreeDecodeRegs = 88, kTreeIssueRegs = 48;
 constexpr int kOffBits = kTreeStages * kTreeStage;    // [2][128][4] uint64: drafts that a row sees
 constexpr int kOffTab = kOffBits + 2 * 128 * 4 * 8;   // float2[512]
 constexpr int kOffMl = kOffTab + 512 * 8;             // [2 pieces][2 warpgroups][128] float2
-constexpr int kOffLate = kOffMl + 2 * 2 * 128 * 8;    // [kLateRing][8] words
+constexpr int kOffBuf = kOffMl + 2 * 2 * 128 * 8;     // 2 KB per softmax warp: rows on their way in and out
+constexpr int kOffLate = kOffBuf + 8 * kStageRows;    // [kLateRing][8] words
 constexpr int kOffTreeBars = kOffLate + kLateRing * 32;
 constexpr int kTreeSmem = kOffTreeBars + 256;
 
@@ -62,7 +63,7 @@ struct TreeParams {
   const uint8_t* mask;
   int64_t mask_b, mask_t;
   __half* out;                              // [batch][drafts][hq][128]
-  float* rec_o;                             // [piece][record rows][128]
+  float* rec_o;                             // [piece][32][record rows][4]: channel / 4, row
   float2* rec_ml;
   int rec_rows;
   int* error;
@@ -78,6 +79,14 @@ struct PageRegs {
   uint2 code[2];
   uint32_t scale[2][2];
   float rscale;
+};
+
+// Unit layout of the two specialised formats (make_layout checks the sizes of any format): offsets
+// known to the compiler become part of the load instructions.
+template <int kMode>
+struct UnitOf {
+  static constexpr int vcodes = kMode == kTreeDefault ? 4096 : 2048, codes = vcodes + 4096,
+                       vscales = codes + (kMode == kTreeDefault ? 1024 : 2048), bytes = vscales + 256;
 };
 
 __device__ __forceinline__ uint4 ldg16(const void* p) {
@@ -98,33 +107,37 @@ __device__ __forceinline__ uint32_t ldg4(const void* p) {
   return r;
 }
 
+// `pg`: the page block; `rscale`: where its radius scale is (int8 radii).
 template <int kMode>
-__device__ __forceinline__ void load_page(PageRegs& R, const PoolArgs& L, int head, int page, int tid) {
-  const uint8_t* pg = L.pages + (int64_t(head) * L.page_capacity + page) * L.page_bytes;
+__device__ __forceinline__ void load_page(PageRegs& R, const PoolArgs& L, const uint8_t* pg, const __half* rscale, int tid) {
   const int warp = tid >> 5, lane = tid & 31, c = tid & 7, l = tid >> 3;
+  const int ub = kMode == kTreeGeneral ? L.unit_bytes : UnitOf<kMode>::bytes;
+  const int vc = kMode == kTreeGeneral ? L.u_vcodes : UnitOf<kMode>::vcodes;
+  const int vs = kMode == kTreeGeneral ? L.u_vscales : UnitOf<kMode>::vscales;
   if (kMode != kTreeGeneral) {
+    const uint8_t* rad = pg + (kMode == kTreeDefault ? radii_f16_offset(l, 8 * c) : l * 64 + 8 * c);
+    const uint8_t* code = pg + UnitOf<kMode>::codes + (kMode == kTreeDefault ? l * 32 + 4 * c : l * 64 + 8 * c);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const uint8_t* un = pg + u * L.unit_bytes;
       if (kMode == kTreeDefault) {
-        R.rad[u] = ldg16(un + radii_f16_offset(l, 8 * c));
-        R.code[u].x = ldg4(un + L.u_codes + l * 32 + 4 * c);
+        R.rad[u] = ldg16(rad + u * ub);
+        R.code[u].x = ldg4(code + u * ub);
       } else {
-        const uint2 r8 = ldg8(un + l * 64 + 8 * c);
+        const uint2 r8 = ldg8(rad + u * ub);
         R.rad[u].x = r8.x, R.rad[u].y = r8.y;
-        R.code[u] = ldg8(un + L.u_codes + l * 64 + 8 * c);
+        R.code[u] = ldg8(code + u * ub);
       }
     }
   }
-  const uint8_t* un = pg + (warp >> 2) * L.unit_bytes;
+  const uint8_t* v = pg + (warp >> 2) * ub + vc + (warp & 3) * 512 + lane * 16;
+  const uint8_t* sc = pg + (warp >> 2) * ub + vs + ((lane & 3) * 16 + (warp & 3) * 2) * 2;
 #pragma unroll
   for (int kk = 0; kk < 2; ++kk) {
-    R.v[kk] = ldg16(un + L.u_vcodes + kk * 2048 + (warp & 3) * 512 + lane * 16);
+    R.v[kk] = ldg16(v + kk * 2048);
 #pragma unroll
-    for (int a = 0; a < 2; ++a)
-      R.scale[kk][a] = ldg4(un + L.u_vscales + (kk * 64 + (lane & 3) * 16 + a * 8 + (warp & 3) * 2) * 2);
+    for (int a = 0; a < 2; ++a) R.scale[kk][a] = ldg4(sc + kk * 128 + a * 16);
   }
-  R.rscale = L.int8_radii ? __half2float(L.radii_scales[int64_t(head) * L.page_capacity + page]) : 0.0f;
+  if (kMode != kTreeDefault) R.rscale = rscale ? __half2float(*rscale) : 0.0f;
 }
 
 __device__ __forceinline__ void st16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -152,7 +165,7 @@ __device__ __forceinline__ void store_pairs(uint32_t k_tile, int row, int c, con
 // values of the others are cleared (their weights are 0, and 0 times a non-finite value is NaN).
 template <int kMode>
 __device__ __forceinline__ void decode_step(const PageRegs& R, const PoolArgs& L, const float2* tab, uint32_t stage,
-                                            int head, int page, int limit, int tid) {
+                                            const uint8_t* pg, int limit, int tid) {
   const int warp = tid >> 5, lane = tid & 31, c = tid & 7, l = tid >> 3;
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
@@ -176,7 +189,7 @@ __device__ __forceinline__ void decode_step(const PageRegs& R, const PoolArgs& L
         w[i] = pack_h2(r * cs.x, r * cs.y);
       }
     } else {
-      const uint8_t* un = L.pages + (int64_t(head) * L.page_capacity + page) * L.page_bytes + u * L.unit_bytes;
+      const uint8_t* un = pg + u * L.unit_bytes;
       const uint8_t* row = un + L.u_codes + l * L.code_row;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -212,10 +225,18 @@ __device__ __forceinline__ void decode_step(const PageRegs& R, const PoolArgs& L
 #pragma unroll
         for (int e = 0; e < 2; ++e)
           o[e] = h2_as_u32(__hmul2(__hsub2(u32_as_h2(prmt(words[2 * a + e], 0x64646464u, b ? 0x4341u : 0x4240u)), bias), s2));
-        if (in_page >= limit) o[0] = o[1] = 0;
         const int chunk = (G & 1) * 4 + (g >> 1);
         st8(v_tile + (G >> 1) * kKvHalf + in_page * 128 + ((chunk ^ (in_page & 7)) << 4) + (g & 1) * 8, o[0], o[1]);
       }
+    }
+  }
+  if (limit < kTreeKeys) {  // this thread's values again, where they are not seen
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int in_page = u * 32 + (i >> 2) * 16 + (i >> 1 & 1) * 8 + 2 * t + (i & 1);
+      const int chunk = (G & 1) * 4 + (g >> 1);
+      if (in_page >= limit)
+        st8(v_tile + (G >> 1) * kKvHalf + in_page * 128 + ((chunk ^ (in_page & 7)) << 4) + (g & 1) * 8, 0, 0);
     }
   }
 }
@@ -312,6 +333,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
     const uint32_t s_addr = kTreeScoreCol + 64 * w + lanes;
     uint64_t* bits = reinterpret_cast<uint64_t*>(smem + kOffBits) + (w * 128 + r0) * 4;
     float2* ml = reinterpret_cast<float2*>(smem + kOffMl);
+    uint8_t* buf = smem + kOffBuf + warp * kStageRows;
     int units = 0, piece = 0, draft_pieces = 0;
     bool ok = true;
     for (int done = 0, seg = seg0, a = step0; done < count && ok; ++piece, ++seg, a = 0) {
@@ -323,15 +345,30 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
       const int g = valid ? r / P.drafts : 0, t = valid ? r - g * P.drafts : 0;
       const int64_t q_at = batch * P.q_b + (int64_t(kvh) * P.group + g) * P.q_h + t * P.q_t;
       if (kPair || w == 0) {
+        // Four lanes to a row, all loads in flight, then 64 bytes of every row at a time through `buf`.
+        uint4 x[4][4];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          uint32_t x[32];
+        for (int i = 0; i < 4; ++i) {
+          const int from = 8 * i + (lane >> 2);
+          const int64_t at = __shfl_sync(0xffffffffu, q_at, from);
+          const bool there = __shfl_sync(0xffffffffu, int(valid), from);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const uint4 v = valid ? dense_chunk(P.q, q_at + half * 64 + 8 * i, P.q_f32) : make_uint4(0, 0, 0, 0);
-            x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
+          for (int p = 0; p < 4; ++p)
+            x[i][p] = there ? dense_chunk(P.q, at + 32 * p + 8 * (lane & 3), P.q_f32) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) *staged(buf, 8 * i + (lane >> 2), lane & 3) = x[i][p];
+          __syncwarp();
+          uint32_t y[16];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint4 v = *staged(buf, lane, i);
+            y[4 * i] = v.x, y[4 * i + 1] = v.y, y[4 * i + 2] = v.z, y[4 * i + 3] = v.w;
           }
-          tmem_st32(64 * w + lanes + 32 * half, x);
+          __syncwarp();
+          tmem_st16(64 * w + lanes + 16 * p, y);
         }
         tmem_wait_st();
       }
@@ -409,14 +446,17 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
                                 : w0 * (w == 0 ? row.sum : other.y) + w1 * (w == 0 ? other.y : row.sum);
         const bool whole = a == 0 && b == P.n_steps;
         const float inv = !whole ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
-        const int64_t rec = (int64_t(blockIdx.x) + seg) * P.rec_rows + (r - rg * kGroupRows);
+        const int64_t rec = int64_t(blockIdx.x) + seg;
+        const int in_rec = r - rg * kGroupRows;
         const int64_t out_at = ((int64_t(batch) * P.drafts + t) * P.hq + int64_t(kvh) * P.group + g) * kD;
+        uint8_t* dst = valid ? reinterpret_cast<uint8_t*>(P.out + out_at) : nullptr;
         const uint32_t* late = late_ring + (draft_pieces & (kLateRing - 1)) * 8;
         bool listed = false;
         if (b > draft0)
           for (int i = 0; i < (P.drafts + 31) >> 5; ++i) listed |= late[i] != 0;
         const int c_begin = kPair ? 0 : 64 * w, c_end = kPair ? kD : 64 * w + 64;
         const uint32_t o0 = kTreeOutCol + (kPair ? 128 * w : 0) + lanes, o1 = kTreeOutCol + 128 + lanes;
+#pragma unroll 1
         for (int c = c_begin; c < c_end; c += 32) {
           float o[32], x[32];
 #pragma unroll
@@ -443,26 +483,27 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
                 float dot = 0.0f;
                 for (int i = 0; i < kD; ++i) dot = fmaf(load_any(P.q, q_at + i, P.q_f32), load_any(P.k, k_at + i, P.kv_f32), dot);
                 const float p = exp2_approx(fmaf(dot, P.scale_log2, -base));
-  #pragma unroll 4
+#pragma unroll
                 for (int i = 0; i < 32; ++i) o[i] = fmaf(p, load_any(P.v, v_at + c + i, P.kv_f32), o[i]);
               }
             }
-            if (whole) {
-              uint4* dst = reinterpret_cast<uint4*>(P.out + out_at + c);
-  #pragma unroll
-              for (int i = 0; i < 4; ++i)
-                dst[i] = make_uint4(pack_h2(o[8 * i] * inv, o[8 * i + 1] * inv), pack_h2(o[8 * i + 2] * inv, o[8 * i + 3] * inv),
-                                    pack_h2(o[8 * i + 4] * inv, o[8 * i + 5] * inv),
-                                    pack_h2(o[8 * i + 6] * inv, o[8 * i + 7] * inv));
-            } else {
-              float4* dst = reinterpret_cast<float4*>(P.rec_o + rec * kD + c);
-  #pragma unroll
-              for (int i = 0; i < 8; ++i) dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-            }
+          }
+          __syncwarp();
+          if (whole) {
+            uint32_t y[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) y[i] = pack_h2(o[2 * i] * inv, o[2 * i + 1] * inv);
+            store_rows64(buf, y, dst ? dst + 2 * c : nullptr);
+          } else {
+            float4* to = reinterpret_cast<float4*>(P.rec_o) + (rec * 32 + c / 4) * P.rec_rows + in_rec;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (valid) to[i * P.rec_rows] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
           }
           __syncwarp();
         }
-        if (!whole && valid && (kPair || w == 0)) P.rec_ml[rec] = make_float2(kPair ? row.ref : top, sum);
+        if (!whole && valid && (kPair || w == 0)) 
+          P.rec_ml[rec * P.rec_rows + in_rec] = make_float2(kPair ? row.ref : top, sum);
       }
       tmem_fence_before();
       if (b > draft0) ++draft_pieces;
@@ -472,45 +513,61 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
     fewer_registers<kTreeDecodeRegs>();
     const int tid = threadIdx.x - 256;
     const uint32_t stages = smem_u32(smem);
-    PageRegs next;
-    int seg = seg0, s = step0, scans = 0, draft_pieces = 0;
+    // Cursor over the CTA's steps: `pg` is the page of step s while s < n_page_steps.
+    int s = step0, seg = seg0, head = seg0 / P.row_groups;
+    const uint8_t* pg = P.pool.pages + (int64_t(head) * P.pool.page_capacity + s) * P.pool.page_bytes;
+    const __half* rs = P.pool.int8_radii ? P.pool.radii_scales + int64_t(head) * P.pool.page_capacity + s : nullptr;
+    int i = 0, st = 0, ph = 1, scans = 0, draft_pieces = 0;  // ph: parity of the stage's last release
     bool ok = true;
-    auto prefetch = [&](int ahead) {  // page of the step `ahead` steps on, into L2
-      int ps = s + ahead, pseg = seg;
-      if (ps >= P.n_steps) ps -= P.n_steps, ++pseg;
-      if (ps < P.n_page_steps) {
-        const uint8_t* pg = P.pool.pages + (int64_t(pseg / P.row_groups) * P.pool.page_capacity + ps) * P.pool.page_bytes;
-        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(pg), "r"(P.pool.page_bytes) : "memory");
-      }
-    };
+    // One page a few steps ahead is fetched into L2, so that the loads one step ahead come from there.
     constexpr int kAhead = 6;
-    if (tid == 0)
-      for (int i = 1; i < min(kAhead, count); ++i)
-        if (i < P.n_steps) prefetch(i);
-    if (count && s < P.n_page_steps) load_page<kMode>(next, P.pool, seg / P.row_groups, s, tid);
-    for (int i = 0; i < count && ok; ++i) {
-      const int st = i % kTreeStages, use = i / kTreeStages;
+    if (tid < min(kAhead, count) && s + tid < P.n_page_steps)
+      asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(pg + int64_t(tid) * P.pool.page_bytes),
+                   "r"(P.pool.page_bytes)
+                   : "memory");
+    // Step i: its page is in `use`; the next step's page goes to `fetch`.  False after the last step.
+    auto step = [&](PageRegs& use, PageRegs& fetch) {
+      const uint8_t* now = pg;
+      const int at = s, h = head;
+      const __half* ahead_rs = rs;
+      const uint8_t* ahead = pg;
+      if (s + 1 < P.n_steps) {
+        ++s;
+        ahead += P.pool.page_bytes;
+        if (rs) ++ahead_rs;
+        if (tid == 0 && s + kAhead - 1 < P.n_page_steps && i + kAhead < count)
+          asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(now + int64_t(kAhead) * P.pool.page_bytes),
+                       "r"(P.pool.page_bytes)
+                       : "memory");
+      } else {
+        s = 0;
+        ++seg;
+        head = seg / P.row_groups;
+        ahead = P.pool.pages + int64_t(head) * P.pool.page_capacity * P.pool.page_bytes;
+        if (rs) ahead_rs = P.pool.radii_scales + int64_t(head) * P.pool.page_capacity;
+        if (tid < kAhead && tid < P.n_page_steps && i + 1 + tid < count)
+          asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(ahead + int64_t(tid) * P.pool.page_bytes),
+                       "r"(P.pool.page_bytes)
+                       : "memory");
+      }
+      pg = ahead;
+      rs = ahead_rs;
+      if (i + 1 < count && s < P.n_page_steps) load_page<kMode>(fetch, P.pool, pg, rs, tid);
       const uint32_t stage = stages + st * kTreeStage;
-      const int head = seg / P.row_groups;
-      const PageRegs now = next;
-      int ns = s + 1, nseg = seg;
-      if (ns == P.n_steps) ns = 0, ++nseg;
-      if (tid == 0 && i + kAhead < count && kAhead < P.n_steps) prefetch(kAhead);
-      if (i + 1 < count && ns < P.n_page_steps) load_page<kMode>(next, P.pool, nseg / P.row_groups, ns, tid);
-      ok = use == 0 || wait_bar(kv_empty + st, (use - 1) & 1, stop);
+      ok = i < kTreeStages || wait_bar(kv_empty + st, ph, stop);
       ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      if (s < P.n_page_steps) {
-        decode_step<kMode>(now, P.pool, tab, stage, head, s, P.visible - s * kTreeKeys, tid);
-      } else if (s < draft0) {
-        const int64_t at = int64_t(head) * kPage * kD * (P.tail_f32 ? 4 : 2);
-        dense_step(stage, static_cast<const uint8_t*>(P.tail_k) + at, static_cast<const uint8_t*>(P.tail_v) + at, kD, kD,
+      if (!ok) return false;
+      if (at < P.n_page_steps) {
+        decode_step<kMode>(use, P.pool, tab, stage, now, P.visible - at * kTreeKeys, tid);
+      } else if (at < draft0) {
+        const int64_t row0 = int64_t(h) * kPage * kD * (P.tail_f32 ? 4 : 2);
+        dense_step(stage, static_cast<const uint8_t*>(P.tail_k) + row0, static_cast<const uint8_t*>(P.tail_v) + row0, kD, kD,
                    P.tail_f32, P.tail_len, nullptr, tid);
       } else {
-        const int batch = head / P.hkv, kvh = head - batch * P.hkv, d0 = (s - draft0) * kTreeKeys;
+        const int batch = h / P.hkv, kvh = h - batch * P.hkv, d0 = (at - draft0) * kTreeKeys;
         const int size = P.kv_f32 ? 4 : 2;
         uint32_t* late = late_ring + (draft_pieces & (kLateRing - 1)) * 8;
-        if (tid < 8 && (s == draft0 || i == 0)) late_ring[((draft_pieces + kLateRing / 2) & (kLateRing - 1)) * 8 + tid] = 0;
+        if (tid < 8 && (at == draft0 || i == 0)) late_ring[((draft_pieces + kLateRing / 2) & (kLateRing - 1)) * 8 + tid] = 0;
         const int n = min(kTreeKeys, P.drafts - d0);
         dense_step(stage, static_cast<const uint8_t*>(P.k) + (batch * P.k_b + kvh * P.k_h + d0 * P.k_t) * size,
                    static_cast<const uint8_t*>(P.v) + (batch * P.v_b + kvh * P.v_h + d0 * P.v_t) * size, P.k_t, P.v_t,
@@ -518,20 +575,24 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
         __syncwarp();
         if (lane == 0) mbar_arrive(scanned);
         ok = __all_sync(0xffffffffu, wait_bar(scanned, scans & 1, stop));
-        if (!ok) break;
+        if (!ok) return false;
         ++scans;
         for (int q = 0; q < 4; ++q) {
           const int row = q * 16 + (tid >> 4);
           if (late[(d0 >> 5) + (row >> 5)] >> (row & 31) & 1)
             st16(stage + 2 * kKvHalf + tile_chunk(row, tid & 15, kTreeKeys), 0, 0, 0, 0);
         }
-        if (s == P.n_steps - 1) ++draft_pieces;
+        if (at == P.n_steps - 1) ++draft_pieces;
       }
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(kv_full + st);
-      s = ns;
-      seg = nseg;
+      if (++st == kTreeStages) st = 0, ph ^= 1;
+      return ++i < count;
+    };
+    PageRegs even, odd;
+    if (count && s < P.n_page_steps) load_page<kMode>(even, P.pool, pg, rs, tid);
+    while (step(even, odd) && step(odd, even)) {
     }
   } else if (fewer_registers<kTreeIssueRegs>(); warp == 16) {
     constexpr uint32_t kScores = mma_idesc(false, kTreeKeys, false), kOut = mma_idesc(false, kD, true);
@@ -603,11 +664,10 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
   if (threadIdx.x == 0 && *stop) *P.error = 1;
 }
 
-// Rows of segments that several CTAs worked on, one warp per row.
-__global__ void __launch_bounds__(256) merge_pieces_kernel(const __grid_constant__ TreeParams P) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+// Rows of segments that several CTAs worked on: 32 rows x 8 channels per block.
+__global__ void __launch_bounds__(kMergeThreads) merge_pieces_kernel(const __grid_constant__ TreeParams P) {
   const int seg = blockIdx.x, head = seg / P.row_groups, rg = seg - head * P.row_groups;
-  const int i = blockIdx.y * 8 + warp, r = rg * kGroupRows + i;
+  const int i0 = blockIdx.y * 32, rows = min(32, min(kGroupRows, P.rows - rg * kGroupRows) - i0);
   // CTAs whose ranges meet the segment's steps [f0, f1).
   const int64_t f0 = int64_t(seg) * P.n_steps, f1 = f0 + P.n_steps;
   int first = int(f0 * P.grid / P.total);
@@ -615,13 +675,17 @@ __global__ void __launch_bounds__(256) merge_pieces_kernel(const __grid_constant
   int last = int((f1 - 1) * P.grid / P.total);
   while (range_begin(P, last + 1) < f1) ++last;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (i >= kGroupRows || r >= P.rows || first == last) return;  // one CTA: it has written the rows
-  const int64_t rec0 = (int64_t(first) + seg) * P.rec_rows + i;
-  const float4 o = merge_row(P.rec_ml + rec0, P.rec_o + rec0 * kD, P.rec_rows, last - first + 1);
+  if (rows <= 0 || first == last) return;  // one CTA: it has written the rows
+  const int64_t rec = int64_t(first) + seg;
+  const float v = merge_block(P.rec_ml + rec * P.rec_rows + i0,
+                              reinterpret_cast<const float4*>(P.rec_o) + (rec * 32 + 2 * blockIdx.z) * P.rec_rows + i0,
+                              P.rec_rows, int64_t(32) * P.rec_rows, P.rec_rows, last - first + 1, rows);
+  const int row = threadIdx.x >> 3;
+  if (row >= rows) return;
+  const int r = rg * kGroupRows + i0 + row;
   const int batch = head / P.hkv, kvh = head - batch * P.hkv, g = r / P.drafts, t = r - g * P.drafts;
-  uint2* dst = reinterpret_cast<uint2*>(P.out + ((int64_t(batch) * P.drafts + t) * P.hq + int64_t(kvh) * P.group + g) * kD +
-                                        4 * lane);
-  *dst = make_uint2(pack_h2(o.x, o.y), pack_h2(o.z, o.w));
+  P.out[((int64_t(batch) * P.drafts + t) * P.hq + int64_t(kvh) * P.group + g) * kD + 8 * blockIdx.z + (threadIdx.x & 7)] =
+      __float2half_rn(v);
 }
 
 // ----------------------------------------------------------------------------- host
@@ -639,7 +703,7 @@ static int launch_tree(const TreeParams& P, int segments, cudaStream_t s) {
   if (e != cudaSuccess) return fail(TP_ERR_CUDA, std::string("tp_tree_attention: ") + cudaGetErrorString(e));
   tree_attention_kernel<kMode, kPair><<<P.grid, kTreeThreads, kTreeSmem, s>>>(P);
   if (P.grid > 1) {
-    e = launch_dependent(merge_pieces_kernel, dim3(segments, (P.rec_rows + 7) / 8), 256, s, P);
+    e = launch_dependent(merge_pieces_kernel, dim3(segments, (P.rec_rows + 31) / 32, kD / 8), kMergeThreads, s, P);
     if (e != cudaSuccess) return fail(TP_ERR_CUDA, std::string("tp_tree_attention: ") + cudaGetErrorString(e));
   }
   return check_launch("tp_tree_attention");

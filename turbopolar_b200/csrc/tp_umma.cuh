@@ -249,27 +249,34 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   return d;
 }
 
-// 2^x of two numbers below +inf on the multiply-add pipe: the special-function unit makes 16
-// exponentials a cycle, as many as a tile's products leave time for, so part of them is made here.
-// x = n + f with f in [-1/2, 1/2]; 2^f by a polynomial of degree 4 whose coefficients minimise the
-// largest relative error, 2.6e-6 (weights are rounded to 2^-12 or 2^-9 afterwards); n goes into the
-// exponent.  Below 2^-125: 0.
-__device__ __forceinline__ void exp2_poly(uint64_t x, float& e0, float& e1) {
-  constexpr float kRound = 12582912.0f;  // 1.5 * 2^23: adding it rounds to an integer in the low bits
-  const uint64_t t = add_pair(x, pair_of(kRound, kRound));
-  const uint64_t n = add_pair(t, pair_of(-kRound, -kRound));
-  const uint64_t f = fma_pair(n, pair_of(-1.0f, -1.0f), x);
+// 2^x of two numbers x <= 8 on the multiply-add pipe (the special-function unit takes 8 cycles for a
+// warp's exponential, which alone would make the softmax as long as the products).  Takes
+// y = x / 256 + 248 / 256 clamped to [0, 1], so x < -248 (masked scores too) counts as -248.  x = n + f
+// with f in [-1/2, 1/2]; 2^f by a polynomial of degree 4 whose coefficients minimise the largest
+// relative error, 2.6e-6; n is added to the exponent, and a result whose exponent falls below the
+// normal range is negative as an integer and becomes 0.  The 24 bits of y limit x to 2^-16, so the
+// result is off by 2^-15 at most (weights are rounded to 2^-11 or 2^-8 afterwards).
+__device__ __forceinline__ void exp2_poly(float y0, float y1, float& e0, float& e1) {
+  constexpr float kMagic = 12582912.0f - 248.0f;  // 1.5 * 2^23: adding it rounds to an integer in the low bits
+  const uint64_t y = pair_of(y0, y1), k256 = pair_of(256.0f, 256.0f);
+  const uint64_t t = fma_pair(y, k256, pair_of(kMagic, kMagic));
+  const uint64_t n = fma_pair(t, pair_of(-1.0f, -1.0f), pair_of(kMagic, kMagic));
+  const uint64_t f = fma_pair(y, k256, n);
   uint64_t p = pair_of(0.009570102207362652f, 0.009570102207362652f);
   p = fma_pair(p, f, pair_of(0.05591785907745361f, 0.05591785907745361f));
   p = fma_pair(p, f, pair_of(0.240247443318367f, 0.240247443318367f));
   p = fma_pair(p, f, pair_of(0.6931217908859253f, 0.6931217908859253f));
   p = fma_pair(p, f, pair_of(0.9999992847442627f, 0.9999992847442627f));
-  float x0, x1, t0, t1, p0, p1;
-  split_pair(x, x0, x1);
+  float t0, t1, p0, p1;
   split_pair(t, t0, t1);
   split_pair(p, p0, p1);
-  e0 = x0 < -125.0f ? 0.0f : __int_as_float(__float_as_int(p0) + (__float_as_int(t0) << 23));
-  e1 = x1 < -125.0f ? 0.0f : __int_as_float(__float_as_int(p1) + (__float_as_int(t1) << 23));
+  e0 = __int_as_float(max(0, __float_as_int(t0) * (1 << 23) + __float_as_int(p0)));
+  e1 = __int_as_float(max(0, __float_as_int(t1) * (1 << 23) + __float_as_int(p1)));
+}
+__device__ __forceinline__ float fma_sat(float a, float b, float c) {
+  float d;
+  asm("fma.rn.sat.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 // Pairs of a tile's columns that take the polynomial.
 constexpr int kPolyPairs = 3;
@@ -343,18 +350,18 @@ __device__ __forceinline__ bool softmax_tile(SoftmaxRow& row, uint32_t s_addr, u
   }
   const float base = row.ref == -INFINITY ? 0.0f : -row.ref;
   const uint64_t scale2 = pair_of(scale_log2, scale_log2), base2 = pair_of(base, base);
+  const float scale_256 = scale_log2 * (1.0f / 256.0f), base_256 = (base + 248.0f) * (1.0f / 256.0f);
   uint64_t add[2] = {0, 0};
 #pragma unroll
   for (int c = 0; c < kCols; c += 32) {
     uint32_t w[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const uint64_t x = fma_pair(pair_of(s[c + 2 * i], s[c + 2 * i + 1]), scale2, base2);
       float e0, e1;
       if (poly_pair(i)) {
-        exp2_poly(x, e0, e1);
+        exp2_poly(fma_sat(s[c + 2 * i], scale_256, base_256), fma_sat(s[c + 2 * i + 1], scale_256, base_256), e0, e1);
       } else {
-        split_pair(x, e0, e1);
+        split_pair(fma_pair(pair_of(s[c + 2 * i], s[c + 2 * i + 1]), scale2, base2), e0, e1);
         e0 = exp2_approx(e0);
         e1 = exp2_approx(e1);
       }
@@ -371,49 +378,93 @@ __device__ __forceinline__ bool softmax_tile(SoftmaxRow& row, uint32_t s_addr, u
   return true;
 }
 
-// ----------------------------------------------------------------------------- merging split rows
-// Four channels (4 * lane ..) of a row whose keys were split: records (ref_k, sum_k) at ml[k * step]
-// and unnormalised outputs at o[k * step * 128 + 4 * lane].  M = max ref_k, w_k = 2^(ref_k - M),
-// sum w_k o_k / sum w_k sum_k; 0 where no record has seen a key.  One warp; each lane makes the
-// weights of every 32nd record, and the outputs of eight records are loaded at a time.
-__device__ __forceinline__ float4 merge_row(const float2* ml, const float* o, int64_t step, int n) {
+// ----------------------------------------------------------------------------- rows in and out
+// A warp's 32 rows of 64 bytes through 2 KB of shared memory, so that global memory is read and written
+// four lanes to a row: chunk c (16 bytes) of row r sits at r * 64 + ((c ^ (r >> 1 & 3)) << 4), free of
+// bank conflicts by rows and by columns.
+constexpr int kStageRows = 2048;
+__device__ __forceinline__ uint4* staged(uint8_t* buf, int row, int chunk) {
+  return reinterpret_cast<uint4*>(buf + row * 64 + ((chunk ^ (row >> 1 & 3)) << 4));
+}
+// Write 64 bytes `w` per lane to the lane's own address `dst` (skipped where it is NULL).
+__device__ __forceinline__ void store_rows64(uint8_t* buf, const uint32_t (&w)[16], uint8_t* dst) {
   const int lane = threadIdx.x & 31;
-  float top = -INFINITY;
-  for (int k = lane; k < n; k += 32) top = fmaxf(top, ml[k * step].x);
 #pragma unroll
-  for (int i = 16; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
-  const float base = top == -INFINITY ? 0.0f : top;
-  float l = 0.0f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int k0 = 0; k0 < n; k0 += 32) {
-    float w = 0.0f;
-    if (k0 + lane < n) {
-      const float2 r = ml[(k0 + lane) * step];
-      w = exp2_approx(r.x - base);
-      l = fmaf(w, r.y, l);
-    }
-    const int m = min(32, n - k0);
-    for (int k = 0; k < m; k += 8) {
-      float4 v[8];
+  for (int i = 0; i < 4; ++i) *staged(buf, lane, i) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+  __syncwarp();
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        v[i] = k + i < m ? *reinterpret_cast<const float4*>(o + (k0 + k + i) * step * kD + 4 * lane)
-                         : make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = 0; i < 4; ++i) {
+    const int row = 8 * i + (lane >> 2);
+    uint8_t* to = reinterpret_cast<uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), row));
+    if (to) reinterpret_cast<uint4*>(to)[lane & 3] = *staged(buf, row, lane & 3);
+  }
+  __syncwarp();
+}
+
+// ----------------------------------------------------------------------------- merging split rows
+// Partial records of rows whose keys were split over items: unnormalised outputs
+// o[record][channel / 4][row][4] (a warp's 32 rows write whole lines) and (reference, sum) ml[record][row].
+//   M = max ref_k, w_k = 2^(ref_k - M), out = sum w_k o_k / sum w_k sum_k, 0 where nothing was seen.
+// A block of eight warps merges 32 rows x 8 channels: lane = row, warps take every eighth record with
+// all their loads in flight, and a second step adds the warps' parts.  `o`, `ml`: of the first record,
+// the block's first row and channel; `rows` live rows of the block.  Thread i returns channel i % 8
+// of row i / 8.
+constexpr int kMergeThreads = 256;
+__device__ __forceinline__ float merge_block(const float2* ml, const float4* o, int64_t ml_step, int64_t o_step,
+                                             int64_t quad_step, int n, int rows) {
+  __shared__ float part[8][10][33];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float ref = -INFINITY, sum = 0.0f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (lane < rows) {
+    for (int k0 = warp; k0 < n; k0 += 32) {  // four records of this warp at a time
+      float2 r[4];
+      float4 x[4], y[4];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float wi = __shfl_sync(0xffffffffu, w, (k + i) & 31);
-        if (k + i >= m) break;
-        acc.x = fmaf(wi, v[i].x, acc.x);
-        acc.y = fmaf(wi, v[i].y, acc.y);
-        acc.z = fmaf(wi, v[i].z, acc.z);
-        acc.w = fmaf(wi, v[i].w, acc.w);
+      for (int i = 0; i < 4; ++i) {
+        const int k = k0 + 8 * i;
+        r[i] = make_float2(-INFINITY, 0.0f);
+        if (k < n) {
+          r[i] = ml[k * ml_step + lane];
+          x[i] = o[k * o_step + lane];
+          y[i] = o[k * o_step + quad_step + lane];
+        }
+      }
+      const float top = fmaxf(fmaxf(fmaxf(r[0].x, r[1].x), fmaxf(r[2].x, r[3].x)), ref);
+      const float base = top == -INFINITY ? 0.0f : top;
+      const float f = exp2_approx(ref - base);
+      ref = top;
+      sum *= f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[i] *= f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (k0 + 8 * i >= n) break;
+        const float w = exp2_approx(r[i].x - base);
+        sum = fmaf(w, r[i].y, sum);
+        const float v[8] = {x[i].x, x[i].y, x[i].z, x[i].w, y[i].x, y[i].y, y[i].z, y[i].w};
+#pragma unroll
+        for (int c = 0; c < 8; ++c) acc[c] = fmaf(w, v[c], acc[c]);
       }
     }
   }
+  part[warp][0][lane] = ref;
+  part[warp][1][lane] = sum;
 #pragma unroll
-  for (int i = 16; i > 0; i >>= 1) l += __shfl_xor_sync(0xffffffffu, l, i);
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  return make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+  for (int c = 0; c < 8; ++c) part[warp][2 + c][lane] = acc[c];
+  __syncthreads();
+  const int row = threadIdx.x >> 3, c = threadIdx.x & 7;
+  float top = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) top = fmaxf(top, part[k][0][row]);
+  const float base = top == -INFINITY ? 0.0f : top;
+  float l = 0.0f, v = 0.0f;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const float w = exp2_approx(part[k][0][row] - base);
+    l = fmaf(w, part[k][1][row], l);
+    v = fmaf(w, part[k][2 + c][row], v);
+  }
+  return l == 0.0f ? 0.0f : v / l;
 }
 
 // Launch a kernel as the programmatic dependent of the previous one in the stream (which lets it
