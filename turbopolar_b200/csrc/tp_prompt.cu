@@ -12,12 +12,12 @@
 //   warps 0-3, 4-7   softmax of tile 0 / 1, one row per thread; output of the rows
 //   warp 8           issues the products
 //   warp 9           loads tiles (TMA) into a ring of five 32 KB stages: K0 V0 K1 V1 ...
-//   warps 10, 11     complete the warpgroup (registers are moved per warpgroup)
+//   warps 10, 11     clean value tiles that some row does not see whole
 //
 // Values that no row may see: keys past the item's range in its last tile belong to another
-// sequence, and a masked weight of 0 times an infinity or NaN is NaN.  The loader clears such rows
-// of the last tile, and in tiles that some row sees only part of it also clears rows with
-// non-finite values and lists them; rows that do see a listed key add it at the end.
+// sequence, and a masked weight of 0 times an infinity or NaN is NaN.  Such rows of the last tile are
+// cleared before its product, and in tiles that some row sees only part of, rows with non-finite
+// values that not every row sees are cleared and marked; rows that do see a marked key add it at the end.
 //
 // Long key ranges with few query rows are split into several items; their unnormalised rows are merged by
 // merge_items_kernel.
@@ -33,12 +33,12 @@ namespace tp {
 
 constexpr int kKeys = 128;               // keys per tile
 constexpr int kRing = 5;                 // K and V tiles in flight
-constexpr int kMaxLate = 384;            // keys of the partly visible tiles of one item: 127 + 255 at most
+constexpr int kPartial = 3;              // partly visible tiles of one item at most: 127 + 255 keys
 // Three warpgroups at 168 registers: 504 in all, of which the softmax threads, with a row of scores
 // each, take 208 and the others 88.
 constexpr int kPromptThreads = 384, kSoftmaxRegs = 208, kIssueRegs = 88;
 constexpr int kPromptBars = 2 * kTileBytes + kRing * kTileBytes;  // byte offset of the barriers
-constexpr int kPromptSmem = kPromptBars + 256 + 2 * kMaxLate;
+constexpr int kPromptSmem = kPromptBars + 512;
 constexpr int kRecordRows = 2 * kTile;   // rows of an item's partial record
 // Tensor memory (a CTA holds all of it, so it starts at column 0): scores of tile t at 128 t.
 constexpr uint32_t kScoreCol = 0, kOutCol = 256;
@@ -82,39 +82,33 @@ __device__ __forceinline__ bool not_finite(uint32_t w) {  // either 16-bit numbe
   return (x & 0xffff0000u) == (e & 0xffff0000u) || (x & 0xffffu) == (e & 0xffffu);
 }
 
-// Clear rows >= `valid` of a value tile; with `scan` also rows that hold a non-finite value, whose
-// places (first + row) are added to the list.  One warp.
+// Rows [first, 128) of a value tile: clear those from `valid` (at most 128) on and those with a non-finite value,
+// whose bits are set in `late`.  Two warps (`which` 0, 1) take pairs of rows in turn, 16 lanes to a row, with
+// eight loads in flight.
 template <bool kBf16>
-__device__ void clean_values(uint8_t* tile, int valid, bool scan, int first, uint16_t* late, int* n_late) {
+__device__ void clean_values(uint8_t* tile, int first, int valid, int which, uint32_t* late) {
   const int lane = threadIdx.x & 31;
   const uint4 zero = make_uint4(0, 0, 0, 0);
-  uint32_t bad[4] = {0, 0, 0, 0};  // rows, the same in every lane
+  uint8_t* at = tile + (lane >> 3 & 1) * kHalfTile + (lane & 7) * 16;  // this lane's chunk of row 0
+  for (int r0 = first + 2 * which; r0 < kKeys; r0 += 32) {
+    uint4 x[8];
 #pragma unroll
-  for (int part = 0; part < 8; ++part) {  // 16 KB halves x groups of 32 rows; four rows per step
-#pragma unroll 4
-    for (int it = 0; it < 8; ++it) {
-      uint4* p = reinterpret_cast<uint4*>(tile) + (part * 8 + it) * 32 + lane;
-      const int row = (part & 3) * 32 + it * 4 + (lane >> 3);
-      bool hit = false;
-      if (row >= valid) {
-        *p = zero;
-      } else if (scan) {
-        const uint4 x = *p;
-        hit = not_finite<kBf16>(x.x) || not_finite<kBf16>(x.y) || not_finite<kBf16>(x.z) || not_finite<kBf16>(x.w);
-      }
-      const uint32_t hits = __ballot_sync(0xffffffffu, hit);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (hits >> (8 * i) & 0xffu) bad[part & 3] |= 1u << (it * 4 + i);
+    for (int i = 0; i < 8; ++i) {
+      const int row = r0 + 4 * i + (lane >> 4);
+      x[i] = zero;
+      if (row < valid) x[i] = *reinterpret_cast<const uint4*>(at + row * 128);
+      else if (row < kKeys) *reinterpret_cast<uint4*>(at + row * 128) = zero;
     }
-  }
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    while (bad[w]) {
-      const int row = w * 32 + __ffs(bad[w]) - 1;
-      bad[w] &= bad[w] - 1;
-      if (lane < 16) *reinterpret_cast<uint4*>(tile + (lane >> 3) * kHalfTile + row * 128 + (lane & 7) * 16) = zero;
-      if (lane == 0) late[(*n_late)++] = uint16_t(first + row);
+    for (int i = 0; i < 8; ++i) {
+      const bool hit = not_finite<kBf16>(x[i].x) || not_finite<kBf16>(x[i].y) || not_finite<kBf16>(x[i].z) ||
+                       not_finite<kBf16>(x[i].w);
+      const uint32_t hits = __ballot_sync(0xffffffffu, hit) >> (lane & 16) & 0xffffu;  // of this lane's row
+      if (hits) {
+        const int row = r0 + 4 * i + (lane >> 4);
+        *reinterpret_cast<uint4*>(at + row * 128) = zero;
+        if ((lane & 15) == 0) atomicOr(late + (row >> 5), 1u << (row & 31));
+      }
     }
   }
 }
@@ -127,13 +121,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
   const int kvh = blockIdx.x % P.hkv;
   uint8_t* ring = smem + 2 * kTileBytes;
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + kPromptBars);
-  uint64_t *full = q_full + 1, *empty = full + kRing, *s_full = empty + kRing, *p_full = s_full + 2,
-           *o_done = p_full + 2, *clean = o_done + 2, *drained = clean + 1;
+  uint64_t *full = q_full + 1, *empty = full + kRing, *s_full = empty + kRing, *p_half = s_full + 2, *p_full = p_half + 2,
+           *o_done = p_full + 2, *asked = o_done + 2, *clean = asked + kPartial, *drained = clean + kPartial;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
-  int* stop_word = reinterpret_cast<int*>(tmem_slot + 1);
-  volatile int* stop = stop_word;
-  int* n_late = stop_word + 1;
-  uint16_t* late = reinterpret_cast<uint16_t*>(smem + kPromptBars + 256);
+  volatile int* stop = reinterpret_cast<int*>(tmem_slot + 1);
+  uint32_t* late = tmem_slot + 2;  // [kPartial][4]: marked keys, from key partial * 128 on
 
   const int n_tiles = (it.k_end - it.k_begin + kKeys - 1) / kKeys;
   const bool two = it.q_tokens > P.tile_tokens;
@@ -149,13 +141,17 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(s_full + i, 1);
+      mbar_init(p_half + i, 4);
       mbar_init(p_full + i, 4);
       mbar_init(o_done + i, 1);
     }
-    mbar_init(clean, 1);
+    for (int i = 0; i < kPartial; ++i) {
+      mbar_init(asked + i, 1);
+      mbar_init(clean + i, 2);
+    }
     mbar_init(drained, 1);
     *stop = 0;
-    *n_late = 0;
+    for (int i = 0; i < 4 * kPartial; ++i) late[i] = 0;
     fence_mbar_init();
   }
   if (warp == 8) tmem_alloc(tmem_slot, 512);
@@ -185,20 +181,28 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
         if (ok && live) {
           tmem_fence_after();
           ok = softmax_tile<kKeys, kBf16>(row, s_addr, o_addr, FirstN{limit - (it.k_begin + j * kKeys)}, P.scale_log2, j == 0,
-                                          [&] { return wait_bar(o_done + t, (j - 1) & 1, stop); });
+                                          [&] { return wait_bar(o_done + t, (j - 1) & 1, stop); },
+                                          [&] {
+                                            tmem_fence_before();
+                                            __syncwarp();
+                                            if (lane == 0) mbar_arrive(p_half + t);
+                                          });
           tmem_fence_before();
+        } else if (ok && lane == 0) {
+          mbar_arrive(p_half + t);
         }
         __syncwarp();
         if (ok && lane == 0) mbar_arrive(p_full + t);
       }
       if (ok && n_tiles) {
         ok = wait_bar(o_done + t, (n_tiles - 1) & 1, stop);
-        if (partial < n_tiles) ok = ok && wait_bar(clean, (n_tiles - partial - 1) & 1, stop);
+        for (int i = 0; i < n_tiles - partial; ++i) ok = ok && wait_bar(clean + i, 0, stop);
         ok = __all_sync(0xffffffffu, ok);
         tmem_fence_after();
       }
       if (ok && live) {
-        const int listed = n_tiles ? *n_late : 0;
+        uint32_t marked = 0;
+        for (int i = 0; i < 4 * kPartial; ++i) marked |= late[i];
         const bool merged = it.slot >= 0;
         const int64_t q_row = int64_t(it.q_row) + tok;
         const int64_t rec = int64_t(it.slot) * P.hkv + kvh;
@@ -214,10 +218,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
 #pragma unroll
             for (int i = 0; i < 32; ++i) o[i] = 0.0f;
           }
-          if (valid) {
-            for (int e = 0; e < listed; ++e) {  // keys with non-finite values that this row sees
-              const int key = it.k_begin + partial * kKeys + late[e];
-              if (key >= limit) continue;
+          if (marked && valid) {  // keys with non-finite values that this row sees
+            for (int e = 0; e < kPartial * kKeys; ++e) {
+              const int key = it.k_begin + partial * kKeys + e;
+              if (key >= limit) break;
+              if (!(late[e >> 5] >> (e & 31) & 1)) continue;
               const uint16_t* qr = P.q + q_row * P.q_t + head * P.q_h;
               const uint16_t* kr = P.k + (int64_t(it.k_row) + key) * P.k_t + kvh * P.k_h;
               const uint16_t* vr = P.v + (int64_t(it.k_row) + key) * P.v_t + kvh * P.v_h;
@@ -276,32 +281,40 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
       for (int j = 0; j < n_tiles && ok; ++j) {
         const int sv = st;
         ok = warp_wait(full + sv, ph, stop);
-        if (ok && j >= partial) ok = warp_wait(clean, (j - partial) & 1, stop);
+        if (ok && j >= partial) ok = warp_wait(clean + j - partial, 0, stop);
         advance();
         const int sk = st;
         const bool more = j + 1 < n_tiles;
-        if (ok && more) {
-          ok = warp_wait(full + sk, ph, stop);
-          advance();
-        }
         const uint32_t v_lo = cols_lo(ring_addr, kHalfTile) + sv * (kTileBytes >> 4);
         for (int t = 0; t < nt && ok; ++t) {
-          ok = warp_wait(p_full + t, j & 1, stop);
-          if (!ok) break;
-          tmem_fence_after();
-          if (elect_one()) {
+          // The first half of the weights' keys, then the second, then the tile's next scores (over
+          // the weights: products complete in order).
 #pragma unroll
-            for (int ks = 0; ks < kKeys / 16; ++ks)
-              mma_ts(kOutCol + 128 * t, kScoreCol + 128 * t + ks * 8, v_lo + ks * (2048 >> 4), kOut, j > 0 || ks > 0);
-            mma_commit(o_done + t);
-            if (t == nt - 1) mma_commit(empty + sv);
-            if (more) {
+          for (int half = 0; half < 2; ++half) {
+            ok = ok && warp_wait((half ? p_full : p_half) + t, j & 1, stop);
+            if (!ok) break;
+            tmem_fence_after();
+            if (elect_one()) {
+#pragma unroll
+              for (int ks = half * (kKeys / 32); ks < (half + 1) * (kKeys / 32); ++ks)
+                mma_ts(kOutCol + 128 * t, kScoreCol + 128 * t + ks * 8, v_lo + ks * (2048 >> 4), kOut, j > 0 || ks > 0);
+              if (half) {
+                mma_commit(o_done + t);
+                if (t == nt - 1) mma_commit(empty + sv);
+              }
+            }
+            __syncwarp();
+          }
+          if (ok && more) {
+            if (t == 0) ok = warp_wait(full + sk, ph, stop);
+            if (ok && elect_one()) {
               scores(t, sk);
               if (t == nt - 1) mma_commit(empty + sk);
             }
+            __syncwarp();
           }
-          __syncwarp();
         }
+        if (more) advance();
       }
       if (elect_one()) mma_commit(drained);
       __syncwarp();
@@ -317,22 +330,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
           tma_tile_3d(smem_u32(smem) + t * kTileBytes + h * kHalfTile, &P.qmap, h * 64, kvh * P.group,
                       it.q_row + t * P.tile_tokens, q_full);
     }
-    int issued = 0, wanted = -1;  // wanted: a value tile to be cleaned
+    int issued = 0;
     bool ok = true;
-    auto clean_one = [&](int i) {
-      const int stage = i % kRing, key = (i >> 1) * kKeys;
-      if (!wait_bar(full + stage, (i / kRing) & 1, stop)) return false;
-      clean_values<kBf16>(ring + stage * kTileBytes, it.k_end - it.k_begin - key, it.q_tokens > 1, key - partial * kKeys,
-                          late, n_late);
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(clean);
-      return true;
-    };
     for (int i = 0; i < 2 * n_tiles && ok; ++i) {
       const int stage = i % kRing, use = i / kRing;
-      ok = use == 0 || wait_bar(empty + stage, (use - 1) & 1, stop);
-      ok = __all_sync(0xffffffffu, ok);
+      ok = use == 0 || warp_wait(empty + stage, (use - 1) & 1, stop);
       if (!ok) break;
       if (lane == 0) {
         const uint32_t dst = smem_u32(ring) + stage * kTileBytes;
@@ -340,18 +342,25 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
         mbar_arrive_expect_tx(full + stage, kTileBytes);
         for (int h = 0; h < 2; ++h)
           tma_tile_3d(dst + h * kHalfTile, map, h * 64, kvh, it.k_row + it.k_begin + (i >> 1) * kKeys, full + stage);
+        if ((i & 1) && (i >> 1) >= partial) mbar_arrive(asked + (i >> 1) - partial);
       }
       issued = i + 1;
-      if (wanted >= 0) {  // after the next tile's load is under way
-        ok = __all_sync(0xffffffffu, clean_one(wanted));
-        wanted = -1;
-      }
-      if ((i & 1) && (i >> 1) >= partial) wanted = i;
     }
-    if (ok && wanted >= 0) clean_one(wanted);
     // No copy may be in flight when the CTA ends.
     drain_bar(q_full, 0);
     for (int i = max(0, issued - kRing); i < issued; ++i) drain_bar(full + i % kRing, (i / kRing) & 1);
+  } else if (n_tiles) {
+    for (int j = partial; j < n_tiles; ++j) {
+      // The stage's barrier is at this tile's phase once the loader has asked for it.
+      const int i = 2 * j + 1, stage = i % kRing;
+      if (!warp_wait(asked + j - partial, 0, stop) || !warp_wait(full + stage, (i / kRing) & 1, stop)) break;
+      const int key = j * kKeys, valid = min(kKeys, it.k_end - it.k_begin - key);
+      clean_values<kBf16>(ring + stage * kTileBytes, min(valid, max(0, whole - key)), valid, warp - 10,
+                          late + 4 * (j - partial));
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(clean + j - partial);
+    }
   }
   __syncthreads();
   if (warp == 8) {

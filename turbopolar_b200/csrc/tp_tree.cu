@@ -412,7 +412,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
             if (n < kTreeKeys) sees = (uint64_t(1) << n) - 1;
           }
           ok = softmax_tile<kTreeKeys, false>(row, s_addr, kTreeOutCol + 128 * w + lanes, Bits64{sees}, P.scale_log2, !any,
-                                              [&] { return wait_bar(o_done + w, (units - 1) & 1, stop); });
+                                              [&] { return wait_bar(o_done + w, (units - 1) & 1, stop); }, [] {});
           tmem_fence_before();
         }
         __syncwarp();

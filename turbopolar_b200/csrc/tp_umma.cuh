@@ -308,10 +308,11 @@ struct Bits64 {
 // columns that the row does not see are masked, whatever they hold.  Writes the 16-bit weights over the
 // scores.  `o_addr`: the row's 128 accumulator columns, rescaled when the reference moves;
 // `before_rescale()` waits until the products issued so far have completed (false: given up) and
-// is not called for the first tile, when the accumulator holds nothing.
-template <int kCols, bool kBf16, class Sees, class Wait>
+// is not called for the first tile, when the accumulator holds nothing.  `half_written()` is called
+// once the weights of the first half of the columns are in tensor memory.
+template <int kCols, bool kBf16, class Sees, class Wait, class Half>
 __device__ __forceinline__ bool softmax_tile(SoftmaxRow& row, uint32_t s_addr, uint32_t o_addr, Sees sees,
-                                             float scale_log2, bool first, Wait before_rescale) {
+                                             float scale_log2, bool first, Wait before_rescale, Half half_written) {
   float s[kCols];
 #pragma unroll
   for (int c = 0; c < kCols; c += 32) tmem_ld32(s_addr + c, s + c);
@@ -369,6 +370,10 @@ __device__ __forceinline__ bool softmax_tile(SoftmaxRow& row, uint32_t s_addr, u
       w[i] = pack2<kBf16>(e0, e1);
     }
     tmem_st16(s_addr + c / 2, w);
+    if (c + 32 == kCols / 2) {
+      tmem_wait_st();
+      half_written();
+    }
   }
   float a0, a1;
   split_pair(add_pair(add[0], add[1]), a0, a1);
