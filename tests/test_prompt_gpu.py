@@ -3,7 +3,7 @@
 Tolerance per element, u = 2^-11 (float16) or 2^-8 (bfloat16), W = sum_j w_j |v_j| with the exact weights:
   u |out|                      the output's rounding
   u W                          each weight's rounding to 16 bits
-  2 eps W, eps = 2^-18 scale max_j sum_d |q_d k_jd| + 2^-15
+  2 eps W, eps = 2^-18 scale max_j sum_d |q_d k_jd| + 2^-20
                                scores: 8 accumulations of 16 products, each off by at most 2^-22 of the sum's
                                size, and as much inside a product group; the exponential and its argument;
                                once in the numerator and once in the sum
@@ -35,7 +35,7 @@ def _expect(q, k, v, q_lens, k_lens, scale):
                 w = torch.nan_to_num(torch.softmax(s, -1))
                 o = w @ vv
                 big = w @ vv.abs()
-                eps = 2.0 ** -18 * scale * (qq.abs() @ kk.abs().T).amax(-1, keepdim=True) + 2.0 ** -15
+                eps = 2.0 ** -18 * scale * (qq.abs() @ kk.abs().T).amax(-1, keepdim=True) + 2.0 ** -20
                 out[qa:qa + nq, h] = o
                 bound[qa:qa + nq, h] = u * o.abs() + (u + 2 * eps) * big + nk * 2.0 ** -25 * vv.abs().max()
         qa, ka = qa + nq, ka + nk

@@ -3,7 +3,7 @@
 Tolerance per element, u = 2^-11, W = sum_j w_j |v_j| with the exact weights:
   u |out|       the output's rounding to float16
   u W           each weight's rounding to float16
-  2 eps W       eps = 2^-18 S + 2^-15 + delta, S = scale max_j sum_d |q_d k_jd|: scores (eight accumulations of 16
+  2 eps W       eps = 2^-18 S + 2^-20 + delta, S = scale max_j sum_d |q_d k_jd|: scores (eight accumulations of 16
                 products) and the exponential, once in the numerator and once in the sum; delta = 2^-11 S
                 where the kernel's radius 2^(code * s) may round to the other neighbour of the float16 key
                 than tp_decode_pages' (int8 radii), and 3 * 2^-11 S where float32 inputs are rounded to float16
@@ -73,7 +73,7 @@ def _check(out, rt, q, kd, vd, mask, scale=128 ** -0.5):
     want = w @ vv
     big = w @ vv.abs()
     size = scale * (q.double().abs() @ kk.abs().transpose(-1, -2)).amax(-1, keepdim=True)
-    eps = 2.0 ** -18 * size + 2.0 ** -15
+    eps = 2.0 ** -18 * size + 2.0 ** -20
     if rt.fmt["int8_radii"]:
         eps = eps + U * size
     if f32:

@@ -35,8 +35,8 @@ constexpr int kKeys = 128;               // keys per tile
 constexpr int kRing = 5;                 // K and V tiles in flight
 constexpr int kPartial = 3;              // partly visible tiles of one item at most: 127 + 255 keys
 // Three warpgroups at 168 registers: 504 in all, of which the softmax threads, with a row of scores
-// each, take 208 and the others 88.
-constexpr int kPromptThreads = 384, kSoftmaxRegs = 208, kIssueRegs = 88;
+// each, take 224 and the others 56.
+constexpr int kPromptThreads = 384, kSoftmaxRegs = 224, kIssueRegs = 56;
 constexpr int kPromptBars = 2 * kTileBytes + kRing * kTileBytes;  // byte offset of the barriers
 constexpr int kPromptSmem = kPromptBars + 512;
 constexpr int kRecordRows = 2 * kTile;   // rows of an item's partial record
@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
   const int kvh = blockIdx.x % P.hkv;
   uint8_t* ring = smem + 2 * kTileBytes;
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + kPromptBars);
-  uint64_t *full = q_full + 1, *empty = full + kRing, *s_full = empty + kRing, *p_half = s_full + 2, *p_full = p_half + 2,
+  uint64_t *full = q_full + 1, *empty = full + kRing, *s_full = empty + kRing, *p_full = s_full + 2,
            *o_done = p_full + 2, *asked = o_done + 2, *clean = asked + kPartial, *drained = clean + kPartial;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
   volatile int* stop = reinterpret_cast<int*>(tmem_slot + 1);
@@ -141,7 +141,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(s_full + i, 1);
-      mbar_init(p_half + i, 4);
       mbar_init(p_full + i, 4);
       mbar_init(o_done + i, 1);
     }
@@ -181,15 +180,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
         if (ok && live) {
           tmem_fence_after();
           ok = softmax_tile<kKeys, kBf16>(row, s_addr, o_addr, FirstN{limit - (it.k_begin + j * kKeys)}, P.scale_log2, j == 0,
-                                          [&] { return wait_bar(o_done + t, (j - 1) & 1, stop); },
-                                          [&] {
-                                            tmem_fence_before();
-                                            __syncwarp();
-                                            if (lane == 0) mbar_arrive(p_half + t);
-                                          });
+                                          [&] { return wait_bar(o_done + t, (j - 1) & 1, stop); });
           tmem_fence_before();
-        } else if (ok && lane == 0) {
-          mbar_arrive(p_half + t);
         }
         __syncwarp();
         if (ok && lane == 0) mbar_arrive(p_full + t);
@@ -287,24 +279,19 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
         const bool more = j + 1 < n_tiles;
         const uint32_t v_lo = cols_lo(ring_addr, kHalfTile) + sv * (kTileBytes >> 4);
         for (int t = 0; t < nt && ok; ++t) {
-          // The first half of the weights' keys, then the second, then the tile's next scores (over
-          // the weights: products complete in order).
+          // The tile's weights times the values, then its next scores (over the weights: products
+          // complete in order).
+          ok = warp_wait(p_full + t, j & 1, stop);
+          if (!ok) break;
+          tmem_fence_after();
+          if (elect_one()) {
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            ok = ok && warp_wait((half ? p_full : p_half) + t, j & 1, stop);
-            if (!ok) break;
-            tmem_fence_after();
-            if (elect_one()) {
-#pragma unroll
-              for (int ks = half * (kKeys / 32); ks < (half + 1) * (kKeys / 32); ++ks)
-                mma_ts(kOutCol + 128 * t, kScoreCol + 128 * t + ks * 8, v_lo + ks * (2048 >> 4), kOut, j > 0 || ks > 0);
-              if (half) {
-                mma_commit(o_done + t);
-                if (t == nt - 1) mma_commit(empty + sv);
-              }
-            }
-            __syncwarp();
+            for (int ks = 0; ks < kKeys / 16; ++ks)
+              mma_ts(kOutCol + 128 * t, kScoreCol + 128 * t + ks * 8, v_lo + ks * (2048 >> 4), kOut, j > 0 || ks > 0);
+            mma_commit(o_done + t);
+            if (t == nt - 1) mma_commit(empty + sv);
           }
+          __syncwarp();
           if (ok && more) {
             if (t == 0) ok = warp_wait(full + sk, ph, stop);
             if (ok && elect_one()) {

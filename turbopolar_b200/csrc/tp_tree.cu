@@ -34,8 +34,8 @@ constexpr int kMaxDrafts = 256;
 constexpr int kGroupRows = 2 * kTile;                 // rows that share a decoded page
 constexpr int kLateRing = 16;                         // segments whose lists may be alive
 constexpr int kTreeThreads = 640;
-// Five warpgroups at 96 registers: 480, of which the softmax threads take 128, decode 88, issue 48.
-constexpr int kTreeSoftmaxRegs = 128, kTreeDecodeRegs = 88, kTreeIssueRegs = 48;
+// Five warpgroups at 96 registers: 480, of which the softmax threads take 136, decode 80, issue 48.
+constexpr int kTreeSoftmaxRegs = 136, kTreeDecodeRegs = 80, kTreeIssueRegs = 48;
 constexpr int kOffBits = kTreeStages * kTreeStage;    // [2][128][4] uint64: drafts that a row sees
 constexpr int kOffTab = kOffBits + 2 * 128 * 4 * 8;   // float2[512]
 constexpr int kOffMl = kOffTab + 512 * 8;             // [2 pieces][2 warpgroups][128] float2
@@ -412,7 +412,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
             if (n < kTreeKeys) sees = (uint64_t(1) << n) - 1;
           }
           ok = softmax_tile<kTreeKeys, false>(row, s_addr, kTreeOutCol + 128 * w + lanes, Bits64{sees}, P.scale_log2, !any,
-                                              [&] { return wait_bar(o_done + w, (units - 1) & 1, stop); }, [] {});
+                                              [&] { return wait_bar(o_done + w, (units - 1) & 1, stop); });
           tmem_fence_before();
         }
         __syncwarp();

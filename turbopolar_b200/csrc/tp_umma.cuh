@@ -243,44 +243,11 @@ __device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
-__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+__device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-
-// 2^x of two numbers x <= 8 on the multiply-add pipe (the special-function unit takes 8 cycles for a
-// warp's exponential, which alone would make the softmax as long as the products).  Takes
-// y = x / 256 + 248 / 256 clamped to [0, 1], so x < -248 (masked scores too) counts as -248.  x = n + f
-// with f in [-1/2, 1/2]; 2^f by a polynomial of degree 4 whose coefficients minimise the largest
-// relative error, 2.6e-6; n is added to the exponent, and a result whose exponent falls below the
-// normal range is negative as an integer and becomes 0.  The 24 bits of y limit x to 2^-16, so the
-// result is off by 2^-15 at most (weights are rounded to 2^-11 or 2^-8 afterwards).
-__device__ __forceinline__ void exp2_poly(float y0, float y1, float& e0, float& e1) {
-  constexpr float kMagic = 12582912.0f - 248.0f;  // 1.5 * 2^23: adding it rounds to an integer in the low bits
-  const uint64_t y = pair_of(y0, y1), k256 = pair_of(256.0f, 256.0f);
-  const uint64_t t = fma_pair(y, k256, pair_of(kMagic, kMagic));
-  const uint64_t n = fma_pair(t, pair_of(-1.0f, -1.0f), pair_of(kMagic, kMagic));
-  const uint64_t f = fma_pair(y, k256, n);
-  uint64_t p = pair_of(0.009570102207362652f, 0.009570102207362652f);
-  p = fma_pair(p, f, pair_of(0.05591785907745361f, 0.05591785907745361f));
-  p = fma_pair(p, f, pair_of(0.240247443318367f, 0.240247443318367f));
-  p = fma_pair(p, f, pair_of(0.6931217908859253f, 0.6931217908859253f));
-  p = fma_pair(p, f, pair_of(0.9999992847442627f, 0.9999992847442627f));
-  float t0, t1, p0, p1;
-  split_pair(t, t0, t1);
-  split_pair(p, p0, p1);
-  e0 = __int_as_float(max(0, __float_as_int(t0) * (1 << 23) + __float_as_int(p0)));
-  e1 = __int_as_float(max(0, __float_as_int(t1) * (1 << 23) + __float_as_int(p1)));
-}
-__device__ __forceinline__ float fma_sat(float a, float b, float c) {
-  float d;
-  asm("fma.rn.sat.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
-// Pairs of a tile's columns that take the polynomial.
-constexpr int kPolyPairs = 3;
-__host__ __device__ constexpr bool poly_pair(int i) { return (i & 7) * kPolyPairs % 8 >= 8 - kPolyPairs; }
 
 // The running softmax of a row: weights are 2^(s * scale_log2 - ref) with a reference that is at
 // least the row's maximum so far minus 8.  It moves only when a maximum exceeds it by more than 8:
@@ -308,11 +275,14 @@ struct Bits64 {
 // columns that the row does not see are masked, whatever they hold.  Writes the 16-bit weights over the
 // scores.  `o_addr`: the row's 128 accumulator columns, rescaled when the reference moves;
 // `before_rescale()` waits until the products issued so far have completed (false: given up) and
-// is not called for the first tile, when the accumulator holds nothing.  `half_written()` is called
-// once the weights of the first half of the columns are in tensor memory.
-template <int kCols, bool kBf16, class Sees, class Wait, class Half>
+// is not called for the first tile, when the accumulator holds nothing.
+//
+// The weights are made with the reference as it is while the maximum is found on another pipe, and
+// made again in the few tiles that move the reference: the special-function unit, which needs 8 cycles
+// for a warp's exponential (1,024 for 128 columns), does not wait for the maximum.
+template <int kCols, bool kBf16, class Sees, class Wait>
 __device__ __forceinline__ bool softmax_tile(SoftmaxRow& row, uint32_t s_addr, uint32_t o_addr, Sees sees,
-                                             float scale_log2, bool first, Wait before_rescale, Half half_written) {
+                                             float scale_log2, bool first, Wait before_rescale) {
   float s[kCols];
 #pragma unroll
   for (int c = 0; c < kCols; c += 32) tmem_ld32(s_addr + c, s + c);
@@ -321,16 +291,32 @@ __device__ __forceinline__ bool softmax_tile(SoftmaxRow& row, uint32_t s_addr, u
 #pragma unroll
     for (int c = 0; c < kCols; ++c) s[c] = sees(c) ? s[c] : -INFINITY;
   }
-  // NaN wins, so a row with a NaN score is known.
-  float top[4] = {s[0], s[1], s[2], s[3]};
+  const uint64_t scale2 = pair_of(scale_log2, scale_log2);
+  uint64_t add[2];
+  for (;;) {
+    const float base = row.ref == -INFINITY ? 0.0f : -row.ref;
+    const uint64_t base2 = pair_of(base, base);
+    add[0] = add[1] = 0;
+    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-  for (int c = 4; c < kCols; c += 8) {
+    for (int c = 0; c < kCols; c += 32) {
+      uint32_t w[16];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) top[i] = c + 4 < kCols ? max3_nan(top[i], s[c + i], s[c + 4 + i]) : max3_nan(top[i], s[c + i], top[i]);
-  }
-  const float m = max3_nan(top[0], top[1], max3_nan(top[2], top[3], top[3])) * scale_log2;
-  const bool moves = m > row.ref + kRefSlack;
-  if (__any_sync(0xffffffffu, moves)) {
+      for (int i = 0; i < 16; ++i) {
+        const float x = s[c + 2 * i], y = s[c + 2 * i + 1];
+        float e0, e1;
+        split_pair(fma_pair(pair_of(x, y), scale2, base2), e0, e1);
+        e0 = exp2_approx(e0);
+        top[i & 3] = max3(top[i & 3], x, y);
+        e1 = exp2_approx(e1);
+        add[i & 1] = add_pair(add[i & 1], pair_of(e0, e1));
+        w[i] = pack2<kBf16>(e0, e1);
+      }
+      tmem_st16(s_addr + c / 2, w);
+    }
+    const float m = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * scale_log2;
+    const bool moves = m > row.ref + kRefSlack;
+    if (!__any_sync(0xffffffffu, moves)) break;
     const float to = moves ? m : row.ref;
     const float f = moves ? exp2_approx(row.ref - to) : 1.0f;
     row.ref = to;
@@ -339,7 +325,7 @@ __device__ __forceinline__ bool softmax_tile(SoftmaxRow& row, uint32_t s_addr, u
       if (!__all_sync(0xffffffffu, before_rescale())) return false;
       tmem_fence_after();
 #pragma unroll
-      for (int c = 0; c < 128; c += 16) {  // a few times per row: registers count more than speed
+      for (int c = 0; c < 128; c += 16) {  // registers count more than speed
         float o[16];
         tmem_ld16(o_addr + c, o);
         tmem_wait_ld<16>(o);
@@ -349,36 +335,9 @@ __device__ __forceinline__ bool softmax_tile(SoftmaxRow& row, uint32_t s_addr, u
       }
     }
   }
-  const float base = row.ref == -INFINITY ? 0.0f : -row.ref;
-  const uint64_t scale2 = pair_of(scale_log2, scale_log2), base2 = pair_of(base, base);
-  const float scale_256 = scale_log2 * (1.0f / 256.0f), base_256 = (base + 248.0f) * (1.0f / 256.0f);
-  uint64_t add[2] = {0, 0};
-#pragma unroll
-  for (int c = 0; c < kCols; c += 32) {
-    uint32_t w[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float e0, e1;
-      if (poly_pair(i)) {
-        exp2_poly(fma_sat(s[c + 2 * i], scale_256, base_256), fma_sat(s[c + 2 * i + 1], scale_256, base_256), e0, e1);
-      } else {
-        split_pair(fma_pair(pair_of(s[c + 2 * i], s[c + 2 * i + 1]), scale2, base2), e0, e1);
-        e0 = exp2_approx(e0);
-        e1 = exp2_approx(e1);
-      }
-      add[i & 1] = add_pair(add[i & 1], pair_of(e0, e1));
-      w[i] = pack2<kBf16>(e0, e1);
-    }
-    tmem_st16(s_addr + c / 2, w);
-    if (c + 32 == kCols / 2) {
-      tmem_wait_st();
-      half_written();
-    }
-  }
   float a0, a1;
   split_pair(add_pair(add[0], add[1]), a0, a1);
-  // A NaN or +inf score makes the whole row NaN, whatever the polynomial made of it.
-  row.sum += m < INFINITY ? a0 + a1 : NAN;
+  row.sum += a0 + a1;
   tmem_wait_st();
   return true;
 }
