@@ -258,9 +258,16 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
         }
         mma_commit(s_full + t);
       };
+      // Issuing blocks until the tensor cores take the product, so time spent waiting is time they idle:
+      // key and value tiles are waited for one step ahead, in the gaps where the weights are not ready yet.
       int st = 0, ph = 0;  // stage and phase of the next tile in the ring
-      auto advance = [&] { st = st + 1 == kRing ? (ph ^= 1, 0) : st + 1; };
-      bool ok = warp_wait(q_full, 0, stop) && warp_wait(full, 0, stop);
+      auto next_tile = [&](bool cleaned, int j) {
+        bool here = warp_wait(full + st, ph, stop);
+        if (here && cleaned && j >= partial) here = warp_wait(clean + j - partial, 0, stop);
+        st = st + 1 == kRing ? (ph ^= 1, 0) : st + 1;
+        return here;
+      };
+      bool ok = warp_wait(q_full, 0, stop) && next_tile(false, 0);
       if (ok) {
         tmem_fence_after();
         if (elect_one()) {
@@ -268,16 +275,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
           mma_commit(empty);
         }
         __syncwarp();
-        advance();
       }
+      int sv = st;
+      ok = ok && next_tile(true, 0);
+      int sk = st;
+      if (n_tiles > 1) ok = ok && next_tile(false, 1);
       for (int j = 0; j < n_tiles && ok; ++j) {
-        const int sv = st;
-        ok = warp_wait(full + sv, ph, stop);
-        if (ok && j >= partial) ok = warp_wait(clean + j - partial, 0, stop);
-        advance();
-        const int sk = st;
         const bool more = j + 1 < n_tiles;
         const uint32_t v_lo = cols_lo(ring_addr, kHalfTile) + sv * (kTileBytes >> 4);
+        int sv_next = 0, sk_next = 0;
         for (int t = 0; t < nt && ok; ++t) {
           // The tile's weights times the values, then its next scores (over the weights: products
           // complete in order).
@@ -290,18 +296,23 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
               mma_ts(kOutCol + 128 * t, kScoreCol + 128 * t + ks * 8, v_lo + ks * (2048 >> 4), kOut, j > 0 || ks > 0);
             mma_commit(o_done + t);
             if (t == nt - 1) mma_commit(empty + sv);
-          }
-          __syncwarp();
-          if (ok && more) {
-            if (t == 0) ok = warp_wait(full + sk, ph, stop);
-            if (ok && elect_one()) {
+            if (more) {
               scores(t, sk);
               if (t == nt - 1) mma_commit(empty + sk);
             }
-            __syncwarp();
+          }
+          __syncwarp();
+          if (t == 0 && more) {
+            sv_next = st;
+            ok = next_tile(true, j + 1);
           }
         }
-        if (more) advance();
+        if (ok && j + 2 < n_tiles) {
+          sk_next = st;
+          ok = next_tile(false, j + 2);
+        }
+        sv = sv_next;
+        sk = sk_next;
       }
       if (elect_one()) mma_commit(drained);
       __syncwarp();
