@@ -32,6 +32,7 @@ constexpr int kTreeStage = 4 * kKvHalf;               // K then V
 constexpr int kTreeStages = 5;
 constexpr int kMaxDrafts = 256;
 constexpr int kGroupRows = 2 * kTile;                 // rows that share a decoded page
+constexpr int kAhead = 8;                             // pages on their way into L2
 constexpr int kLateRing = 16;                         // segments whose lists may be alive
 constexpr int kTreeThreads = 640;
 // Five warpgroups at 96 registers: 480, of which the softmax threads take 136, decode 80, issue 48.
@@ -293,6 +294,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
            *o_done = p_full + 2, *q_full = o_done + 2, *met = q_full + 1, *scanned = met + 1, *drained = scanned + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
   volatile int* stop = reinterpret_cast<int*>(tmem_slot + 1);
+  volatile int* progress = stop + 1;  // step that the decode warps have reached
 
   for (int i = threadIdx.x; i < 512; i += kTreeThreads) tab[i] = P.cs[i];
   for (int i = threadIdx.x; i < kLateRing * 8; i += kTreeThreads) late_ring[i] = 0;
@@ -311,6 +313,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
     mbar_init(scanned, 8);
     mbar_init(drained, 1);
     *stop = 0;
+    *progress = 0;
     fence_mbar_init();
   }
   if (warp == 16) tmem_alloc(tmem_slot, 512);
@@ -519,12 +522,6 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
     const __half* rs = P.pool.int8_radii ? P.pool.radii_scales + int64_t(head) * P.pool.page_capacity + s : nullptr;
     int i = 0, st = 0, ph = 1, scans = 0, draft_pieces = 0;  // ph: parity of the stage's last release
     bool ok = true;
-    // One page a few steps ahead is fetched into L2, so that the loads one step ahead come from there.
-    constexpr int kAhead = 6;
-    if (tid < min(kAhead, count) && s + tid < P.n_page_steps)
-      asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(pg + int64_t(tid) * P.pool.page_bytes),
-                   "r"(P.pool.page_bytes)
-                   : "memory");
     // Step i: its page is in `use`; the next step's page goes to `fetch`.  False after the last step.
     auto step = [&](PageRegs& use, PageRegs& fetch) {
       const uint8_t* now = pg;
@@ -535,23 +532,16 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
         ++s;
         ahead += P.pool.page_bytes;
         if (rs) ++ahead_rs;
-        if (tid == 0 && s + kAhead - 1 < P.n_page_steps && i + kAhead < count)
-          asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(now + int64_t(kAhead) * P.pool.page_bytes),
-                       "r"(P.pool.page_bytes)
-                       : "memory");
       } else {
         s = 0;
         ++seg;
         head = seg / P.row_groups;
         ahead = P.pool.pages + int64_t(head) * P.pool.page_capacity * P.pool.page_bytes;
         if (rs) ahead_rs = P.pool.radii_scales + int64_t(head) * P.pool.page_capacity;
-        if (tid < kAhead && tid < P.n_page_steps && i + 1 + tid < count)
-          asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(ahead + int64_t(tid) * P.pool.page_bytes),
-                       "r"(P.pool.page_bytes)
-                       : "memory");
       }
       pg = ahead;
       rs = ahead_rs;
+      if (tid == 0) *progress = i;
       if (i + 1 < count && s < P.n_page_steps) load_page<kMode>(fetch, P.pool, pg, rs, tid);
       const uint32_t stage = stages + st * kTreeStage;
       ok = i < kTreeStages || wait_bar(kv_empty + st, ph, stop);
@@ -655,6 +645,20 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
     __syncwarp();
     drain_bar(drained, 0);
     __syncwarp();
+  } else if (warp == 17 && lane == 0) {
+    // Pages are fetched into L2 kAhead steps before the decode warps load them.  (One thread that does
+    // nothing else: issuing a bulk operation blocks it for some hundred cycles.)
+    int s = step0, seg = seg0;
+    const long long t0 = clock64();
+    for (int i = 0; i < count && !*stop; ++i) {
+      while (i - *progress > kAhead && !*stop && clock64() - t0 < kWaitCycles) __nanosleep(50);
+      if (s < P.n_page_steps) {
+        const uint8_t* pg =
+            P.pool.pages + (int64_t(seg / P.row_groups) * P.pool.page_capacity + s) * P.pool.page_bytes;
+        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(pg), "r"(P.pool.page_bytes) : "memory");
+      }
+      if (++s == P.n_steps) s = 0, ++seg;
+    }
   }
   __syncthreads();
   if (warp == 16) {
