@@ -35,8 +35,8 @@ constexpr int kGroupRows = 2 * kTile;                 // rows that share a decod
 constexpr int kAhead = 8;                             // pages on their way into L2
 constexpr int kLateRing = 16;                         // segments whose lists may be alive
 constexpr int kTreeThreads = 640;
-// Five warpgroups at 96 registers: 480, of which the softmax threads take 136, decode 80, issue 48.
-constexpr int kTreeSoftmaxRegs = 136, kTreeDecodeRegs = 80, kTreeIssueRegs = 48;
+// Five warpgroups at 96 registers: 480, of which the softmax threads take 128, decode 88, issue 48.
+constexpr int kTreeSoftmaxRegs = 128, kTreeDecodeRegs = 88, kTreeIssueRegs = 48;
 constexpr int kOffBits = kTreeStages * kTreeStage;    // [2][128][4] uint64: drafts that a row sees
 constexpr int kOffTab = kOffBits + 2 * 128 * 4 * 8;   // float2[512]
 constexpr int kOffMl = kOffTab + 512 * 8;             // [2 pieces][2 warpgroups][128] float2
@@ -90,53 +90,46 @@ struct UnitOf {
                        vscales = codes + (kMode == kTreeDefault ? 1024 : 2048), bytes = vscales + 256;
 };
 
-__device__ __forceinline__ uint4 ldg16(const void* p) {
-  uint4 r;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
-               : "l"(p));
-  return r;
-}
-__device__ __forceinline__ uint2 ldg8(const void* p) {
-  uint2 r;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
-  return r;
-}
-__device__ __forceinline__ uint32_t ldg4(const void* p) {
-  uint32_t r;
-  asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(r) : "l"(p));
-  return r;
-}
+// Decode thread tid takes pairs [8c, 8c + 8) of row l of both units; its warp, steps kk = 0, 1 (16 tokens)
+// x 32 channels of group G of unit vu.  Eight neighbouring lanes hold four c of two rows: their chunks of
+// a K tile lie in different banks.
+struct DecodeShare {
+  int c, l, G, vu, lane;
+  __device__ __forceinline__ explicit DecodeShare(int tid)
+      : c((tid & 3) | (tid >> 3 & 1) << 2), l((tid >> 2 & 1) | (tid >> 4) << 1), G(tid >> 5 & 3), vu(tid >> 7),
+        lane(tid & 31) {}
+};
+
+template <class T>
+__device__ __forceinline__ T stream_load(const uint8_t* p) { return __ldcs(reinterpret_cast<const T*>(p)); }
 
 // `pg`: the page block; `rscale`: where its radius scale is (int8 radii).
 template <int kMode>
 __device__ __forceinline__ void load_page(PageRegs& R, const PoolArgs& L, const uint8_t* pg, const __half* rscale, int tid) {
-  const int warp = tid >> 5, lane = tid & 31, c = tid & 7, l = tid >> 3;
-  const int ub = kMode == kTreeGeneral ? L.unit_bytes : UnitOf<kMode>::bytes;
-  const int vc = kMode == kTreeGeneral ? L.u_vcodes : UnitOf<kMode>::vcodes;
-  const int vs = kMode == kTreeGeneral ? L.u_vscales : UnitOf<kMode>::vscales;
-  if (kMode != kTreeGeneral) {
-    const uint8_t* rad = pg + (kMode == kTreeDefault ? radii_f16_offset(l, 8 * c) : l * 64 + 8 * c);
-    const uint8_t* code = pg + UnitOf<kMode>::codes + (kMode == kTreeDefault ? l * 32 + 4 * c : l * 64 + 8 * c);
+  const DecodeShare D(tid);
+  const uint32_t ub = kMode == kTreeGeneral ? L.unit_bytes : UnitOf<kMode>::bytes;
+  const uint32_t vc = kMode == kTreeGeneral ? L.u_vcodes : UnitOf<kMode>::vcodes;
+  const uint32_t vs = kMode == kTreeGeneral ? L.u_vscales : UnitOf<kMode>::vscales;
+  // 32-bit offsets from the page, which is the same for all threads.
+  const uint32_t rad = kMode == kTreeDefault ? radii_f16_offset(D.l, 8 * D.c) : D.l * 64 + 8 * D.c;
+  const uint32_t code = UnitOf<kMode>::codes + (kMode == kTreeDefault ? D.l * 32 + 4 * D.c : D.l * 64 + 8 * D.c);
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      if (kMode == kTreeDefault) {
-        R.rad[u] = ldg16(rad + u * ub);
-        R.code[u].x = ldg4(code + u * ub);
-      } else {
-        const uint2 r8 = ldg8(rad + u * ub);
-        R.rad[u].x = r8.x, R.rad[u].y = r8.y;
-        R.code[u] = ldg8(code + u * ub);
-      }
+  for (uint32_t u = 0; u < 2; ++u) {
+    if (kMode == kTreeDefault) {
+      R.rad[u] = stream_load<uint4>(pg + rad + u * ub);
+      R.code[u].x = stream_load<uint32_t>(pg + code + u * ub);
+    } else if (kMode == kTreeAdapter) {
+      const uint2 r8 = stream_load<uint2>(pg + rad + u * ub);
+      R.rad[u].x = r8.x, R.rad[u].y = r8.y;
+      R.code[u] = stream_load<uint2>(pg + code + u * ub);
     }
   }
-  const uint8_t* v = pg + (warp >> 2) * ub + vc + (warp & 3) * 512 + lane * 16;
-  const uint8_t* sc = pg + (warp >> 2) * ub + vs + ((lane & 3) * 16 + (warp & 3) * 2) * 2;
+  const uint32_t v = D.vu * ub + vc + D.G * 512 + D.lane * 16, sc = D.vu * ub + vs + ((D.lane & 3) * 16 + D.G * 2) * 2;
 #pragma unroll
-  for (int kk = 0; kk < 2; ++kk) {
-    R.v[kk] = ldg16(v + kk * 2048);
+  for (uint32_t kk = 0; kk < 2; ++kk) {
+    R.v[kk] = stream_load<uint4>(pg + v + kk * 2048);
 #pragma unroll
-    for (int a = 0; a < 2; ++a) R.scale[kk][a] = ldg4(sc + kk * 128 + a * 16);
+    for (uint32_t a = 0; a < 2; ++a) R.scale[kk][a] = stream_load<uint32_t>(pg + sc + kk * 128 + a * 16);
   }
   if (kMode != kTreeDefault) R.rscale = rscale ? __half2float(*rscale) : 0.0f;
 }
@@ -148,18 +141,12 @@ __device__ __forceinline__ void st8(uint32_t addr, uint32_t a, uint32_t b) {
   asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(addr), "r"(a), "r"(b) : "memory");
 }
 
-// The 16 channels of 8 decoded pairs of row `row`: two 16-byte chunks; the two halves of the warp's
-// chunks are stored in opposite order, so that eight lanes always cover all banks.
+// The 16 channels of 8 decoded pairs of row `row`: two 16-byte chunks.
 __device__ __forceinline__ void store_pairs(uint32_t k_tile, int row, int c, const uint32_t (&w)[8]) {
   const uint32_t base = k_tile + (c >> 2) * kKvHalf + row * 128;
-  const int c0 = (2 * c) & 7, odd = c >> 2;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int which = i ^ odd;
-    const uint32_t at = base + (((c0 + which) ^ (row & 7)) << 4);
-    if (which == 0) st16(at, w[0], w[1], w[2], w[3]);
-    else st16(at, w[4], w[5], w[6], w[7]);
-  }
+  const int c0 = (2 * c) & 7;
+  st16(base + ((c0 ^ (row & 7)) << 4), w[0], w[1], w[2], w[3]);
+  st16(base + (((c0 + 1) ^ (row & 7)) << 4), w[4], w[5], w[6], w[7]);
 }
 
 // Decode one page into the stage (K tile, V tile).  `limit`: tokens of the page that are seen;
@@ -167,18 +154,23 @@ __device__ __forceinline__ void store_pairs(uint32_t k_tile, int row, int c, con
 template <int kMode>
 __device__ __forceinline__ void decode_step(const PageRegs& R, const PoolArgs& L, const float2* tab, uint32_t stage,
                                             const uint8_t* pg, int limit, int tid) {
-  const int warp = tid >> 5, lane = tid & 31, c = tid & 7, l = tid >> 3;
+  const DecodeShare D(tid);
+  const int c = D.c, l = D.l;
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     uint32_t w[8];
     if (kMode == kTreeDefault) {
+      // r (cos, sin) in float16 pairs with the cosine and sine as sums of two float16 numbers (an error
+      // of 2^-22): r lo, then r hi + that, is the float32 product rounded once but for rare ties.  Half the
+      // instructions of the float32 form; the decode warps' instructions bound this kernel.
       const uint32_t rr[4] = {R.rad[u].x, R.rad[u].y, R.rad[u].z, R.rad[u].w};
+      const uint32_t even = R.code[u].x << 3 & 0x78787878u, odd = R.code[u].x >> 1 & 0x78787878u;  // bytes: 8 * code
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float2 cs = tab[(R.code[u].x >> (4 * i)) & 15];
-        const float2 r2 = __half22float2(u32_as_h2(rr[i >> 1]));
-        const float r = i & 1 ? r2.y : r2.x;
-        w[i] = pack_h2(r * cs.x, r * cs.y);
+        const uint32_t at = prmt(i & 1 ? odd : even, 0, 0x4440 + (i >> 1));
+        const uint2 cs = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(tab) + at);
+        const __half2 r2 = u32_as_h2(rr[i >> 1]), r = i & 1 ? __high2half2(r2) : __low2half2(r2);
+        w[i] = h2_as_u32(__hfma2(r, u32_as_h2(cs.x), __hmul2(r, u32_as_h2(cs.y))));
       }
     } else if (kMode == kTreeAdapter) {
       const float s = R.rscale * 1.4426950408889634f;
@@ -210,7 +202,7 @@ __device__ __forceinline__ void decode_step(const PageRegs& R, const PoolArgs& L
   }
   // Values: byte x of a word is code + 128; 0x6400 | x is the float16 number 1024 + x.
   const uint32_t v_tile = stage + 2 * kKvHalf;
-  const int u = warp >> 2, G = warp & 3, g = lane >> 2, t = lane & 3;
+  const int u = D.vu, G = D.G, g = D.lane >> 2, t = D.lane & 3;
   const __half2 bias = __float2half2_rn(1152.0f);
 #pragma unroll
   for (int kk = 0; kk < 2; ++kk) {
@@ -296,7 +288,17 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
   volatile int* stop = reinterpret_cast<int*>(tmem_slot + 1);
   volatile int* progress = stop + 1;  // step that the decode warps have reached
 
-  for (int i = threadIdx.x; i < 512; i += kTreeThreads) tab[i] = P.cs[i];
+  // (cos, sin) of every code; for the default format's 16 codes as float16 pairs, rounded and remainder.
+  for (int i = threadIdx.x; i < (kMode == kTreeDefault ? 16 : 512); i += kTreeThreads) {
+    const float2 cs = P.cs[i];
+    if (kMode == kTreeDefault) {
+      const __half2 hi = __floats2half2_rn(cs.x, cs.y);
+      const __half2 lo = __floats2half2_rn(cs.x - __low2float(hi), cs.y - __high2float(hi));
+      reinterpret_cast<uint2*>(tab)[i] = make_uint2(h2_as_u32(hi), h2_as_u32(lo));
+    } else {
+      tab[i] = cs;
+    }
+  }
   for (int i = threadIdx.x; i < kLateRing * 8; i += kTreeThreads) late_ring[i] = 0;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kTreeStages; ++i) {
