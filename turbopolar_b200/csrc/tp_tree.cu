@@ -13,7 +13,8 @@
 //   warps 0-3, 4-7   softmax, one row per thread (queries live in tensor memory as operand A)
 //   warps 8-15       decode: 64 keys and values per step into a ring of 32 KB stages
 //   warp 16          issues the products
-//   warps 17-19      complete the warpgroup (registers are moved per warpgroup)
+//   warp 17          copies pages as they are stored into a ring of three (bulk copies)
+//   warps 18, 19     complete the warpgroup (registers are moved per warpgroup)
 // With more than 128 rows the softmax warpgroups have a tile each; with fewer they take
 // alternate steps of the one tile, each with its own running maximum, sum and accumulator, and
 // merge at the segment's end.
@@ -29,15 +30,17 @@ namespace tp {
 constexpr int kTreeKeys = 64;                         // keys per step: one page
 constexpr int kKvHalf = kTreeKeys * 128;              // 64 keys x 64 channels
 constexpr int kTreeStage = 4 * kKvHalf;               // K then V
-constexpr int kTreeStages = 5;
+constexpr int kTreeStages = 4;
+constexpr int kPageRing = 3, kPageSlot = 2 * kMaxUnitBytes;  // stored pages on their way
+constexpr int kPageCopiers = 4;
 constexpr int kMaxDrafts = 256;
 constexpr int kGroupRows = 2 * kTile;                 // rows that share a decoded page
-constexpr int kAhead = 8;                             // pages on their way into L2
 constexpr int kLateRing = 16;                         // segments whose lists may be alive
 constexpr int kTreeThreads = 640;
 // Five warpgroups at 96 registers: 480, of which the softmax threads take 128, decode 88, issue 48.
 constexpr int kTreeSoftmaxRegs = 128, kTreeDecodeRegs = 88, kTreeIssueRegs = 48;
-constexpr int kOffBits = kTreeStages * kTreeStage;    // [2][128][4] uint64: drafts that a row sees
+constexpr int kOffPages = kTreeStages * kTreeStage;
+constexpr int kOffBits = kOffPages + kPageRing * kPageSlot;  // [2][128][4] uint64: drafts that a row sees
 constexpr int kOffTab = kOffBits + 2 * 128 * 4 * 8;   // float2[512]
 constexpr int kOffMl = kOffTab + 512 * 8;             // [2 pieces][2 warpgroups][128] float2
 constexpr int kOffBuf = kOffMl + 2 * 2 * 128 * 8;     // 2 KB per softmax warp: rows on their way in and out
@@ -73,17 +76,8 @@ struct TreeParams {
 
 __device__ __forceinline__ int64_t range_begin(const TreeParams& P, int cta) { return P.total * cta / P.grid; }
 
-// A thread's share of one page in flight: two radius chunks (8 pairs of a row each), their codes, two
-// value words and their scales.
-struct PageRegs {
-  uint4 rad[2], v[2];
-  uint2 code[2];
-  uint32_t scale[2][2];
-  float rscale;
-};
-
-// Unit layout of the two specialised formats (make_layout checks the sizes of any format): offsets
-// known to the compiler become part of the load instructions.
+// Unit layout of the two specialised formats: offsets known to the compiler become part of the load
+// instructions.
 template <int kMode>
 struct UnitOf {
   static constexpr int vcodes = kMode == kTreeDefault ? 4096 : 2048, codes = vcodes + 4096,
@@ -100,40 +94,6 @@ struct DecodeShare {
         lane(tid & 31) {}
 };
 
-template <class T>
-__device__ __forceinline__ T stream_load(const uint8_t* p) { return __ldcs(reinterpret_cast<const T*>(p)); }
-
-// `pg`: the page block; `rscale`: where its radius scale is (int8 radii).
-template <int kMode>
-__device__ __forceinline__ void load_page(PageRegs& R, const PoolArgs& L, const uint8_t* pg, const __half* rscale, int tid) {
-  const DecodeShare D(tid);
-  const uint32_t ub = kMode == kTreeGeneral ? L.unit_bytes : UnitOf<kMode>::bytes;
-  const uint32_t vc = kMode == kTreeGeneral ? L.u_vcodes : UnitOf<kMode>::vcodes;
-  const uint32_t vs = kMode == kTreeGeneral ? L.u_vscales : UnitOf<kMode>::vscales;
-  // 32-bit offsets from the page, which is the same for all threads.
-  const uint32_t rad = kMode == kTreeDefault ? radii_f16_offset(D.l, 8 * D.c) : D.l * 64 + 8 * D.c;
-  const uint32_t code = UnitOf<kMode>::codes + (kMode == kTreeDefault ? D.l * 32 + 4 * D.c : D.l * 64 + 8 * D.c);
-#pragma unroll
-  for (uint32_t u = 0; u < 2; ++u) {
-    if (kMode == kTreeDefault) {
-      R.rad[u] = stream_load<uint4>(pg + rad + u * ub);
-      R.code[u].x = stream_load<uint32_t>(pg + code + u * ub);
-    } else if (kMode == kTreeAdapter) {
-      const uint2 r8 = stream_load<uint2>(pg + rad + u * ub);
-      R.rad[u].x = r8.x, R.rad[u].y = r8.y;
-      R.code[u] = stream_load<uint2>(pg + code + u * ub);
-    }
-  }
-  const uint32_t v = D.vu * ub + vc + D.G * 512 + D.lane * 16, sc = D.vu * ub + vs + ((D.lane & 3) * 16 + D.G * 2) * 2;
-#pragma unroll
-  for (uint32_t kk = 0; kk < 2; ++kk) {
-    R.v[kk] = stream_load<uint4>(pg + v + kk * 2048);
-#pragma unroll
-    for (uint32_t a = 0; a < 2; ++a) R.scale[kk][a] = stream_load<uint32_t>(pg + sc + kk * 128 + a * 16);
-  }
-  if (kMode != kTreeDefault) R.rscale = rscale ? __half2float(*rscale) : 0.0f;
-}
-
 __device__ __forceinline__ void st16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
@@ -149,40 +109,48 @@ __device__ __forceinline__ void store_pairs(uint32_t k_tile, int row, int c, con
   st16(base + (((c0 + 1) ^ (row & 7)) << 4), w[4], w[5], w[6], w[7]);
 }
 
-// Decode one page into the stage (K tile, V tile).  `limit`: tokens of the page that are seen;
-// values of the others are cleared (their weights are 0, and 0 times a non-finite value is NaN).
+// Decode the stored page at `pg` (shared memory) into the stage (K tile, V tile).  `limit`: tokens of
+// the page that are seen; values of the others are cleared (their weights are 0, and 0 times a
+// non-finite value is NaN).  `rscale`: the page's radius scale (int8 radii).
 template <int kMode>
-__device__ __forceinline__ void decode_step(const PageRegs& R, const PoolArgs& L, const float2* tab, uint32_t stage,
-                                            const uint8_t* pg, int limit, int tid) {
+__device__ __forceinline__ void decode_step(const uint8_t* pg, const PoolArgs& L, const float2* tab, float rscale,
+                                            uint32_t stage, int limit, int tid) {
   const DecodeShare D(tid);
   const int c = D.c, l = D.l;
+  const int ub = kMode == kTreeGeneral ? L.unit_bytes : UnitOf<kMode>::bytes;
+  const int vc = kMode == kTreeGeneral ? L.u_vcodes : UnitOf<kMode>::vcodes;
+  const int vs = kMode == kTreeGeneral ? L.u_vscales : UnitOf<kMode>::vscales;
+  uint32_t w[2][8];
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
-    uint32_t w[8];
+    const uint8_t* un = pg + u * ub;
     if (kMode == kTreeDefault) {
       // r (cos, sin) in float16 pairs with the cosine and sine as sums of two float16 numbers (an error
       // of 2^-22): r lo, then r hi + that, is the float32 product rounded once but for rare ties.  Half the
       // instructions of the float32 form; the decode warps' instructions bound this kernel.
-      const uint32_t rr[4] = {R.rad[u].x, R.rad[u].y, R.rad[u].z, R.rad[u].w};
-      const uint32_t even = R.code[u].x << 3 & 0x78787878u, odd = R.code[u].x >> 1 & 0x78787878u;  // bytes: 8 * code
+      const uint4 rad = *reinterpret_cast<const uint4*>(un + radii_f16_offset(l, 8 * c));
+      const uint32_t code = *reinterpret_cast<const uint32_t*>(un + UnitOf<kMode>::codes + l * 32 + 4 * c);
+      const uint32_t rr[4] = {rad.x, rad.y, rad.z, rad.w};
+      const uint32_t even = code << 3 & 0x78787878u, odd = code >> 1 & 0x78787878u;  // bytes: 8 * code
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const uint32_t at = prmt(i & 1 ? odd : even, 0, 0x4440 + (i >> 1));
         const uint2 cs = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(tab) + at);
         const __half2 r2 = u32_as_h2(rr[i >> 1]), r = i & 1 ? __high2half2(r2) : __low2half2(r2);
-        w[i] = h2_as_u32(__hfma2(r, u32_as_h2(cs.x), __hmul2(r, u32_as_h2(cs.y))));
+        w[u][i] = h2_as_u32(__hfma2(r, u32_as_h2(cs.x), __hmul2(r, u32_as_h2(cs.y))));
       }
     } else if (kMode == kTreeAdapter) {
-      const float s = R.rscale * 1.4426950408889634f;
+      const uint2 rad = *reinterpret_cast<const uint2*>(un + l * 64 + 8 * c);
+      const uint2 code = *reinterpret_cast<const uint2*>(un + UnitOf<kMode>::codes + l * 64 + 8 * c);
+      const float s = rscale * 1.4426950408889634f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const uint32_t rw = i < 4 ? R.rad[u].x : R.rad[u].y, cw = i < 4 ? R.code[u].x : R.code[u].y;
+        const uint32_t rw = i < 4 ? rad.x : rad.y, cw = i < 4 ? code.x : code.y;
         const float2 cs = tab[256 + ((cw >> (8 * (i & 3))) & 255)];
         const float r = exp2_approx(float(int8_t(rw >> (8 * (i & 3)))) * s);
-        w[i] = pack_h2(r * cs.x, r * cs.y);
+        w[u][i] = pack_h2(r * cs.x, r * cs.y);
       }
     } else {
-      const uint8_t* un = pg + u * L.unit_bytes;
       const uint8_t* row = un + L.u_codes + l * L.code_row;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -192,42 +160,47 @@ __device__ __forceinline__ void decode_step(const PageRegs& R, const PoolArgs& L
         const int at = rel * bits;
         const uint32_t code = (row[(l1 ? 0 : L.l1_row) + (at >> 3)] >> (at & 7)) & ((1u << bits) - 1);
         const float r = L.int8_radii
-                            ? exp2_approx(float(reinterpret_cast<const int8_t*>(un)[l * 64 + j]) * R.rscale * 1.4426950408889634f)
+                            ? exp2_approx(float(reinterpret_cast<const int8_t*>(un)[l * 64 + j]) * rscale * 1.4426950408889634f)
                             : __half2float(*reinterpret_cast<const __half*>(un + radii_f16_offset(l, j)));
         const float2 cs = tab[(l1 ? 0 : 256) + code];
-        w[i] = pack_h2(r * cs.x, r * cs.y);
+        w[u][i] = pack_h2(r * cs.x, r * cs.y);
       }
     }
-    store_pairs(stage, u * 32 + l, c, w);
   }
   // Values: byte x of a word is code + 128; 0x6400 | x is the float16 number 1024 + x.
   const uint32_t v_tile = stage + 2 * kKvHalf;
-  const int u = D.vu, G = D.G, g = D.lane >> 2, t = D.lane & 3;
+  const int G = D.G, g = D.lane >> 2, t = D.lane & 3, chunk = (G & 1) * 4 + (g >> 1);
   const __half2 bias = __float2half2_rn(1152.0f);
+  uint32_t o[2][4][2];
 #pragma unroll
   for (int kk = 0; kk < 2; ++kk) {
-    const uint32_t words[4] = {R.v[kk].x, R.v[kk].y, R.v[kk].z, R.v[kk].w};
+    const uint4 v = *reinterpret_cast<const uint4*>(pg + D.vu * ub + vc + G * 512 + D.lane * 16 + kk * 2048);
+    const uint32_t words[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int a = 0; a < 2; ++a) {
+      const __half2 sc = *reinterpret_cast<const __half2*>(pg + D.vu * ub + vs + (t * 16 + G * 2) * 2 + kk * 128 + a * 16);
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        const __half s = b ? __high2half(u32_as_h2(R.scale[kk][a])) : __low2half(u32_as_h2(R.scale[kk][a]));
-        const __half2 s2 = __half2half2(s);
-        const int in_page = u * 32 + kk * 16 + 8 * a + 2 * t + b;
-        uint32_t o[2];
+        const __half2 s2 = b ? __high2half2(sc) : __low2half2(sc);
 #pragma unroll
         for (int e = 0; e < 2; ++e)
-          o[e] = h2_as_u32(__hmul2(__hsub2(u32_as_h2(prmt(words[2 * a + e], 0x64646464u, b ? 0x4341u : 0x4240u)), bias), s2));
-        const int chunk = (G & 1) * 4 + (g >> 1);
-        st8(v_tile + (G >> 1) * kKvHalf + in_page * 128 + ((chunk ^ (in_page & 7)) << 4) + (g & 1) * 8, o[0], o[1]);
+          o[kk][2 * a + b][e] =
+              h2_as_u32(__hmul2(__hsub2(u32_as_h2(prmt(words[2 * a + e], 0x64646464u, b ? 0x4341u : 0x4240u)), bias), s2));
       }
     }
+  }
+#pragma unroll
+  for (int u = 0; u < 2; ++u) store_pairs(stage, u * 32 + l, c, w[u]);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int in_page = D.vu * 32 + (i >> 2) * 16 + (i >> 1 & 1) * 8 + 2 * t + (i & 1);
+    st8(v_tile + (G >> 1) * kKvHalf + in_page * 128 + ((chunk ^ (in_page & 7)) << 4) + (g & 1) * 8, o[i >> 2][i & 3][0],
+        o[i >> 2][i & 3][1]);
   }
   if (limit < kTreeKeys) {  // this thread's values again, where they are not seen
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int in_page = u * 32 + (i >> 2) * 16 + (i >> 1 & 1) * 8 + 2 * t + (i & 1);
-      const int chunk = (G & 1) * 4 + (g >> 1);
+      const int in_page = D.vu * 32 + (i >> 2) * 16 + (i >> 1 & 1) * 8 + 2 * t + (i & 1);
       if (in_page >= limit)
         st8(v_tile + (G >> 1) * kKvHalf + in_page * 128 + ((chunk ^ (in_page & 7)) << 4) + (g & 1) * 8, 0, 0);
     }
@@ -255,7 +228,7 @@ __device__ __forceinline__ bool chunk_not_finite(uint4 x) {
 // With `late`, a row with a non-finite value sets its bit there.  All 256 decode threads.
 __device__ __forceinline__ void dense_step(uint32_t stage, const void* k, const void* v, int64_t kt, int64_t vt, int f32,
                                            int valid, uint32_t* late, int tid) {
-#pragma unroll 2
+#pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int row = i * 16 + (tid >> 4), c = tid & 15;
     uint4 x = make_uint4(0, 0, 0, 0), y = x;
@@ -283,10 +256,10 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
   uint32_t* late_ring = reinterpret_cast<uint32_t*>(smem + kOffLate);
   uint64_t* kv_full = reinterpret_cast<uint64_t*>(smem + kOffTreeBars);
   uint64_t *kv_empty = kv_full + kTreeStages, *s_full = kv_empty + kTreeStages, *p_full = s_full + 2,
-           *o_done = p_full + 2, *q_full = o_done + 2, *met = q_full + 1, *scanned = met + 1, *drained = scanned + 1;
+           *o_done = p_full + 2, *page_full = o_done + 2, *page_empty = page_full + kPageRing,
+           *q_full = page_empty + kPageRing, *met = q_full + 1, *scanned = met + 1, *drained = scanned + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
   volatile int* stop = reinterpret_cast<int*>(tmem_slot + 1);
-  volatile int* progress = stop + 1;  // step that the decode warps have reached
 
   // (cos, sin) of every code; for the default format's 16 codes as float16 pairs, rounded and remainder.
   for (int i = threadIdx.x; i < (kMode == kTreeDefault ? 16 : 512); i += kTreeThreads) {
@@ -310,12 +283,15 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
       mbar_init(p_full + i, 4);
       mbar_init(o_done + i, 1);
     }
+    for (int i = 0; i < kPageRing; ++i) {
+      mbar_init(page_full + i, kPageCopiers);
+      mbar_init(page_empty + i, 8);
+    }
     mbar_init(q_full, 8);
     mbar_init(met, 8);
     mbar_init(scanned, 8);
     mbar_init(drained, 1);
     *stop = 0;
-    *progress = 0;
     fence_mbar_init();
   }
   if (warp == 16) tmem_alloc(tmem_slot, 512);
@@ -518,39 +494,36 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
     fewer_registers<kTreeDecodeRegs>();
     const int tid = threadIdx.x - 256;
     const uint32_t stages = smem_u32(smem);
-    // Cursor over the CTA's steps: `pg` is the page of step s while s < n_page_steps.
     int s = step0, seg = seg0, head = seg0 / P.row_groups;
-    const uint8_t* pg = P.pool.pages + (int64_t(head) * P.pool.page_capacity + s) * P.pool.page_bytes;
-    const __half* rs = P.pool.int8_radii ? P.pool.radii_scales + int64_t(head) * P.pool.page_capacity + s : nullptr;
-    int i = 0, st = 0, ph = 1, scans = 0, draft_pieces = 0;  // ph: parity of the stage's last release
+    int st = 0, ph = 1, scans = 0, draft_pieces = 0;  // ph: parity of the stage's last release
+    int slot = 0, slot_ph = 0;                        // page ring
+    float rscale = 0.0f, rscale_next = 0.0f;
+    auto radius_scale = [&](int h, int page) {
+      return P.pool.int8_radii ? __half2float(P.pool.radii_scales[int64_t(h) * P.pool.page_capacity + page]) : 0.0f;
+    };
+    if (kMode != kTreeDefault && s < P.n_page_steps) rscale_next = radius_scale(head, s);
     bool ok = true;
-    // Step i: its page is in `use`; the next step's page goes to `fetch`.  False after the last step.
-    auto step = [&](PageRegs& use, PageRegs& fetch) {
-      const uint8_t* now = pg;
+    for (int i = 0; i < count && ok; ++i) {
       const int at = s, h = head;
-      const __half* ahead_rs = rs;
-      const uint8_t* ahead = pg;
-      if (s + 1 < P.n_steps) {
-        ++s;
-        ahead += P.pool.page_bytes;
-        if (rs) ++ahead_rs;
-      } else {
+      if (++s == P.n_steps) {
         s = 0;
         ++seg;
         head = seg / P.row_groups;
-        ahead = P.pool.pages + int64_t(head) * P.pool.page_capacity * P.pool.page_bytes;
-        if (rs) ahead_rs = P.pool.radii_scales + int64_t(head) * P.pool.page_capacity;
       }
-      pg = ahead;
-      rs = ahead_rs;
-      if (tid == 0) *progress = i;
-      if (i + 1 < count && s < P.n_page_steps) load_page<kMode>(fetch, P.pool, pg, rs, tid);
+      if (kMode != kTreeDefault) {
+        rscale = rscale_next;
+        if (i + 1 < count && s < P.n_page_steps) rscale_next = radius_scale(head, s);
+      }
       const uint32_t stage = stages + st * kTreeStage;
-      ok = i < kTreeStages || wait_bar(kv_empty + st, ph, stop);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) return false;
+      ok = i < kTreeStages || warp_wait(kv_empty + st, ph, stop);
+      if (!ok) break;
       if (at < P.n_page_steps) {
-        decode_step<kMode>(use, P.pool, tab, stage, now, P.visible - at * kTreeKeys, tid);
+        ok = warp_wait(page_full + slot, slot_ph, stop);
+        if (!ok) break;
+        decode_step<kMode>(smem + kOffPages + slot * kPageSlot, P.pool, tab, rscale, stage, P.visible - at * kTreeKeys, tid);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(page_empty + slot);
+        if (++slot == kPageRing) slot = 0, slot_ph ^= 1;
       } else if (at < draft0) {
         const int64_t row0 = int64_t(h) * kPage * kD * (P.tail_f32 ? 4 : 2);
         dense_step(stage, static_cast<const uint8_t*>(P.tail_k) + row0, static_cast<const uint8_t*>(P.tail_v) + row0, kD, kD,
@@ -566,8 +539,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
                    P.kv_f32, n, late + (d0 >> 5), tid);
         __syncwarp();
         if (lane == 0) mbar_arrive(scanned);
-        ok = __all_sync(0xffffffffu, wait_bar(scanned, scans & 1, stop));
-        if (!ok) return false;
+        ok = warp_wait(scanned, scans & 1, stop);
+        if (!ok) break;
         ++scans;
         for (int q = 0; q < 4; ++q) {
           const int row = q * 16 + (tid >> 4);
@@ -580,11 +553,6 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
       __syncwarp();
       if (lane == 0) mbar_arrive(kv_full + st);
       if (++st == kTreeStages) st = 0, ph ^= 1;
-      return ++i < count;
-    };
-    PageRegs even, odd;
-    if (count && s < P.n_page_steps) load_page<kMode>(even, P.pool, pg, rs, tid);
-    while (step(even, odd) && step(odd, even)) {
     }
   } else if (fewer_registers<kTreeIssueRegs>(); warp == 16) {
     constexpr uint32_t kScores = mma_idesc(false, kTreeKeys, false), kOut = mma_idesc(false, kD, true);
@@ -647,20 +615,26 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
     __syncwarp();
     drain_bar(drained, 0);
     __syncwarp();
-  } else if (warp == 17 && lane == 0) {
-    // Pages are fetched into L2 kAhead steps before the decode warps load them.  (One thread that does
-    // nothing else: issuing a bulk operation blocks it for some hundred cycles.)
-    int s = step0, seg = seg0;
-    const long long t0 = clock64();
-    for (int i = 0; i < count && !*stop; ++i) {
-      while (i - *progress > kAhead && !*stop && clock64() - t0 < kWaitCycles) __nanosleep(50);
+  } else if (warp == 17 && lane < kPageCopiers) {
+    // Each of four lanes copies a quarter of every page (issuing a copy blocks a thread for some hundred
+    // cycles; lanes dispatch in parallel).
+    const uint32_t part = P.pool.page_bytes / kPageCopiers;
+    const uint64_t policy = l2_evict_first_policy();
+    int s = step0, seg = seg0, slot = 0, slot_ph = 1, issued = 0;
+    for (int i = 0; i < count; ++i) {
       if (s < P.n_page_steps) {
+        if (issued >= kPageRing && !wait_bar(page_empty + slot, slot_ph, stop)) break;
         const uint8_t* pg =
-            P.pool.pages + (int64_t(seg / P.row_groups) * P.pool.page_capacity + s) * P.pool.page_bytes;
-        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(pg), "r"(P.pool.page_bytes) : "memory");
+            P.pool.pages + (int64_t(seg / P.row_groups) * P.pool.page_capacity + s) * P.pool.page_bytes + lane * part;
+        mbar_arrive_expect_tx(page_full + slot, part);
+        bulk_g2s_hint(smem + kOffPages + slot * kPageSlot + lane * part, pg, part, page_full + slot, policy);
+        ++issued;
+        if (++slot == kPageRing) slot = 0, slot_ph ^= 1;
       }
       if (++s == P.n_steps) s = 0, ++seg;
     }
+    // No copy may be in flight when the CTA ends.
+    for (int i = max(0, issued - kPageRing); i < issued; ++i) drain_bar(page_full + i % kPageRing, (i / kPageRing) & 1);
   }
   __syncthreads();
   if (warp == 16) {
