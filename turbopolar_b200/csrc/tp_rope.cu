@@ -28,9 +28,10 @@ struct RopeParams {
   const void *cos, *sin;
   const void* positions;
   int64_t table_stride, pos_b, pos_t;
-  int64_t n_units;      // batch * tokens * head groups
+  uint32_t n_units;     // batch * tokens * head groups
   int batch, tokens, hq, hkv, table_rows, table_b_rows;
   int pos64, table_dtype, weight_dtype, interleaved;
+  int table_words, weight_words;  // rows allow loads of four elements at a time
   float eps;
 };
 
@@ -60,8 +61,26 @@ template <> struct Pack4<__nv_bfloat16> {
   }
 };
 
+// N (2 or 4) weights or angles from element i; `words`: N elements on their own boundary.
 template <int N>
-__device__ __forceinline__ void load_small(const void* p, int64_t i, int dtype, float* f) {  // weights and angle rows
+__device__ __forceinline__ void load_small(const void* p, int64_t i, int dtype, bool words, float* f) {
+  if (dtype == TP_F32 && words) {
+    const float* q = static_cast<const float*>(p) + i;
+    if (N == 4) {
+      const float4 v = __ldg(reinterpret_cast<const float4*>(q));
+      f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w;
+    } else {
+      const float2 v = __ldg(reinterpret_cast<const float2*>(q));
+      f[0] = v.x, f[1] = v.y;
+    }
+    return;
+  }
+  if (words && N == 4) {
+    const uint2 v = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i));
+    if (dtype == TP_F16) reinterpret_cast<const Pack4<__half>&>(v).get(f);
+    else reinterpret_cast<const Pack4<__nv_bfloat16>&>(v).get(f);
+    return;
+  }
 #pragma unroll
   for (int j = 0; j < N; ++j) {
     f[j] = dtype == TP_F32   ? static_cast<const float*>(p)[i + j]
@@ -71,26 +90,29 @@ __device__ __forceinline__ void load_small(const void* p, int64_t i, int dtype, 
 }
 
 // kRows heads of one token per 16-lane group.
-template <typename T, int kRows>
+template <typename T, int kRows, bool kInterleaved>
 __global__ void __launch_bounds__(256) norm_rope_kernel(const __grid_constant__ RopeParams P) {
   const int lane = threadIdx.x & 15;
   const unsigned group_mask = 0xffffu << (threadIdx.x & 16);
-  const int64_t unit = (int64_t(blockIdx.x) * blockDim.x + threadIdx.x) >> 4;
+  const uint32_t unit = blockIdx.x * (blockDim.x >> 4) + (threadIdx.x >> 4);
   if (unit >= P.n_units) return;
   const int heads = P.hq + P.hkv;
-  const int hgroups = (heads + kRows - 1) / kRows;
-  const int64_t row = unit / hgroups;
+  const uint32_t hgroups = (heads + kRows - 1) / kRows;
+  const uint32_t row = unit / hgroups;
   const int h0 = int(unit - row * hgroups) * kRows;
-  const int b = int(row / P.tokens), t = int(row - int64_t(b) * P.tokens);
+  const int b = int(row / uint32_t(P.tokens)), t = int(row - uint32_t(b) * uint32_t(P.tokens));
 
   Pack4<T> raw[kRows][2];
+  const T* in = nullptr;  // of row r; a group may hold the last query heads and the first key heads
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
     const int h = h0 + r;
     if (h < heads) {
       const RopeSide& S = h < P.hq ? P.q : P.k;
-      const int hs = h < P.hq ? h : h - P.hq;
-      const T* in = static_cast<const T*>(S.in) + b * S.in_b + t * S.in_t + hs * S.in_h + 4 * lane;
+      if (r == 0 || h == P.hq)
+        in = static_cast<const T*>(S.in) + b * S.in_b + t * S.in_t + (h < P.hq ? h : h - P.hq) * S.in_h + 4 * lane;
+      else
+        in += S.in_h;
       raw[r][0] = *reinterpret_cast<const Pack4<T>*>(in);
       raw[r][1] = *reinterpret_cast<const Pack4<T>*>(in + 64);
     }
@@ -106,65 +128,74 @@ __global__ void __launch_bounds__(256) norm_rope_kernel(const __grid_constant__ 
   float c[4], s[4];
   if (known) {
     const int64_t base = pos * P.table_stride;
-    if (P.interleaved) {
-      load_small<2>(P.cos, base + 2 * lane, P.table_dtype, c);
-      load_small<2>(P.cos, base + 32 + 2 * lane, P.table_dtype, c + 2);
-      load_small<2>(P.sin, base + 2 * lane, P.table_dtype, s);
-      load_small<2>(P.sin, base + 32 + 2 * lane, P.table_dtype, s + 2);
+    if (kInterleaved) {
+      load_small<2>(P.cos, base + 2 * lane, P.table_dtype, P.table_words, c);
+      load_small<2>(P.cos, base + 32 + 2 * lane, P.table_dtype, P.table_words, c + 2);
+      load_small<2>(P.sin, base + 2 * lane, P.table_dtype, P.table_words, s);
+      load_small<2>(P.sin, base + 32 + 2 * lane, P.table_dtype, P.table_words, s + 2);
     } else {
-      load_small<4>(P.cos, base + 4 * lane, P.table_dtype, c);
-      load_small<4>(P.sin, base + 4 * lane, P.table_dtype, s);
+      load_small<4>(P.cos, base + 4 * lane, P.table_dtype, P.table_words, c);
+      load_small<4>(P.sin, base + 4 * lane, P.table_dtype, P.table_words, s);
     }
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i) c[i] = s[i] = __int_as_float(0x7fc00000);
   }
+  // With x the channels as they are, out_a = inv (x_a ac - x_b bs) and out_b = inv (x_b bc + x_a as):
+  // the weights are multiplied into the angles once per group instead of once per row.
+  float ac[4], bs[4], bc[4], as[4];
+  T* out = nullptr;
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
     const int h = h0 + r;
     if (h >= heads) break;  // uniform in the group
     const RopeSide& S = h < P.hq ? P.q : P.k;
-    const int hs = h < P.hq ? h : h - P.hq;
     float lo[4], hi[4];
     raw[r][0].get(lo);
     raw[r][1].get(hi);
+    if (r == 0 || h == P.hq) {
+      out = static_cast<T*>(S.out) + b * S.out_b + t * S.out_t + (h < P.hq ? h : h - P.hq) * S.out_h + 4 * lane;
+      float wl[4] = {1.f, 1.f, 1.f, 1.f}, wh[4] = {1.f, 1.f, 1.f, 1.f};
+      if (S.weight) {
+        load_small<4>(S.weight, 4 * lane, P.weight_dtype, P.weight_words, wl);
+        load_small<4>(S.weight, 64 + 4 * lane, P.weight_dtype, P.weight_words, wh);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        // Pair i of the lane: channels (lo[i], hi[i]), or with adjacent pairs (lo[2i], lo[2i + 1]), then of hi.
+        const float wa = kInterleaved ? (i < 2 ? wl[2 * i] : wh[2 * i - 4]) : wl[i];
+        const float wb = kInterleaved ? (i < 2 ? wl[2 * i + 1] : wh[2 * i - 3]) : wh[i];
+        ac[i] = wa * c[i], bs[i] = wb * s[i], bc[i] = wb * c[i], as[i] = wa * s[i];
+      }
+    } else {
+      out += S.out_h;
+    }
+    float inv = 1.0f;
     if (S.weight) {
       float ss = 0.f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) ss = fmaf(lo[i], lo[i], fmaf(hi[i], hi[i], ss));
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) ss += __shfl_xor_sync(group_mask, ss, o);
-      const float inv = rsqrtf(ss * (1.0f / kD) + P.eps);
-      float wl[4], wh[4];
-      load_small<4>(S.weight, 4 * lane, P.weight_dtype, wl);
-      load_small<4>(S.weight, 64 + 4 * lane, P.weight_dtype, wh);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        lo[i] = lo[i] * inv * wl[i];
-        hi[i] = hi[i] * inv * wh[i];
-      }
+      inv = rsqrtf(ss * (1.0f / kD) + P.eps);
     }
-    float ol[4], oh[4];
-    if (P.interleaved) {
+    float a[4], e[4];  // the pairs' first and second channels
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        ol[2 * i] = lo[2 * i] * c[i] - lo[2 * i + 1] * s[i];
-        ol[2 * i + 1] = lo[2 * i + 1] * c[i] + lo[2 * i] * s[i];
-        oh[2 * i] = hi[2 * i] * c[2 + i] - hi[2 * i + 1] * s[2 + i];
-        oh[2 * i + 1] = hi[2 * i + 1] * c[2 + i] + hi[2 * i] * s[2 + i];
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        ol[i] = lo[i] * c[i] - hi[i] * s[i];
-        oh[i] = hi[i] * c[i] + lo[i] * s[i];
-      }
+    for (int i = 0; i < 4; ++i) {
+      a[i] = kInterleaved ? (i < 2 ? lo[2 * i] : hi[2 * i - 4]) : lo[i];
+      e[i] = kInterleaved ? (i < 2 ? lo[2 * i + 1] : hi[2 * i - 3]) : hi[i];
+      const float x = (a[i] * ac[i] - e[i] * bs[i]) * inv, y = (e[i] * bc[i] + a[i] * as[i]) * inv;
+      a[i] = x, e[i] = y;
     }
-    T* out = static_cast<T*>(S.out) + b * S.out_b + t * S.out_t + hs * S.out_h + 4 * lane;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      lo[i] = kInterleaved ? (i & 1 ? e[i >> 1] : a[i >> 1]) : a[i];
+      hi[i] = kInterleaved ? (i & 1 ? e[2 + (i >> 1)] : a[2 + (i >> 1)]) : e[i];
+    }
     Pack4<T> p;
-    p.set(ol);
+    p.set(lo);
     *reinterpret_cast<Pack4<T>*>(out) = p;
-    p.set(oh);
+    p.set(hi);
     *reinterpret_cast<Pack4<T>*>(out + 64) = p;
   }
 }
@@ -179,11 +210,15 @@ static void launch_rope(RopeParams& P, cudaStream_t s) {
   const int heads = P.hq + P.hkv;
   const int64_t wide = rows * ((heads + kRopeRows - 1) / kRopeRows);
   if (wide >= 148 * 16) {
-    P.n_units = wide;
-    norm_rope_kernel<T, kRopeRows><<<unsigned((wide + 15) / 16), 256, 0, s>>>(P);
+    P.n_units = uint32_t(wide);
+    const unsigned grid = unsigned((wide + 15) / 16);
+    if (P.interleaved) norm_rope_kernel<T, kRopeRows, true><<<grid, 256, 0, s>>>(P);
+    else norm_rope_kernel<T, kRopeRows, false><<<grid, 256, 0, s>>>(P);
   } else {
-    P.n_units = rows * heads;
-    norm_rope_kernel<T, 1><<<unsigned((P.n_units + 3) / 4), 64, 0, s>>>(P);
+    P.n_units = uint32_t(rows * heads);
+    const unsigned grid = (P.n_units + 3) / 4;
+    if (P.interleaved) norm_rope_kernel<T, 1, true><<<grid, 64, 0, s>>>(P);
+    else norm_rope_kernel<T, 1, false><<<grid, 64, 0, s>>>(P);
   }
 }
 
@@ -228,8 +263,8 @@ extern "C" int tp_norm_rope(const tp_rope_layout* layout, const void* q, const v
   if (!positions && int64_t(L.batch_rows) * (L.batch - 1) + L.tokens > L.table_rows)
     return fail(TP_ERR_INVALID, "tp_norm_rope: the angle table has fewer rows than tokens");
   const int64_t heads = int64_t(L.q_heads) + L.k_heads, tokens = int64_t(L.batch) * L.tokens;
-  if (heads > (1 << 20) || tokens > (int64_t(1) << 32) / heads)
-    return fail(TP_ERR_INVALID, "tp_norm_rope: more than 2^32 rows");
+  if (heads > (1 << 20) || tokens > (int64_t(1) << 31) / heads)
+    return fail(TP_ERR_INVALID, "tp_norm_rope: more than 2^31 rows");
   RopeParams P;
   P.q = rope_side(q, q_out, q_weight, L.q_in, L.q_out);
   P.k = rope_side(k, k_out, k_weight, L.k_in, L.k_out);
@@ -250,6 +285,9 @@ extern "C" int tp_norm_rope(const tp_rope_layout* layout, const void* q, const v
   P.weight_dtype = L.weight_dtype;
   P.interleaved = L.interleaved;
   P.eps = L.eps;
+  const int tw = L.table_dtype == TP_F32 ? 16 : 8, ww = L.weight_dtype == TP_F32 ? 16 : 8;
+  P.table_words = (uintptr_t(cos) | uintptr_t(sin)) % tw == 0 && (L.row_stride % 4 == 0 || L.table_rows == 1);
+  P.weight_words = (uintptr_t(q_weight) | uintptr_t(k_weight)) % ww == 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (L.dtype == TP_F16) launch_rope<__half>(P, s);
   else if (L.dtype == TP_BF16) launch_rope<__nv_bfloat16>(P, s);
