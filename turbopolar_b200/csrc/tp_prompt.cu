@@ -370,7 +370,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
 
 // Rows of split token blocks: 32 rows x 8 channels per block.
 template <bool kBf16>
-__global__ void __launch_bounds__(kMergeThreads) merge_items_kernel(const __grid_constant__ PromptParams P) {
+__global__ void __launch_bounds__(kMergeThreads, 4) merge_items_kernel(const __grid_constant__ PromptParams P) {
   const PromptMerge m = P.merges[blockIdx.x / P.hkv];
   const int kvh = blockIdx.x % P.hkv;
   const int tile_rows = P.tile_tokens * P.group;
@@ -379,15 +379,17 @@ __global__ void __launch_bounds__(kMergeThreads) merge_items_kernel(const __grid
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (rows <= 0) return;
   const int64_t rec = int64_t(m.slot) * P.hkv + kvh;
-  const float v = merge_block(P.rec_ml + rec * kRecordRows + r0,
-                              reinterpret_cast<const float4*>(P.rec_o) + (rec * 32 + 2 * blockIdx.z) * kRecordRows + r0,
-                              int64_t(P.hkv) * kRecordRows, int64_t(P.hkv) * 32 * kRecordRows, kRecordRows, m.n, rows);
-  const int row = threadIdx.x >> 3;
-  if (row >= rows) return;
-  const int i = t * tile_rows + (r0 & 127) + row;
-  const int64_t at = ((int64_t(m.q_row) + i / P.group) * P.hq + kvh * P.group + i % P.group) * kD + 8 * blockIdx.z +
-                     (threadIdx.x & 7);
-  P.out[at] = uint16_t(pack2<kBf16>(v, 0.0f));
+  MergePart p;
+  if (!merge_records<false>(p, P.rec_ml + rec * kRecordRows + r0,
+                            reinterpret_cast<const float4*>(P.rec_o) + (rec * 32 + 2 * blockIdx.z) * kRecordRows + r0,
+                            int64_t(P.hkv) * kRecordRows, int64_t(P.hkv) * 32 * kRecordRows, kRecordRows, m.n, rows) ||
+      int(threadIdx.x) >= rows)
+    return;
+  const int i = t * tile_rows + (r0 & 127) + threadIdx.x;
+  const int64_t at = ((int64_t(m.q_row) + i / P.group) * P.hq + kvh * P.group + i % P.group) * kD + 8 * blockIdx.z;
+  *reinterpret_cast<uint4*>(P.out + at) =
+      make_uint4(pack2<kBf16>(p.acc[0], p.acc[1]), pack2<kBf16>(p.acc[2], p.acc[3]), pack2<kBf16>(p.acc[4], p.acc[5]),
+                 pack2<kBf16>(p.acc[6], p.acc[7]));
 }
 
 // ----------------------------------------------------------------------------- host

@@ -59,8 +59,7 @@ struct TreeParams {
   int tail_f32, q_f32, kv_f32;
   int heads, hkv, hq, group, drafts, rows;  // heads: batch * hkv; rows: drafts * group
   int row_groups, n_page_steps, tail_len, n_tail_steps, n_steps, visible;
-  int64_t total;                            // segments * n_steps
-  int grid;
+  int grid, range, longer;                  // CTAs; steps of each, one more in the first `longer` of them
   float scale_log2;
   const void *q, *k, *v;
   int64_t q_b, q_h, q_t, k_b, k_h, k_t, v_b, v_h, v_t;
@@ -74,7 +73,12 @@ struct TreeParams {
   float2 cs[512];                           // (cos, sin) of the level-1 codes, then of the deep codes
 };
 
-__device__ __forceinline__ int64_t range_begin(const TreeParams& P, int cta) { return P.total * cta / P.grid; }
+__device__ __forceinline__ int range_begin(const TreeParams& P, int cta) { return P.range * cta + min(cta, P.longer); }
+// The CTA whose range holds step f of the flat list.
+__device__ __forceinline__ int range_of(const TreeParams& P, int f) {
+  const int split = P.longer * (P.range + 1);
+  return f < split ? f / (P.range + 1) : P.longer + (f - split) / P.range;
+}
 
 // Unit layout of the two specialised formats: offsets known to the compiler become part of the load
 // instructions.
@@ -301,9 +305,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
   asm volatile("griddepcontrol.launch_dependents;");  // merge_pieces_kernel waits for this grid itself
   const uint32_t tmem = *tmem_slot;
   if (tmem != 0 && threadIdx.x == 0) *stop = 1;  // all 512 columns: always at 0
-  const int64_t f0 = range_begin(P, blockIdx.x), f1 = range_begin(P, blockIdx.x + 1);
-  const int seg0 = int(f0 / P.n_steps), step0 = int(f0 - int64_t(seg0) * P.n_steps);
-  const int count = int(f1 - f0);
+  const int f0 = range_begin(P, blockIdx.x), count = range_begin(P, blockIdx.x + 1) - f0;
+  const int seg0 = f0 / P.n_steps, step0 = f0 - seg0 * P.n_steps;
   const int draft0 = P.n_page_steps + P.n_tail_steps;  // first step of draft tiles
 
   if (warp < 8) {
@@ -644,28 +647,30 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
   if (threadIdx.x == 0 && *stop) *P.error = 1;
 }
 
-// Rows of segments that several CTAs worked on: 32 rows x 8 channels per block.
-__global__ void __launch_bounds__(kMergeThreads) merge_pieces_kernel(const __grid_constant__ TreeParams P) {
+// Rows of segments that several CTAs worked on: 32 rows x 8 channels per block, or per warp where a
+// segment has few records.
+template <bool kFew>
+__global__ void __launch_bounds__(kMergeThreads, kFew ? 2 : 4) merge_pieces_kernel(const __grid_constant__ TreeParams P) {
   const int seg = blockIdx.x, head = seg / P.row_groups, rg = seg - head * P.row_groups;
   const int i0 = blockIdx.y * 32, rows = min(32, min(kGroupRows, P.rows - rg * kGroupRows) - i0);
-  // CTAs whose ranges meet the segment's steps [f0, f1).
-  const int64_t f0 = int64_t(seg) * P.n_steps, f1 = f0 + P.n_steps;
-  int first = int(f0 * P.grid / P.total);
-  while (range_begin(P, first + 1) <= f0) ++first;
-  int last = int((f1 - 1) * P.grid / P.total);
-  while (range_begin(P, last + 1) < f1) ++last;
+  const int part = kFew ? blockIdx.z * (kMergeThreads / 32) + (threadIdx.x >> 5) : blockIdx.z;  // channels 8 part ..
+  const int lane = threadIdx.x & 31;
+  // CTAs whose ranges meet the segment's steps.
+  const int first = range_of(P, seg * P.n_steps), last = range_of(P, (seg + 1) * P.n_steps - 1);
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (rows <= 0 || first == last) return;  // one CTA: it has written the rows
   const int64_t rec = int64_t(first) + seg;
-  const float v = merge_block(P.rec_ml + rec * P.rec_rows + i0,
-                              reinterpret_cast<const float4*>(P.rec_o) + (rec * 32 + 2 * blockIdx.z) * P.rec_rows + i0,
-                              P.rec_rows, int64_t(32) * P.rec_rows, P.rec_rows, last - first + 1, rows);
-  const int row = threadIdx.x >> 3;
-  if (row >= rows) return;
-  const int r = rg * kGroupRows + i0 + row;
+  MergePart p;
+  if (!merge_records<kFew>(p, P.rec_ml + rec * P.rec_rows + i0,
+                           reinterpret_cast<const float4*>(P.rec_o) + (rec * 32 + 2 * part) * P.rec_rows + i0, P.rec_rows,
+                           int64_t(32) * P.rec_rows, P.rec_rows, last - first + 1, rows) ||
+      lane >= rows)
+    return;
+  const int r = rg * kGroupRows + i0 + lane;
   const int batch = head / P.hkv, kvh = head - batch * P.hkv, g = r / P.drafts, t = r - g * P.drafts;
-  P.out[((int64_t(batch) * P.drafts + t) * P.hq + int64_t(kvh) * P.group + g) * kD + 8 * blockIdx.z + (threadIdx.x & 7)] =
-      __float2half_rn(v);
+  *reinterpret_cast<uint4*>(P.out + ((int64_t(batch) * P.drafts + t) * P.hq + int64_t(kvh) * P.group + g) * kD + 8 * part) =
+      make_uint4(pack_h2(p.acc[0], p.acc[1]), pack_h2(p.acc[2], p.acc[3]), pack_h2(p.acc[4], p.acc[5]),
+                 pack_h2(p.acc[6], p.acc[7]));
 }
 
 // ----------------------------------------------------------------------------- host
@@ -683,7 +688,10 @@ static int launch_tree(const TreeParams& P, int segments, cudaStream_t s) {
   if (e != cudaSuccess) return fail(TP_ERR_CUDA, std::string("tp_tree_attention: ") + cudaGetErrorString(e));
   tree_attention_kernel<kMode, kPair><<<P.grid, kTreeThreads, kTreeSmem, s>>>(P);
   if (P.grid > 1) {
-    e = launch_dependent(merge_pieces_kernel, dim3(segments, (P.rec_rows + 31) / 32, kD / 8), kMergeThreads, s, P);
+    const int blocks = (P.rec_rows + 31) / 32;
+    const bool few = P.n_steps / P.range + 2 <= kFewRecords;  // CTAs that can share a segment
+    e = few ? launch_dependent(merge_pieces_kernel<true>, dim3(segments, blocks, kD / 8 / (kMergeThreads / 32)), kMergeThreads, s, P)
+            : launch_dependent(merge_pieces_kernel<false>, dim3(segments, blocks, kD / 8), kMergeThreads, s, P);
     if (e != cudaSuccess) return fail(TP_ERR_CUDA, std::string("tp_tree_attention: ") + cudaGetErrorString(e));
   }
   return check_launch("tp_tree_attention");
@@ -797,10 +805,12 @@ int tp_tree_attention(const tp_page_pool* pool, const tp_tail* tail, tp_state st
   P.n_tail_steps = P.tail_len > 0;
   P.n_steps = P.n_page_steps + P.n_tail_steps + (D.n_drafts + kTreeKeys - 1) / kTreeKeys;
   const int64_t segments = int64_t(heads) * P.row_groups;
-  P.total = segments * P.n_steps;
-  if (segments > (1 << 24) || P.total > (int64_t(1) << 31))
+  const int64_t total = segments * P.n_steps;
+  if (segments > (1 << 24) || total > (1 << 30))
     return fail(TP_ERR_UNSUPPORTED, "tp_tree_attention: too many heads, drafts or pages");
-  P.grid = int(std::min<int64_t>(device_sms(), P.total));
+  P.grid = int(std::min<int64_t>(device_sms(), total));
+  P.range = int(total / P.grid);
+  P.longer = int(total % P.grid);
   P.scale_log2 = scale * 1.4426950408889634f;
   P.q = q, P.k = k, P.v = v;
   P.q_b = D.q[0], P.q_h = D.q[1], P.q_t = D.q[2];

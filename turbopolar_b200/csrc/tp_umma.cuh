@@ -369,66 +369,88 @@ __device__ __forceinline__ void store_rows64(uint8_t* buf, const uint32_t (&w)[1
 // Partial records of rows whose keys were split over items: unnormalised outputs
 // o[record][channel / 4][row][4] (a warp's 32 rows write whole lines) and (reference, sum) ml[record][row].
 //   M = max ref_k, w_k = 2^(ref_k - M), out = sum w_k o_k / sum w_k sum_k, 0 where nothing was seen.
-// A block of eight warps merges 32 rows x 8 channels: lane = row, warps take every eighth record with
-// all their loads in flight, and a second step adds the warps' parts.  `o`, `ml`: of the first record,
-// the block's first row and channel; `rows` live rows of the block.  Thread i returns channel i % 8
-// of row i / 8.
-constexpr int kMergeThreads = 256;
-__device__ __forceinline__ float merge_block(const float2* ml, const float4* o, int64_t ml_step, int64_t o_step,
-                                             int64_t quad_step, int n, int rows) {
-  __shared__ float part[8][10][33];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+// Lane = row, so that a warp reads whole lines; `o`, `ml`: of the first record, the warp's first row and
+// channel; `rows` live rows.  With few records (kFew) a warp merges 32 rows x 8 channels by itself, else
+// the block's eight warps take every eighth record each and a second step adds their parts.  Either
+// way the eight channels of a row end in one thread, which writes 16 bytes.
+constexpr int kMergeThreads = 256, kFewRecords = 6;
+struct MergePart {
   float ref = -INFINITY, sum = 0.0f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (lane < rows) {
-    for (int k0 = warp; k0 < n; k0 += 32) {  // four records of this warp at a time
-      float2 r[4];
-      float4 x[4], y[4];
+  // Add records k, k + step, ... (at most kLoads, below n) with all their loads in flight.
+  template <int kLoads>
+  __device__ __forceinline__ void add(const float2* ml, const float4* o, int64_t ml_step, int64_t o_step, int64_t quad_step,
+                                      int k, int step, int n) {
+    float2 r[kLoads];
+    float4 x[kLoads], y[kLoads];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int k = k0 + 8 * i;
-        r[i] = make_float2(-INFINITY, 0.0f);
-        if (k < n) {
-          r[i] = ml[k * ml_step + lane];
-          x[i] = o[k * o_step + lane];
-          y[i] = o[k * o_step + quad_step + lane];
-        }
-      }
-      const float top = fmaxf(fmaxf(fmaxf(r[0].x, r[1].x), fmaxf(r[2].x, r[3].x)), ref);
-      const float base = top == -INFINITY ? 0.0f : top;
-      const float f = exp2_approx(ref - base);
-      ref = top;
-      sum *= f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) acc[i] *= f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (k0 + 8 * i >= n) break;
-        const float w = exp2_approx(r[i].x - base);
-        sum = fmaf(w, r[i].y, sum);
-        const float v[8] = {x[i].x, x[i].y, x[i].z, x[i].w, y[i].x, y[i].y, y[i].z, y[i].w};
-#pragma unroll
-        for (int c = 0; c < 8; ++c) acc[c] = fmaf(w, v[c], acc[c]);
+    for (int i = 0; i < kLoads; ++i) {
+      r[i] = make_float2(-INFINITY, 0.0f);
+      x[i] = y[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (k + i * step < n) {
+        r[i] = ml[(k + i * step) * ml_step];
+        x[i] = o[(k + i * step) * o_step];
+        y[i] = o[(k + i * step) * o_step + quad_step];
       }
     }
+    float top = ref;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) top = fmaxf(top, r[i].x);
+    const float base = top == -INFINITY ? 0.0f : top, f = exp2_approx(ref - base);
+    ref = top;
+    sum *= f;
+#pragma unroll
+    for (int c = 0; c < 8; ++c) acc[c] *= f;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      if (k + i * step >= n) break;
+      const float w = exp2_approx(r[i].x - base);
+      const float v[8] = {x[i].x, x[i].y, x[i].z, x[i].w, y[i].x, y[i].y, y[i].z, y[i].w};
+      sum = fmaf(w, r[i].y, sum);
+#pragma unroll
+      for (int c = 0; c < 8; ++c) acc[c] = fmaf(w, v[c], acc[c]);
+    }
   }
-  part[warp][0][lane] = ref;
-  part[warp][1][lane] = sum;
+};
+// Eight merged channels of this lane's row, in acc.  A warp of its own (kFew), or the first warp of a
+// block; the others return false.
+template <bool kFew>
+__device__ __forceinline__ bool merge_records(MergePart& p, const float2* ml, const float4* o, int64_t ml_step,
+                                              int64_t o_step, int64_t quad_step, int n, int rows) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (kFew) {
+    if (lane < rows)
+      for (int k = 0; k < n; k += kFewRecords) p.add<kFewRecords>(ml + lane, o + lane, ml_step, o_step, quad_step, k, 1, n);
+  } else {
+    __shared__ float part[7][10][32];
+    if (lane < rows)
+      for (int k = warp; k < n; k += 24) p.add<3>(ml + lane, o + lane, ml_step, o_step, quad_step, k, 8, n);
+    if (warp) {
+      part[warp - 1][0][lane] = p.ref;
+      part[warp - 1][1][lane] = p.sum;
 #pragma unroll
-  for (int c = 0; c < 8; ++c) part[warp][2 + c][lane] = acc[c];
-  __syncthreads();
-  const int row = threadIdx.x >> 3, c = threadIdx.x & 7;
-  float top = -INFINITY;
+      for (int c = 0; c < 8; ++c) part[warp - 1][2 + c][lane] = p.acc[c];
+    }
+    __syncthreads();
+    if (warp) return false;
+    float top = p.ref;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) top = fmaxf(top, part[k][0][row]);
-  const float base = top == -INFINITY ? 0.0f : top;
-  float l = 0.0f, v = 0.0f;
+    for (int k = 0; k < 7; ++k) top = fmaxf(top, part[k][0][lane]);
+    const float base = top == -INFINITY ? 0.0f : top, f = exp2_approx(p.ref - base);
+    p.sum *= f;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const float w = exp2_approx(part[k][0][row] - base);
-    l = fmaf(w, part[k][1][row], l);
-    v = fmaf(w, part[k][2 + c][row], v);
+    for (int c = 0; c < 8; ++c) p.acc[c] *= f;
+#pragma unroll
+    for (int k = 0; k < 7; ++k) {
+      const float w = exp2_approx(part[k][0][lane] - base);
+      p.sum = fmaf(w, part[k][1][lane], p.sum);
+#pragma unroll
+      for (int c = 0; c < 8; ++c) p.acc[c] = fmaf(w, part[k][2 + c][lane], p.acc[c]);
+    }
   }
-  return l == 0.0f ? 0.0f : v / l;
+  const float inv = p.sum == 0.0f ? 0.0f : 1.0f / p.sum;
+#pragma unroll
+  for (int c = 0; c < 8; ++c) p.acc[c] *= inv;
+  return true;
 }
 
 // Launch a kernel as the programmatic dependent of the previous one in the stream (which lets it
