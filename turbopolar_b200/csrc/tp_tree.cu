@@ -59,7 +59,7 @@ struct TreeParams {
   int tail_f32, q_f32, kv_f32;
   int heads, hkv, hq, group, drafts, rows;  // heads: batch * hkv; rows: drafts * group
   int row_groups, n_page_steps, tail_len, n_tail_steps, n_steps, visible;
-  int grid, range, longer;                  // CTAs; steps of each, one more in the first `longer` of them
+  int total, grid;                          // segments * n_steps; CTAs
   float scale_log2;
   const void *q, *k, *v;
   int64_t q_b, q_h, q_t, k_b, k_h, k_t, v_b, v_h, v_t;
@@ -73,11 +73,14 @@ struct TreeParams {
   float2 cs[512];                           // (cos, sin) of the level-1 codes, then of the deep codes
 };
 
-__device__ __forceinline__ int range_begin(const TreeParams& P, int cta) { return P.range * cta + min(cta, P.longer); }
+__device__ __forceinline__ int range_begin(const TreeParams& P, int cta) {
+  return int(uint64_t(uint32_t(P.total)) * uint32_t(cta) / uint32_t(P.grid));
+}
 // The CTA whose range holds step f of the flat list.
 __device__ __forceinline__ int range_of(const TreeParams& P, int f) {
-  const int split = P.longer * (P.range + 1);
-  return f < split ? f / (P.range + 1) : P.longer + (f - split) / P.range;
+  int cta = int(uint64_t(uint32_t(f)) * uint32_t(P.grid) / uint32_t(P.total));
+  while (range_begin(P, cta + 1) <= f) ++cta;
+  return cta;
 }
 
 // Unit layout of the two specialised formats: offsets known to the compiler become part of the load
@@ -689,7 +692,7 @@ static int launch_tree(const TreeParams& P, int segments, cudaStream_t s) {
   tree_attention_kernel<kMode, kPair><<<P.grid, kTreeThreads, kTreeSmem, s>>>(P);
   if (P.grid > 1) {
     const int blocks = (P.rec_rows + 31) / 32;
-    const bool few = P.n_steps / P.range + 2 <= kFewRecords;  // CTAs that can share a segment
+    const bool few = P.n_steps / (P.total / P.grid) + 2 <= kFewRecords;  // CTAs that can share a segment
     e = few ? launch_dependent(merge_pieces_kernel<true>, dim3(segments, blocks, kD / 8 / (kMergeThreads / 32)), kMergeThreads, s, P)
             : launch_dependent(merge_pieces_kernel<false>, dim3(segments, blocks, kD / 8), kMergeThreads, s, P);
     if (e != cudaSuccess) return fail(TP_ERR_CUDA, std::string("tp_tree_attention: ") + cudaGetErrorString(e));
@@ -809,8 +812,7 @@ int tp_tree_attention(const tp_page_pool* pool, const tp_tail* tail, tp_state st
   if (segments > (1 << 24) || total > (1 << 30))
     return fail(TP_ERR_UNSUPPORTED, "tp_tree_attention: too many heads, drafts or pages");
   P.grid = int(std::min<int64_t>(device_sms(), total));
-  P.range = int(total / P.grid);
-  P.longer = int(total % P.grid);
+  P.total = int(total);
   P.scale_log2 = scale * 1.4426950408889634f;
   P.q = q, P.k = k, P.v = v;
   P.q_b = D.q[0], P.q_h = D.q[1], P.q_t = D.q[2];
