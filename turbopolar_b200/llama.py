@@ -112,6 +112,14 @@ class TurboPolarFastCache(CacheLayerMixin):
         # Append and attention in one tp_decode_step call.
         return self.runtime.decode_step(k_new, v_new, q_squeezed, scale=scale)
 
+    def tree_attention(self, q: torch.Tensor, k_draft: torch.Tensor, v_draft: torch.Tensor, mask: torch.Tensor,
+                       scale: float) -> torch.Tensor:
+        """Attention of drafted tokens over the cache and each other
+        (:meth:`TurboPolarKVCacheRuntime.tree_attention`); nothing is appended.  RoPE'd ``q``
+        ``(B, H_q, T, D)``, ``k_draft, v_draft`` ``(B, H_kv, T, D)``; returns float16 ``(B, H_q, T, D)``."""
+        as_half = lambda x: x if x.dtype in (torch.float16, torch.float32) else x.to(torch.float16)
+        return self.runtime.tree_attention(as_half(q), as_half(k_draft), as_half(v_draft), mask, scale=scale)
+
     def size(self) -> int:
         return self.offset
 
