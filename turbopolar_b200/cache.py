@@ -69,9 +69,11 @@ class TurboPolarKVCacheRuntime:
         self.pool: Optional[PagePool] = None
         self.tail_k: Optional[torch.Tensor] = None
         self.tail_v: Optional[torch.Tensor] = None
+        self._tail: Optional[_lib.Tail] = None
         self.d_state: Optional[torch.Tensor] = None
         self._workspace: Optional[torch.Tensor] = None
         self._tree_workspace: Optional[torch.Tensor] = None
+        self._tree_room = 0
         self._tree_layouts: dict = {}  # checked layouts of tree_attention calls, by shapes, strides and types
         self.n_pages = 0
         self.tail_len = 0
@@ -141,6 +143,7 @@ class TurboPolarKVCacheRuntime:
 
     def _allocate_tail(self):
         dev = self.device
+        self._tail = None
         self.tail_k = guard.zeros((self.heads, PAGE, 128), self._input_dtype, dev, "dense tail (K)")
         self.tail_v = guard.zeros((self.heads, PAGE, 128), self._input_dtype, dev, "dense tail (V)")
         self.d_state = guard.zeros((_lib.STATE_WORDS,), torch.int32, dev, "state words")
@@ -245,8 +248,10 @@ class TurboPolarKVCacheRuntime:
             self.d_state[2] = local_end + self.later_tokens
 
     def tail_struct(self) -> _lib.Tail:
-        return _lib.Tail(self.tail_k.data_ptr(), self.tail_v.data_ptr(),
-                         _lib.TP_F16 if self._input_dtype == torch.float16 else _lib.TP_F32)
+        if self._tail is None:
+            self._tail = _lib.Tail(self.tail_k.data_ptr(), self.tail_v.data_ptr(),
+                                   _lib.TP_F16 if self._input_dtype == torch.float16 else _lib.TP_F32)
+        return self._tail
 
     def pool_struct(self) -> _lib.PagePool:
         if self.pool is not None:
@@ -396,7 +401,8 @@ class TurboPolarKVCacheRuntime:
             raise RuntimeError("TurboPolar cache returned no blocks after append")
         if self.first_page or self.later_tokens:
             raise NotImplementedError("tree_attention works on whole sequences, not on sequence shards")
-        refuse_gradients(q, k_draft, v_draft)
+        if torch.is_grad_enabled():
+            refuse_gradients(q, k_draft, v_draft)
         key = (q.shape, q.stride(), q.dtype, q.device, k_draft.shape, k_draft.stride(), k_draft.dtype, k_draft.device,
                v_draft.shape, v_draft.stride(), v_draft.dtype, v_draft.device, mask.shape, mask.stride(), mask.dtype,
                mask.device)
@@ -412,20 +418,22 @@ class TurboPolarKVCacheRuntime:
                 self._tree_layouts.clear()
             self._tree_layouts[key] = known
         layout, need = known
-        B, Hq, T = layout.batch, layout.num_q_heads, layout.n_drafts
         if out is None:
-            out = torch.empty((B, T, Hq, 128), dtype=torch.float16, device=self.device)
+            out = q.new_empty((q.shape[0], q.shape[2], q.shape[1], 128), dtype=torch.float16)
         else:
+            B, Hq, T = layout.batch, layout.num_q_heads, layout.n_drafts
             check_out(out, (B, T, Hq, 128), torch.float16, self.device, "out")
             if not out.is_contiguous() or out.data_ptr() & 15:
                 raise ValueError("out must be contiguous and 16-byte aligned")
             if not all(disjoint(out, x) for x in (q, k_draft, v_draft)):
                 raise ValueError("out shares memory with an input")
-        if self._tree_workspace is None or self._tree_workspace.numel() < need:
+        if self._tree_room < need:
             self._tree_workspace = torch.zeros(need, dtype=torch.uint8, device=self.device)
-        status = launch(self.device, _lib.lib().tp_tree_attention, self.pool_struct(), self.tail_struct(), self.state(),
-                        layout, qp, kp, vp, mask.data_ptr(), float(self.config.attention_scale if scale is None else scale),
-                        out.data_ptr(), self._tree_workspace.data_ptr(), self._tree_workspace.numel())
+            self._tree_room = need
+        status = launch(self.device, _lib.lib().tp_tree_attention, self.pool_struct(), self.tail_struct(),
+                        _lib.State(self.n_pages, self.tail_len, self.actual_seq_len, 0), layout, qp, kp, vp,
+                        mask.data_ptr(), self.config.attention_scale if scale is None else scale, out.data_ptr(),
+                        self._tree_workspace.data_ptr(), self._tree_room)
         if status:
             _lib.check(status)
         return out.transpose(1, 2)

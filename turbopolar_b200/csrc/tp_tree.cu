@@ -34,6 +34,7 @@ constexpr int kTreeStages = 4;
 constexpr int kPageRing = 3, kPageSlot = 2 * kMaxUnitBytes;  // stored pages on their way
 constexpr int kPageCopiers = 4;
 constexpr int kMaxDrafts = 256;
+constexpr int kWholeSteps = 4;
 constexpr int kGroupRows = 2 * kTile;                 // rows that share a decoded page
 constexpr int kLateRing = 16;                         // segments whose lists may be alive
 constexpr int kTreeThreads = 640;
@@ -70,7 +71,11 @@ struct TreeParams {
   float2* rec_ml;
   int rec_rows;
   int* error;
-  float2 cs[512];                           // (cos, sin) of the level-1 codes, then of the deep codes
+};
+// (cos, sin) of the level-1 codes, then of the deep codes; of the 16 codes of both for the default format.
+template <int kMode>
+struct TreeAngles {
+  float2 cs[kMode == kTreeDefault ? 16 : 512];
 };
 
 __device__ __forceinline__ int range_begin(const TreeParams& P, int cta) {
@@ -256,7 +261,8 @@ __device__ __forceinline__ float load_any(const void* p, int64_t i, int f32) {
 
 // kPair: a tile per softmax warpgroup (more than 128 rows).
 template <int kMode, bool kPair>
-__global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const __grid_constant__ TreeParams P) {
+__global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const __grid_constant__ TreeParams P,
+                                                                          const __grid_constant__ TreeAngles<kMode> A) {
   extern __shared__ __align__(1024) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   float2* tab = reinterpret_cast<float2*>(smem + kOffTab);
@@ -269,8 +275,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
   volatile int* stop = reinterpret_cast<int*>(tmem_slot + 1);
 
   // (cos, sin) of every code; for the default format's 16 codes as float16 pairs, rounded and remainder.
-  for (int i = threadIdx.x; i < (kMode == kTreeDefault ? 16 : 512); i += kTreeThreads) {
-    const float2 cs = P.cs[i];
+  for (int i = threadIdx.x; i < int(sizeof(A.cs) / sizeof(float2)); i += kTreeThreads) {
+    const float2 cs = A.cs[i];
     if (kMode == kTreeDefault) {
       const __half2 hi = __floats2half2_rn(cs.x, cs.y);
       const __half2 lo = __floats2half2_rn(cs.x - __low2float(hi), cs.y - __high2float(hi));
@@ -677,34 +683,6 @@ __global__ void __launch_bounds__(kMergeThreads, kFew ? 2 : 4) merge_pieces_kern
 }
 
 // ----------------------------------------------------------------------------- host
-template <int kMode, bool kPair>
-static int launch_tree(const TreeParams& P, int segments, cudaStream_t s) {
-  static bool allowed[64] = {};  // the attribute belongs to a device's copy of the kernel
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess && (dev >= 64 || !allowed[dev])) {
-    const int st = allow_kernel(reinterpret_cast<const void*>(tree_attention_kernel<kMode, kPair>), kTreeSmem, kTreeThreads,
-                                2 * kTreeSoftmaxRegs + 2 * kTreeDecodeRegs + kTreeIssueRegs, "tp_tree_attention");
-    if (st != TP_OK) return st;
-    if (dev < 64) allowed[dev] = true;
-  }
-  if (e != cudaSuccess) return fail(TP_ERR_CUDA, std::string("tp_tree_attention: ") + cudaGetErrorString(e));
-  tree_attention_kernel<kMode, kPair><<<P.grid, kTreeThreads, kTreeSmem, s>>>(P);
-  if (P.grid > 1) {
-    const int blocks = (P.rec_rows + 31) / 32;
-    const bool few = P.n_steps / (P.total / P.grid) + 2 <= kFewRecords;  // CTAs that can share a segment
-    e = few ? launch_dependent(merge_pieces_kernel<true>, dim3(segments, blocks, kD / 8 / (kMergeThreads / 32)), kMergeThreads, s, P)
-            : launch_dependent(merge_pieces_kernel<false>, dim3(segments, blocks, kD / 8), kMergeThreads, s, P);
-    if (e != cudaSuccess) return fail(TP_ERR_CUDA, std::string("tp_tree_attention: ") + cudaGetErrorString(e));
-  }
-  return check_launch("tp_tree_attention");
-}
-
-template <int kMode>
-static int launch_tree_rows(const TreeParams& P, int segments, cudaStream_t s) {
-  return P.rows > kTile ? launch_tree<kMode, true>(P, segments, s) : launch_tree<kMode, false>(P, segments, s);
-}
-
 // (cos, sin) of every code of 2, 4 or 8 bits, the decoder's angle formula in float32 (rfsn_v11/quant/
 // polar/decoder.py:36-56), cosine and sine rounded to float32; computed once.
 static void copy_angles(float2* cs, int bits) {
@@ -722,6 +700,37 @@ static void copy_angles(float2* cs, int bits) {
     }
   });
   std::copy_n(table[bits], 1 << bits, cs);
+}
+
+template <int kMode, bool kPair>
+static int launch_tree(const TreeParams& P, const tp_format& fmt, int segments, cudaStream_t s) {
+  static bool allowed[64] = {};  // the attribute belongs to a device's copy of the kernel
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev >= 64 || !allowed[dev])) {
+    const int st = allow_kernel(reinterpret_cast<const void*>(tree_attention_kernel<kMode, kPair>), kTreeSmem, kTreeThreads,
+                                2 * kTreeSoftmaxRegs + 2 * kTreeDecodeRegs + kTreeIssueRegs, "tp_tree_attention");
+    if (st != TP_OK) return st;
+    if (dev < 64) allowed[dev] = true;
+  }
+  if (e != cudaSuccess) return fail(TP_ERR_CUDA, std::string("tp_tree_attention: ") + cudaGetErrorString(e));
+  TreeAngles<kMode> A;
+  copy_angles(A.cs, fmt.l1_bits);
+  if (kMode != kTreeDefault) copy_angles(A.cs + 256, fmt.deep_bits);
+  tree_attention_kernel<kMode, kPair><<<P.grid, kTreeThreads, kTreeSmem, s>>>(P, A);
+  if (P.grid != segments) {  // else each CTA has a segment to itself
+    const int blocks = (P.rec_rows + 31) / 32;
+    const bool few = P.n_steps / (P.total / P.grid) + 2 <= kFewRecords;  // CTAs that can share a segment
+    e = few ? launch_dependent(merge_pieces_kernel<true>, dim3(segments, blocks, kD / 8 / (kMergeThreads / 32)), kMergeThreads, s, P)
+            : launch_dependent(merge_pieces_kernel<false>, dim3(segments, blocks, kD / 8), kMergeThreads, s, P);
+    if (e != cudaSuccess) return fail(TP_ERR_CUDA, std::string("tp_tree_attention: ") + cudaGetErrorString(e));
+  }
+  return check_launch("tp_tree_attention");
+}
+
+template <int kMode>
+static int launch_tree_rows(const TreeParams& P, const tp_format& fmt, int segments, cudaStream_t s) {
+  return P.rows > kTile ? launch_tree<kMode, true>(P, fmt, segments, s) : launch_tree<kMode, false>(P, fmt, segments, s);
 }
 
 static int row_groups_of(int64_t rows) { return int((rows + kGroupRows - 1) / kGroupRows); }
@@ -788,7 +797,7 @@ int tp_tree_attention(const tp_page_pool* pool, const tp_tail* tail, tp_state st
   if (!workspace || workspace_bytes < need)
     return fail(TP_ERR_INVALID, "tp_tree_attention: workspace too small (need " + std::to_string(need) + " bytes)");
 
-  static thread_local TreeParams P;  // 4.6 KB, filled anew by each call
+  TreeParams P;
   P.pool = pool_args(*pool, L);
   P.tail_k = tail ? tail->k : nullptr;
   P.tail_v = tail ? tail->v : nullptr;
@@ -811,7 +820,8 @@ int tp_tree_attention(const tp_page_pool* pool, const tp_tail* tail, tp_state st
   const int64_t total = segments * P.n_steps;
   if (segments > (1 << 24) || total > (1 << 30))
     return fail(TP_ERR_UNSUPPORTED, "tp_tree_attention: too many heads, drafts or pages");
-  P.grid = int(std::min<int64_t>(device_sms(), total));
+  // A CTA per segment where that is at most kWholeSteps steps: no second kernel.  Otherwise one CTA per SM.
+  P.grid = int(P.n_steps <= kWholeSteps && segments <= device_sms() ? segments : std::min<int64_t>(device_sms(), total));
   P.total = int(total);
   P.scale_log2 = scale * 1.4426950408889634f;
   P.q = q, P.k = k, P.v = v;
@@ -825,14 +835,12 @@ int tp_tree_attention(const tp_page_pool* pool, const tp_tail* tail, tp_state st
   P.rec_rows = int(std::min<int64_t>(rows, kGroupRows));
   P.rec_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + 256);
   P.rec_ml = reinterpret_cast<float2*>(P.rec_o + (segments + device_sms()) * P.rec_rows * kD);
-  copy_angles(P.cs, pool->fmt.l1_bits);
-  copy_angles(P.cs + 256, pool->fmt.deep_bits);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const tp_format& F = pool->fmt;
   if (F.l1_bits == 4 && F.deep_bits == 4 && F.split_dim == 64 && !F.int8_radii)
-    return launch_tree_rows<kTreeDefault>(P, int(segments), s);
-  if (F.int8_radii && F.split_dim == 0 && F.deep_bits == 8) return launch_tree_rows<kTreeAdapter>(P, int(segments), s);
-  return launch_tree_rows<kTreeGeneral>(P, int(segments), s);
+    return launch_tree_rows<kTreeDefault>(P, F, int(segments), s);
+  if (F.int8_radii && F.split_dim == 0 && F.deep_bits == 8) return launch_tree_rows<kTreeAdapter>(P, F, int(segments), s);
+  return launch_tree_rows<kTreeGeneral>(P, F, int(segments), s);
 }
 
 }  // extern "C"
