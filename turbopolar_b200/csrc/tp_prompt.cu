@@ -193,8 +193,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
         tmem_fence_after();
       }
       if (ok && live) {
-        uint32_t marked = 0;
-        for (int i = 0; i < 4 * kPartial; ++i) marked |= late[i];
+        const bool marked = __any_sync(0xffffffffu, lane < 4 * kPartial && late[lane]);
         const bool merged = it.slot >= 0;
         const int64_t q_row = int64_t(it.q_row) + tok;
         const int64_t rec = int64_t(it.slot) * P.hkv + kvh;

@@ -291,6 +291,12 @@ __device__ __forceinline__ bool softmax_tile(SoftmaxRow& row, uint32_t s_addr, u
 #pragma unroll
     for (int c = 0; c < kCols; ++c) s[c] = sees(c) ? s[c] : -INFINITY;
   }
+  if (first) {  // no reference to try: one pass of maxima costs less than a pass of weights
+    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int c = 0; c < kCols; c += 2) top[c >> 1 & 3] = max3(top[c >> 1 & 3], s[c], s[c + 1]);
+    row.ref = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * scale_log2;
+  }
   const uint64_t scale2 = pair_of(scale_log2, scale_log2);
   uint64_t add[2];
   for (;;) {
