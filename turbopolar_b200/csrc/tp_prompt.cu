@@ -5,14 +5,29 @@
 //
 // One CTA takes one work item: one KV head, one or two tiles of 128 query rows, a range of keys.  A
 // tile's rows are 128 / G tokens times the G query heads of the KV head, so the group's heads read
-// each key tile once and a single token fills G rows.  Four products per key tile (two tiles, Q K^T and P V)
-// run on the tensor cores while the two softmax warpgroups work on each other's turn: the
-// scores of one tile are being made while the weights of the other are.
+// each key tile once and a single token fills G rows.  The two softmax warpgroups work on each other's turn:
+// the tensor cores make the scores of one while the weights of the other are made.
+//   Two query tiles: one per warpgroup, four products per key tile, which is read once for both.
+//   One query tile (batches too small to fill the SMs with pairs): the warpgroups take key tiles in turn, each
+//   with its own reference, sum and accumulator, which are added at the end.  Four single tokens over 22K
+//   keys: 30.6 us with one warpgroup, 27.9 us with both; 148 CTAs of 16 key tiles each: 65.2 and 48.6 us.
 //
-//   warps 0-3, 4-7   softmax of tile 0 / 1, one row per thread; output of the rows
+//   warps 0-3, 4-7   softmax, one row per thread; output of the rows
 //   warp 8           issues the products
-//   warp 9           loads tiles (TMA) into a ring of five 32 KB stages: K0 V0 K1 V1 ...
+//   warp 9           loads tiles (TMA) into a ring of five or six 32 KB stages: K0 V0 K1 V1 ...
 //   warps 10, 11     clean value tiles that some row does not see whole
+//
+// Bound, one 16K prompt of 32 + 8 heads (1.85 to 1.95 ms by the clock that the power limit leaves, about
+// 1,150 TFLOP/s of the causal half's products): exponentials and the chain around them.  128 keys for both tiles
+// take about 3,170 cycles, of which the two softmaxes' special-function work is 2,048 and the products
+// 1,040; what is left is the latency of scores, weights and products after one another.  Keys in units of 64
+// with two score buffers per tile took 4,500 (products with 64 columns wait for shared memory), two issuing
+// warps and a share of the exponentials as polynomials on the FMA pipe were slower too.
+// Bound, packed requests (12 of 1 to 2,500 tokens, 156 us): an item has 7 key tiles in the mean, and its
+// start and end, about 8 us, stand beside 12 us of tiles.  CTAs that stay and take items in turn,
+// with the next item's loads and first scores under the last one's end, gained that back for items of one or
+// two key tiles only (9.1 instead of 9.9 us each) and lost a ring stage: 162 us.
+// Bound, single tokens: memory (100 MB; the floor is 15.3 us), launch, the first loads and the merge.
 //
 // Values that no row may see: keys past the item's range in its last tile belong to another
 // sequence, and a masked weight of 0 times an infinity or NaN is NaN.  Such rows of the last tile are
@@ -32,13 +47,14 @@
 namespace tp {
 
 constexpr int kKeys = 128;               // keys per tile
-constexpr int kRing = 5;                 // K and V tiles in flight
+constexpr int kRing = 6;                 // K and V tiles in flight: six with one query tile, five with two
 constexpr int kPartial = 3;              // partly visible tiles of one item at most: 127 + 255 keys
 // Three warpgroups at 168 registers: 504 in all, of which the softmax threads, with a row of scores
 // each, take 224 and the others 56.
 constexpr int kPromptThreads = 384, kSoftmaxRegs = 224, kIssueRegs = 56;
-constexpr int kPromptBars = 2 * kTileBytes + kRing * kTileBytes;  // byte offset of the barriers
-constexpr int kPromptSmem = kPromptBars + 512;
+constexpr int kPromptMl = kTileBytes + kRing * kTileBytes;  // byte offset of references and sums to exchange
+constexpr int prompt_bars(bool pair) { return kPromptMl + (pair ? 0 : 2 * kTile * 8); }  // of the barriers
+constexpr int prompt_smem(bool pair) { return prompt_bars(pair) + 512; }
 constexpr int kRecordRows = 2 * kTile;   // rows of an item's partial record
 // Tensor memory (a CTA holds all of it, so it starts at column 0): scores of tile t at 128 t.
 constexpr uint32_t kScoreCol = 0, kOutCol = 256;
@@ -113,22 +129,28 @@ __device__ void clean_values(uint8_t* tile, int first, int valid, int which, uin
   }
 }
 
-template <bool kBf16>
+// kPair: items have up to two query tiles, one per softmax warpgroup.  Otherwise an item is one query
+// tile whose key tiles the warpgroups take in turn, each with an accumulator.
+template <bool kBf16, bool kPair>
 __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(const __grid_constant__ PromptParams P) {
   extern __shared__ __align__(1024) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const PromptItem it = P.items[blockIdx.x / P.hkv];
   const int kvh = blockIdx.x % P.hkv;
-  uint8_t* ring = smem + 2 * kTileBytes;
-  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + kPromptBars);
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + prompt_bars(kPair));
   uint64_t *full = q_full + 1, *empty = full + kRing, *s_full = empty + kRing, *p_full = s_full + 2,
-           *o_done = p_full + 2, *asked = o_done + 2, *clean = asked + kPartial, *drained = clean + kPartial;
+           *o_done = p_full + 2, *asked = o_done + 2, *clean = asked + kPartial, *met = clean + kPartial, *drained = met + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
   volatile int* stop = reinterpret_cast<int*>(tmem_slot + 1);
   uint32_t* late = tmem_slot + 2;  // [kPartial][4]: marked keys, from key partial * 128 on
+  // The item for the end of the softmax threads, which have no registers for it while they work.
+  volatile PromptItem* held = reinterpret_cast<PromptItem*>(late + 4 * kPartial);
 
   const int n_tiles = (it.k_end - it.k_begin + kKeys - 1) / kKeys;
-  const bool two = it.q_tokens > P.tile_tokens;
+  const int nt = kPair && it.q_tokens > P.tile_tokens ? 2 : 1;  // query tiles
+  // With one query tile the second's memory belongs to the ring.
+  constexpr int stages = kPair ? kRing - 1 : kRing;
+  uint8_t* ring = smem + (kPair ? 2 : 1) * kTileBytes;
   // Tiles from `partial` on are not seen whole by every row (or end after the item's keys).
   const int whole = min(it.sees, it.k_end) - it.k_begin;
   const int partial = whole <= 0 ? 0 : whole / kKeys;
@@ -148,8 +170,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
       mbar_init(asked + i, 1);
       mbar_init(clean + i, 2);
     }
+    if (!kPair) mbar_init(met, 8);
     mbar_init(drained, 1);
     *stop = 0;
+    held->q_row = it.q_row, held->q_tokens = it.q_tokens;
+    held->k_row = it.k_row, held->k_begin = it.k_begin, held->slot = it.slot;
     for (int i = 0; i < 4 * kPartial; ++i) late[i] = 0;
     fence_mbar_init();
   }
@@ -164,154 +189,244 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
   if (warp < 8) {
     more_registers<kSoftmaxRegs>();
     const int t = warp >> 2;
-    const int r = (warp & 3) * 32 + lane;
-    const int tok = t * P.tile_tokens + r / P.group, head = kvh * P.group + r % P.group;
-    const bool valid = r < P.tile_tokens * P.group && tok < it.q_tokens;
+    int r = (warp & 3) * 32 + lane;
     const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
     const uint32_t s_addr = kScoreCol + 128 * t + lanes, o_addr = kOutCol + 128 * t + lanes;
-    // Rows that are not there see everything, so they ask for no masking; they are not written.
-    const int limit = valid ? min(it.sees + tok, it.k_end) : it.k_end;
-    const bool live = __any_sync(0xffffffffu, valid);
+    // Keys of the item that the row sees.  Rows that are not there see everything, so they ask for no masking;
+    // they are not written.
+    auto token = [&](int row) { return (kPair ? t * P.tile_tokens : 0) + row / P.group; };
+    auto exists = [&](int row, int tok, int q_tokens) { return row < P.tile_tokens * P.group && tok < q_tokens; };
+    const int limit = (exists(r, token(r), it.q_tokens) ? min(it.sees + token(r), it.k_end) : it.k_end) - it.k_begin;
+    const bool live = __any_sync(0xffffffffu, exists(r, token(r), it.q_tokens));
     SoftmaxRow row;
     bool ok = true;
-    if (t == 0 || two) {
-      for (int j = 0; j < n_tiles && ok; ++j) {
-        ok = __all_sync(0xffffffffu, wait_bar(s_full + t, j & 1, stop));
+    int n = 0;  // tiles of this warpgroup so far: all of the item's, or every second one
+    if constexpr (kPair) {  // two loops: one for both forms, with a variable step, cost pairs 2.5%
+      if (t < nt) {
+        for (int j = 0; j < n_tiles && ok; ++j) {
+          ok = __all_sync(0xffffffffu, wait_bar(s_full + t, j & 1, stop));
+          if (ok && live) {
+            tmem_fence_after();
+            ok = softmax_tile<kKeys, kBf16>(row, s_addr, o_addr, FirstN{limit - j * kKeys}, P.scale_log2, j == 0,
+                                            [&] { return wait_bar(o_done + t, (j - 1) & 1, stop); });
+            tmem_fence_before();
+          }
+          __syncwarp();
+          if (ok && lane == 0) mbar_arrive(p_full + t);
+        }
+        n = n_tiles;
+      }
+    } else {
+      for (int j = t; j < n_tiles && ok; j += 2, ++n) {
+        ok = __all_sync(0xffffffffu, wait_bar(s_full + t, n & 1, stop));
         if (ok && live) {
           tmem_fence_after();
-          ok = softmax_tile<kKeys, kBf16>(row, s_addr, o_addr, FirstN{limit - (it.k_begin + j * kKeys)}, P.scale_log2, j == 0,
-                                          [&] { return wait_bar(o_done + t, (j - 1) & 1, stop); });
+          ok = softmax_tile<kKeys, kBf16>(row, s_addr, o_addr, FirstN{limit - j * kKeys}, P.scale_log2, n == 0,
+                                          [&] { return wait_bar(o_done + t, (n - 1) & 1, stop); });
           tmem_fence_before();
         }
         __syncwarp();
         if (ok && lane == 0) mbar_arrive(p_full + t);
       }
-      if (ok && n_tiles) {
-        ok = wait_bar(o_done + t, (n_tiles - 1) & 1, stop);
-        for (int i = 0; i < n_tiles - partial; ++i) ok = ok && wait_bar(clean + i, 0, stop);
-        ok = __all_sync(0xffffffffu, ok);
-        tmem_fence_after();
-      }
-      if (ok && live) {
-        const bool marked = __any_sync(0xffffffffu, lane < 4 * kPartial && late[lane]);
-        const bool merged = it.slot >= 0;
-        const int64_t q_row = int64_t(it.q_row) + tok;
-        const int64_t rec = int64_t(it.slot) * P.hkv + kvh;
-        const float inv = row.sum == 0.0f ? 0.0f : 1.0f / row.sum;
-        uint8_t* dst = valid ? reinterpret_cast<uint8_t*>(P.out + (q_row * P.hq + head) * kD) : nullptr;
+    }
+    if (ok && n) {
+      ok = wait_bar(o_done + t, (n - 1) & 1, stop);
+      for (int i = 0; i < n_tiles - partial; ++i) ok = ok && wait_bar(clean + i, 0, stop);
+      ok = __all_sync(0xffffffffu, ok);
+    }
+    float2 other = make_float2(-INFINITY, 0.0f);
+    if (!kPair && ok) {
+      // Both warpgroups hold parts of the same rows: exchange references and sums, then each writes half
+      // of the channels of both accumulators' weighted sum.
+      float2* ml = reinterpret_cast<float2*>(smem + kPromptMl);
+      ml[t * kTile + r] = make_float2(row.ref, row.sum);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(met);
+      ok = __all_sync(0xffffffffu, wait_bar(met, 0, stop));
+      if (ok) other = ml[(t ^ 1) * kTile + r];
+    }
+    if (ok && live) {
+      tmem_fence_after();
+      const float top = kPair ? row.ref : fmaxf(row.ref, other.x);
+      const float base = top == -INFINITY ? 0.0f : top;
+      const float mine = kPair ? 1.0f : exp2_approx(row.ref - base), others = kPair ? 0.0f : exp2_approx(other.x - base);
+      const float sum = kPair ? row.sum : mine * row.sum + others * other.y;
+      const bool here = n > 0, there = !kPair && n_tiles > (t ^ 1);  // accumulators that hold something
+      const bool marked = __any_sync(0xffffffffu, lane < 4 * kPartial && late[lane]);
+      asm volatile("" : "+r"(r));  // computed again, not kept
+      const int tok = token(r), head = kvh * P.group + r % P.group, slot = held->slot, k_begin = held->k_begin, k_row = held->k_row;
+      const bool valid = exists(r, tok, held->q_tokens), merged = slot >= 0;
+      const int64_t q_row = int64_t(held->q_row) + tok;
+      const int64_t rec = int64_t(slot) * P.hkv + kvh;
+      const int rec_row = (kPair ? t * kTile : 0) + r;
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      uint8_t* dst = valid ? reinterpret_cast<uint8_t*>(P.out + (q_row * P.hq + head) * kD) : nullptr;
+      // The query tile has been read: its memory carries the rows out.
+      uint8_t* buf = smem + (kPair ? t * kTileBytes + (warp & 3) * kStageRows : warp * kStageRows);
+      const int c_begin = kPair ? 0 : 64 * t, c_end = kPair ? kD : 64 * t + 64;
 #pragma unroll 1
-        for (int c = 0; c < kD; c += 32) {
-          float o[32];
-          if (n_tiles) {
-            tmem_ld32(o_addr + c, o);
-            tmem_wait_ld<32>(o);
-          } else {
+      for (int c = c_begin; c < c_end; c += 32) {
+        float o[32];
+        if (here) {
+          tmem_ld32(o_addr + c, o);
+          tmem_wait_ld<32>(o);
+        } else {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = 0.0f;
-          }
-          if (marked && valid) {  // keys with non-finite values that this row sees
-            for (int e = 0; e < kPartial * kKeys; ++e) {
-              const int key = it.k_begin + partial * kKeys + e;
-              if (key >= limit) break;
-              if (!(late[e >> 5] >> (e & 31) & 1)) continue;
-              const uint16_t* qr = P.q + q_row * P.q_t + head * P.q_h;
-              const uint16_t* kr = P.k + (int64_t(it.k_row) + key) * P.k_t + kvh * P.k_h;
-              const uint16_t* vr = P.v + (int64_t(it.k_row) + key) * P.v_t + kvh * P.v_h;
-              float dot = 0.0f;
-              for (int d = 0; d < kD; ++d) dot = fmaf(widen<kBf16>(qr[d]), widen<kBf16>(kr[d]), dot);
-              const float p = exp2_approx(fmaf(dot, P.scale_log2, -row.ref));
-#pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = fmaf(p, widen<kBf16>(vr[c + i]), o[i]);
-            }
-          }
-          __syncwarp();
-          if (merged) {
-            float4* to = reinterpret_cast<float4*>(P.rec_o) + (rec * 32 + c / 4) * kRecordRows + t * kTile + r;
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (valid) to[i * kRecordRows] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-          } else {
-            uint32_t w[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) w[i] = pack2<kBf16>(o[2 * i] * inv, o[2 * i + 1] * inv);
-            // The query tile has been read: its memory carries the rows out.
-            store_rows64(smem + t * kTileBytes + (warp & 3) * kStageRows, w, dst ? dst + 2 * c : nullptr);
-          }
-          __syncwarp();
+          for (int i = 0; i < 32; ++i) o[i] = 0.0f;
         }
-        if (merged && valid) P.rec_ml[rec * kRecordRows + t * kTile + r] = make_float2(row.ref, row.sum);
+        if (!kPair) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] *= mine;
+          if (there) {
+            float x[32];
+            tmem_ld32(kOutCol + 128 * (t ^ 1) + lanes + c, x);
+            tmem_wait_ld<32>(x);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = fmaf(others, x[i], o[i]);
+          }
+        }
+        if (marked && valid) {  // keys with non-finite values that this row sees
+          for (int e = 0; e < kPartial * kKeys; ++e) {
+            if (partial * kKeys + e >= limit) break;
+            const int key = k_begin + partial * kKeys + e;
+            if (!(late[e >> 5] >> (e & 31) & 1)) continue;
+            const uint16_t* qr = P.q + q_row * P.q_t + head * P.q_h;
+            const uint16_t* kr = P.k + (int64_t(k_row) + key) * P.k_t + kvh * P.k_h;
+            const uint16_t* vr = P.v + (int64_t(k_row) + key) * P.v_t + kvh * P.v_h;
+            float dot = 0.0f;
+            for (int d = 0; d < kD; ++d) dot = fmaf(widen<kBf16>(qr[d]), widen<kBf16>(kr[d]), dot);
+            const float p = exp2_approx(fmaf(dot, P.scale_log2, -base));
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = fmaf(p, widen<kBf16>(vr[c + i]), o[i]);
+          }
+        }
+        __syncwarp();
+        if (merged) {
+          float4* to = reinterpret_cast<float4*>(P.rec_o) + (rec * 32 + c / 4) * kRecordRows + rec_row;
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (valid) to[i * kRecordRows] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        } else {
+          uint32_t w[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) w[i] = pack2<kBf16>(o[2 * i] * inv, o[2 * i + 1] * inv);
+          store_rows64(buf, w, dst ? dst + 2 * c : nullptr);
+        }
+        __syncwarp();
       }
+      if (merged && valid && (kPair || t == 0)) P.rec_ml[rec * kRecordRows + rec_row] = make_float2(top, sum);
     }
     tmem_fence_before();
   } else if (fewer_registers<kIssueRegs>(); warp == 8) {
     if (n_tiles) {
       constexpr uint32_t kScores = mma_idesc(kBf16, kKeys, false), kOut = mma_idesc(kBf16, kD, true);
       const uint32_t q_lo = rows_lo(smem_u32(smem)), ring_addr = smem_u32(ring);
-      const int nt = two ? 2 : 1;
-      auto scores = [&](int t, int stage) {  // one thread
+      auto scores = [&](int t, int q_tile, int stage) {  // one thread
         const uint32_t k_lo = rows_lo(ring_addr) + stage * (kTileBytes >> 4);
 #pragma unroll
         for (int ks = 0; ks < kD / 16; ++ks) {
           const uint32_t off = ((ks >> 2) * kHalfTile + (ks & 3) * 32) >> 4;
-          mma_ss(kScoreCol + 128 * t, q_lo + t * (kTileBytes >> 4) + off, k_lo + off, kScores, ks > 0);
+          mma_ss(kScoreCol + 128 * t, q_lo + q_tile * (kTileBytes >> 4) + off, k_lo + off, kScores, ks > 0);
         }
         mma_commit(s_full + t);
       };
+      auto values = [&](int t, uint32_t v_lo, bool add) {  // one thread
+#pragma unroll
+        for (int ks = 0; ks < kKeys / 16; ++ks)
+          mma_ts(kOutCol + 128 * t, kScoreCol + 128 * t + ks * 8, v_lo + ks * (2048 >> 4), kOut, add || ks > 0);
+        mma_commit(o_done + t);
+      };
       // Issuing blocks until the tensor cores take the product, so time spent waiting is time they idle:
       // key and value tiles are waited for one step ahead, in the gaps where the weights are not ready yet.
-      int st = 0, ph = 0;  // stage and phase of the next tile in the ring
-      auto next_tile = [&](bool cleaned, int j) {
-        bool here = warp_wait(full + st, ph, stop);
-        if (here && cleaned && j >= partial) here = warp_wait(clean + j - partial, 0, stop);
-        st = st + 1 == kRing ? (ph ^= 1, 0) : st + 1;
-        return here;
-      };
-      bool ok = warp_wait(q_full, 0, stop) && next_tile(false, 0);
-      if (ok) {
-        tmem_fence_after();
-        if (elect_one()) {
-          for (int t = 0; t < nt; ++t) scores(t, 0);
-          mma_commit(empty);
+      bool ok = warp_wait(q_full, 0, stop);
+      if constexpr (kPair) {
+        int st = 0, ph = 0;  // stage and phase of the next tile in the ring
+        auto next_tile = [&](bool cleaned, int j) {
+          bool here = warp_wait(full + st, ph, stop);
+          if (here && cleaned && j >= partial) here = warp_wait(clean + j - partial, 0, stop);
+          st = st + 1 == stages ? (ph ^= 1, 0) : st + 1;
+          return here;
+        };
+        ok = ok && next_tile(false, 0);
+        if (ok) {
+          tmem_fence_after();
+          if (elect_one()) {
+            for (int t = 0; t < nt; ++t) scores(t, t, 0);
+            mma_commit(empty);
+          }
+          __syncwarp();
         }
-        __syncwarp();
-      }
-      int sv = st;
-      ok = ok && next_tile(true, 0);
-      int sk = st;
-      if (n_tiles > 1) ok = ok && next_tile(false, 1);
-      for (int j = 0; j < n_tiles && ok; ++j) {
-        const bool more = j + 1 < n_tiles;
+        int sv = st;
+        ok = ok && next_tile(true, 0);
+        int sk = st;
+        if (n_tiles > 1) ok = ok && next_tile(false, 1);
+        for (int j = 0; j < n_tiles && ok; ++j) {
+          const bool more = j + 1 < n_tiles;
+          int sv_next = 0, sk_next = 0;
         const uint32_t v_lo = cols_lo(ring_addr, kHalfTile) + sv * (kTileBytes >> 4);
-        int sv_next = 0, sk_next = 0;
-        for (int t = 0; t < nt && ok; ++t) {
-          // The tile's weights times the values, then its next scores (over the weights: products
-          // complete in order).
-          ok = warp_wait(p_full + t, j & 1, stop);
+          for (int t = 0; t < nt && ok; ++t) {
+            // The tile's weights times the values, then its next scores (over the weights: products
+            // complete in order).
+            ok = warp_wait(p_full + t, j & 1, stop);
+            if (!ok) break;
+            tmem_fence_after();
+            if (elect_one()) {
+              values(t, v_lo, j > 0);
+              if (t == nt - 1) mma_commit(empty + sv);
+              if (more) {
+                scores(t, t, sk);
+                if (t == nt - 1) mma_commit(empty + sk);
+              }
+            }
+            __syncwarp();
+            if (t == 0 && more) {
+              sv_next = st;
+              ok = next_tile(true, j + 1);
+            }
+          }
+          if (ok && j + 2 < n_tiles) {
+            sk_next = st;
+            ok = next_tile(false, j + 2);
+          }
+          sv = sv_next;
+          sk = sk_next;
+        }
+      } else {
+        // Key tile j belongs to warpgroup j & 1, and its scores follow the values of tile j - 2.  No tile is
+        // loaded into a stage before the one there has been used, so tiles may be waited for out of order.
+        auto keys_here = [&](int j) { return j >= n_tiles || warp_wait(full + 2 * j % stages, 2 * j / stages & 1, stop); };
+        auto values_here = [&](int j) {
+          return j >= n_tiles || (warp_wait(full + (2 * j + 1) % stages, (2 * j + 1) / stages & 1, stop) &&
+                                  (j < partial || warp_wait(clean + j - partial, 0, stop)));
+        };
+        for (int j = 0; j < min(2, n_tiles) && ok; ++j) {
+          ok = keys_here(j);
           if (!ok) break;
           tmem_fence_after();
           if (elect_one()) {
-#pragma unroll
-            for (int ks = 0; ks < kKeys / 16; ++ks)
-              mma_ts(kOutCol + 128 * t, kScoreCol + 128 * t + ks * 8, v_lo + ks * (2048 >> 4), kOut, j > 0 || ks > 0);
-            mma_commit(o_done + t);
-            if (t == nt - 1) mma_commit(empty + sv);
-            if (more) {
-              scores(t, sk);
-              if (t == nt - 1) mma_commit(empty + sk);
+            scores(j, 0, 2 * j);
+            mma_commit(empty + 2 * j);
+          }
+          __syncwarp();
+        }
+        ok = ok && values_here(0) && keys_here(2);
+        for (int j = 0; j < n_tiles && ok; ++j) {
+          const int t = j & 1;
+          ok = warp_wait(p_full + t, j >> 1 & 1, stop);
+          if (!ok) break;
+          tmem_fence_after();
+          if (elect_one()) {
+            const int sv = (2 * j + 1) % stages, sk = (2 * j + 4) % stages;
+            values(t, cols_lo(ring_addr, kHalfTile) + sv * (kTileBytes >> 4), j > 1);
+            mma_commit(empty + sv);
+            if (j + 2 < n_tiles) {
+              scores(t, 0, sk);
+              mma_commit(empty + sk);
             }
           }
           __syncwarp();
-          if (t == 0 && more) {
-            sv_next = st;
-            ok = next_tile(true, j + 1);
-          }
+          ok = values_here(j + 1) && keys_here(j + 3);
         }
-        if (ok && j + 2 < n_tiles) {
-          sk_next = st;
-          ok = next_tile(false, j + 2);
-        }
-        sv = sv_next;
-        sk = sk_next;
       }
       if (elect_one()) mma_commit(drained);
       __syncwarp();
@@ -319,7 +434,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
     }
     __syncwarp();
   } else if (warp == 9 && n_tiles) {
-    const int nt = two ? 2 : 1;
     if (lane == 0) {
       mbar_arrive_expect_tx(q_full, uint32_t(nt * P.tile_tokens * P.group * 256));
       for (int t = 0; t < nt; ++t)
@@ -330,7 +444,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
     int issued = 0;
     bool ok = true;
     for (int i = 0; i < 2 * n_tiles && ok; ++i) {
-      const int stage = i % kRing, use = i / kRing;
+      const int stage = i % stages, use = i / stages;
       ok = use == 0 || warp_wait(empty + stage, (use - 1) & 1, stop);
       if (!ok) break;
       if (lane == 0) {
@@ -345,12 +459,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
     }
     // No copy may be in flight when the CTA ends.
     drain_bar(q_full, 0);
-    for (int i = max(0, issued - kRing); i < issued; ++i) drain_bar(full + i % kRing, (i / kRing) & 1);
+    for (int i = max(0, issued - stages); i < issued; ++i) drain_bar(full + i % stages, (i / stages) & 1);
   } else if (n_tiles) {
     for (int j = partial; j < n_tiles; ++j) {
       // The stage's barrier is at this tile's phase once the loader has asked for it.
-      const int i = 2 * j + 1, stage = i % kRing;
-      if (!warp_wait(asked + j - partial, 0, stop) || !warp_wait(full + stage, (i / kRing) & 1, stop)) break;
+      const int i = 2 * j + 1, stage = i % stages;
+      if (!warp_wait(asked + j - partial, 0, stop) || !warp_wait(full + stage, (i / stages) & 1, stop)) break;
       const int key = j * kKeys, valid = min(kKeys, it.k_end - it.k_begin - key);
       clean_values<kBf16>(ring + stage * kTileBytes, min(valid, max(0, whole - key)), valid, warp - 10,
                           late + 4 * (j - partial));
@@ -433,22 +547,22 @@ static size_t record_bytes(int64_t slots, int hkv) {
   return size_t(slots) * hkv * kRecordRows * (kD * sizeof(float) + sizeof(float2));
 }
 
-template <bool kBf16>
+template <bool kBf16, bool kPair>
 static int launch_prompt(const PromptParams& P, const tp_prompt_plan& plan, cudaStream_t s) {
   static bool allowed[64] = {};  // the attribute belongs to a device's copy of the kernel
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess && (dev >= 64 || !allowed[dev])) {
-    const int st = allow_kernel(reinterpret_cast<const void*>(prompt_attention_kernel<kBf16>), kPromptSmem, kPromptThreads,
-                                2 * kSoftmaxRegs + kIssueRegs, "tp_prompt_attention");
+    const int st = allow_kernel(reinterpret_cast<const void*>(prompt_attention_kernel<kBf16, kPair>), prompt_smem(kPair),
+                                kPromptThreads, 2 * kSoftmaxRegs + kIssueRegs, "tp_prompt_attention");
     if (st != TP_OK) return st;
     if (dev < 64) allowed[dev] = true;
   }
   if (e != cudaSuccess) return fail(TP_ERR_CUDA, std::string("tp_prompt_attention: ") + cudaGetErrorString(e));
   if (plan.items)
-    prompt_attention_kernel<kBf16><<<unsigned(plan.items) * plan.num_kv_heads, kPromptThreads, kPromptSmem, s>>>(P);
+    prompt_attention_kernel<kBf16, kPair><<<unsigned(plan.items) * plan.num_kv_heads, kPromptThreads, prompt_smem(kPair), s>>>(P);
   if (plan.merges) {
-    const int rows = plan.block_tokens > P.tile_tokens ? kRecordRows : plan.block_tokens * P.group;
+    const int rows = kPair ? kRecordRows : plan.block_tokens * P.group;
     e = launch_dependent(merge_items_kernel<kBf16>, dim3(unsigned(plan.merges) * plan.num_kv_heads, (rows + 31) / 32, kD / 8),
                          kMergeThreads, s, P);
     if (e != cudaSuccess) return fail(TP_ERR_CUDA, std::string("tp_prompt_attention: ") + cudaGetErrorString(e));
@@ -593,7 +707,9 @@ int tp_prompt_attention(const tp_prompt_plan* plan, const int32_t* words, const 
   const size_t slots_rows = (plan->workspace_bytes - 256) / (kD * sizeof(float) + sizeof(float2));
   P.rec_ml = reinterpret_cast<float2*>(P.rec_o + slots_rows * kD);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return bf16 ? launch_prompt<true>(P, *plan, s) : launch_prompt<false>(P, *plan, s);
+  if (plan->block_tokens > P.tile_tokens)
+    return bf16 ? launch_prompt<true, true>(P, *plan, s) : launch_prompt<false, true>(P, *plan, s);
+  return bf16 ? launch_prompt<true, false>(P, *plan, s) : launch_prompt<false, false>(P, *plan, s);
 }
 
 }  // extern "C"

@@ -716,7 +716,7 @@ static int launch_tree(const TreeParams& P, const tp_format& fmt, int segments, 
   if (e != cudaSuccess) return fail(TP_ERR_CUDA, std::string("tp_tree_attention: ") + cudaGetErrorString(e));
   TreeAngles<kMode> A;
   copy_angles(A.cs, fmt.l1_bits);
-  if (kMode != kTreeDefault) copy_angles(A.cs + 256, fmt.deep_bits);
+  if constexpr (kMode != kTreeDefault) copy_angles(A.cs + 256, fmt.deep_bits);
   tree_attention_kernel<kMode, kPair><<<P.grid, kTreeThreads, kTreeSmem, s>>>(P, A);
   if (P.grid != segments) {  // else each CTA has a segment to itself
     const int blocks = (P.rec_rows + 31) / 32;
