@@ -79,6 +79,7 @@ struct PromptParams {
   const PromptItem* items;
   const PromptMerge* merges;
   int hq, hkv, group, tile_tokens;
+  int merged;                 // merge_items_kernel follows
   float scale_log2;
   const uint16_t *q, *k, *v;  // for listed keys
   int64_t q_t, q_h, k_t, k_h, v_t, v_h;
@@ -184,7 +185,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
   tmem_fence_after();
   const uint32_t tmem = *tmem_slot;
   if (tmem != 0 && threadIdx.x == 0) *stop = 1;  // all 512 columns: always at 0
-  asm volatile("griddepcontrol.launch_dependents;");  // merge_items_kernel waits for this grid itself
+  // merge_items_kernel waits for this grid itself; nothing else may start before it has completed.
+  if (P.merged) asm volatile("griddepcontrol.launch_dependents;");
 
   if (warp < 8) {
     more_registers<kSoftmaxRegs>();
@@ -696,6 +698,7 @@ int tp_prompt_attention(const tp_prompt_plan* plan, const int32_t* words, const 
   if (st != TP_OK) return st;
   P.items = reinterpret_cast<const PromptItem*>(words);
   P.merges = reinterpret_cast<const PromptMerge*>(P.items + plan->items);
+  P.merged = plan->merges > 0;
   P.scale_log2 = scale * 1.4426950408889634f;
   P.q = static_cast<const uint16_t*>(q);
   P.k = static_cast<const uint16_t*>(k);

@@ -61,6 +61,7 @@ struct TreeParams {
   int heads, hkv, hq, group, drafts, rows;  // heads: batch * hkv; rows: drafts * group
   int row_groups, n_page_steps, tail_len, n_tail_steps, n_steps, visible;
   int total, grid;                          // segments * n_steps; CTAs
+  int merged;                               // merge_pieces_kernel follows
   float scale_log2;
   const void *q, *k, *v;
   int64_t q_b, q_h, q_t, k_b, k_h, k_t, v_b, v_h, v_t;
@@ -311,7 +312,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
   tmem_fence_before();
   __syncthreads();
   tmem_fence_after();
-  asm volatile("griddepcontrol.launch_dependents;");  // merge_pieces_kernel waits for this grid itself
+  // merge_pieces_kernel waits for this grid itself; nothing else may start before it has completed.
+  if (P.merged) asm volatile("griddepcontrol.launch_dependents;");
   const uint32_t tmem = *tmem_slot;
   if (tmem != 0 && threadIdx.x == 0) *stop = 1;  // all 512 columns: always at 0
   const int f0 = range_begin(P, blockIdx.x), count = range_begin(P, blockIdx.x + 1) - f0;
@@ -718,7 +720,7 @@ static int launch_tree(const TreeParams& P, const tp_format& fmt, int segments, 
   copy_angles(A.cs, fmt.l1_bits);
   if constexpr (kMode != kTreeDefault) copy_angles(A.cs + 256, fmt.deep_bits);
   tree_attention_kernel<kMode, kPair><<<P.grid, kTreeThreads, kTreeSmem, s>>>(P, A);
-  if (P.grid != segments) {  // else each CTA has a segment to itself
+  if (P.merged) {
     const int blocks = (P.rec_rows + 31) / 32;
     const bool few = P.n_steps / (P.total / P.grid) + 2 <= kFewRecords;  // CTAs that can share a segment
     e = few ? launch_dependent(merge_pieces_kernel<true>, dim3(segments, blocks, kD / 8 / (kMergeThreads / 32)), kMergeThreads, s, P)
@@ -823,6 +825,7 @@ int tp_tree_attention(const tp_page_pool* pool, const tp_tail* tail, tp_state st
   // A CTA per segment where that is at most kWholeSteps steps: no second kernel.  Otherwise one CTA per SM.
   P.grid = int(P.n_steps <= kWholeSteps && segments <= device_sms() ? segments : std::min<int64_t>(device_sms(), total));
   P.total = int(total);
+  P.merged = P.grid != segments;  // else each CTA has a segment to itself
   P.scale_log2 = scale * 1.4426950408889634f;
   P.q = q, P.k = k, P.v = v;
   P.q_b = D.q[0], P.q_h = D.q[1], P.q_t = D.q[2];
