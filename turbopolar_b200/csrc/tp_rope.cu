@@ -9,15 +9,17 @@
 //
 // Bound: memory (read + write of q and k; 8,192 bfloat16 tokens of 32 + 8 heads move 172 MB).  A
 // group of 16 lanes owns a row: lane i holds channels [4i, 4i+4) and [64+4i, 64+4i+4), so both
-// pairings are inside one lane and only the sum of squares crosses lanes (four shuffles).
+// pairings are inside one lane and only the sum of squares crosses lanes: for four rows at once in nine
+// shuffles and one reciprocal root, where row by row takes sixteen and four.
 //
-// Measured, those 8,192 tokens: 36.6 us, 4.7 TB/s, where a copy of the size takes 26.6 us.  What is left is
-// instructions (two thirds of the issue slots) and latency: each group loads, works and stores once.
-// Groups of 8 lanes with 16-byte words took 41.7 us (123 registers), two or eight heads per group 44 to
-// 62 us, five heads 45 us.  One token of 40 heads takes 1.9 us, 48 float32 tokens 2.4 us: launch latency.
+// Measured, those 8,192 tokens: 29.7 us, 5.8 TB/s, where a copy of the size takes 26.6 us.  Issue slots are 60%
+// used: a group's heads are all query or all key heads and sums and rotations are two float32 to an instruction,
+// which took 36.6 us to that.  CTAs of 256 threads 31.2 us; bounds for ten or twelve CTAs per SM 31.5 and 40.6.
+// Earlier and slower: groups of 8 lanes with 16-byte words (123 registers), two, five or eight heads per group.
+// One token of 40 heads takes 1.9 us, 48 float32 tokens 2.5 us: launch latency.
 #include <cuda_bf16.h>
 
-#include "tp_common.cuh"
+#include "tp_umma.cuh"
 
 namespace tp {
 
@@ -34,6 +36,7 @@ struct RopeParams {
   const void* positions;
   int64_t table_stride, pos_b, pos_t;
   uint32_t n_units;     // batch * tokens * head groups
+  uint32_t groups, q_groups;  // head groups of a token, and those of its query heads
   int batch, tokens, hq, hkv, table_rows, table_b_rows;
   int pos64, table_dtype, weight_dtype, interleaved;
   int table_words, weight_words;  // rows allow loads of four elements at a time
@@ -94,7 +97,7 @@ __device__ __forceinline__ void load_small(const void* p, int64_t i, int dtype, 
   }
 }
 
-// Many rows pass by once and are marked as the first to leave the L2 (8,192 tokens: 40.0 us without, 37.4 us
+// Many rows pass by once and are marked as the first to leave the L2 (8,192 tokens: 32.5 us without, 29.7 us
 // with); the rows of a few tokens stay for whoever reads them next.
 template <int kRows, typename T>
 __device__ __forceinline__ auto load_row(const T* from) {
@@ -108,32 +111,34 @@ __device__ __forceinline__ void store_row(T* to, const Pack4<T>& x) {
   else *p = x.v;
 }
 
-// kRows heads of one token per 16-lane group.
+__device__ __forceinline__ uint64_t mul_pair(uint64_t a, uint64_t b) {  // two float32 each
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+// kRows query heads, or key heads, of one token per 16-lane group.
 template <typename T, int kRows, bool kInterleaved>
 __global__ void __launch_bounds__(128) norm_rope_kernel(const __grid_constant__ RopeParams P) {
+  static_assert(kRows == 1 || kRows == 4, "the sums of squares are reduced for one row or four");
   const int lane = threadIdx.x & 15;
   const unsigned group_mask = 0xffffu << (threadIdx.x & 16);
   const uint32_t unit = blockIdx.x * (blockDim.x >> 4) + (threadIdx.x >> 4);
   if (unit >= P.n_units) return;
-  const int heads = P.hq + P.hkv;
-  const uint32_t hgroups = (heads + kRows - 1) / kRows;
-  const uint32_t row = unit / hgroups;
-  const int h0 = int(unit - row * hgroups) * kRows;
-  const int b = int(row / uint32_t(P.tokens)), t = int(row - uint32_t(b) * uint32_t(P.tokens));
+  const uint32_t row = unit / P.groups, hg = unit - row * P.groups;
+  const bool is_q = hg < P.q_groups;
+  const RopeSide& S = is_q ? P.q : P.k;
+  const int h0 = int(is_q ? hg : hg - P.q_groups) * kRows;
+  const int n = min(kRows, (is_q ? P.hq : P.hkv) - h0);
+  const int b = P.batch == 1 ? 0 : int(row / uint32_t(P.tokens)), t = int(row - uint32_t(b) * uint32_t(P.tokens));
 
   Pack4<T> raw[kRows][2];
-  const T* in = nullptr;  // of row r; a group may hold the last query heads and the first key heads
+  const T* in = static_cast<const T*>(S.in) + b * S.in_b + t * S.in_t + h0 * S.in_h + 4 * lane;
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
-    const int h = h0 + r;
-    if (h < heads) {
-      const RopeSide& S = h < P.hq ? P.q : P.k;
-      if (r == 0 || h == P.hq)
-        in = static_cast<const T*>(S.in) + b * S.in_b + t * S.in_t + (h < P.hq ? h : h - P.hq) * S.in_h + 4 * lane;
-      else
-        in += S.in_h;
-      raw[r][0].v = load_row<kRows>(in);
-      raw[r][1].v = load_row<kRows>(in + 64);
+    if (r < n) {
+      raw[r][0].v = load_row<kRows>(in + r * S.in_h);
+      raw[r][1].v = load_row<kRows>(in + r * S.in_h + 64);
     }
   }
   // The row of the angle table; a position outside the table gives NaN rows.
@@ -160,62 +165,93 @@ __global__ void __launch_bounds__(128) norm_rope_kernel(const __grid_constant__ 
 #pragma unroll
     for (int i = 0; i < 4; ++i) c[i] = s[i] = __int_as_float(0x7fc00000);
   }
-  // With x the channels as they are, out_a = inv (x_a ac - x_b bs) and out_b = inv (x_b bc + x_a as):
-  // the weights are multiplied into the angles once per group instead of once per row.
-  float ac[4], bs[4], bc[4], as[4];
-  T* out = nullptr;
+  float wl[4] = {1.f, 1.f, 1.f, 1.f}, wh[4] = {1.f, 1.f, 1.f, 1.f};
+  if (S.weight) {
+    load_small<4>(S.weight, 4 * lane, P.weight_dtype, P.weight_words, wl);
+    load_small<4>(S.weight, 64 + 4 * lane, P.weight_dtype, P.weight_words, wh);
+  }
+  // Pair i of the lane: channels (lo[i], hi[i]), or with adjacent pairs (lo[2i], lo[2i + 1]), then of hi.
+  auto first_of = [](const float* lo, const float* hi, int i) {
+    return kInterleaved ? (i < 2 ? lo[2 * i] : hi[2 * i - 4]) : lo[i];
+  };
+  auto second_of = [](const float* lo, const float* hi, int i) {
+    return kInterleaved ? (i < 2 ? lo[2 * i + 1] : hi[2 * i - 3]) : hi[i];
+  };
+  // With x the channels as they are, out_a = inv (x_a ac - x_b bs) and out_b = inv (x_b bc + x_a as), two pairs
+  // at a time: the weights are multiplied into the angles once per group instead of once per row.
+  uint64_t ac[2], bs[2], bc[2], as[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint64_t c2 = pair_of(c[2 * i], c[2 * i + 1]), s2 = pair_of(s[2 * i], s[2 * i + 1]);
+    const uint64_t wa = pair_of(first_of(wl, wh, 2 * i), first_of(wl, wh, 2 * i + 1));
+    const uint64_t wb = pair_of(second_of(wl, wh, 2 * i), second_of(wl, wh, 2 * i + 1));
+    ac[i] = mul_pair(wa, c2), bc[i] = mul_pair(wb, c2), as[i] = mul_pair(wa, s2);
+    bs[i] = mul_pair(wb, pair_of(-s[2 * i], -s[2 * i + 1]));
+  }
+  float inv[kRows];
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) inv[r] = 1.0f;
+  if (S.weight) {
+    float ss[kRows];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      float x[8];
+      raw[r][0].get(x);
+      raw[r][1].get(x + 4);
+      uint64_t sum = 0;
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) {
+        const uint64_t p = pair_of(x[i], x[i + 1]);
+        sum = fma_pair(p, p, sum);
+      }
+      float s0, s1;
+      split_pair(sum, s0, s1);
+      ss[r] = s0 + s1;
+    }
+    if constexpr (kRows == 4) {
+      // Lanes trade the rows they do not keep: after two steps lane l holds row l / 4, and two more end its sum.
+      const bool upper = lane & 8, odd = lane & 4;
+      float a = upper ? ss[2] : ss[0], e = upper ? ss[3] : ss[1];
+      a += __shfl_xor_sync(group_mask, upper ? ss[0] : ss[2], 8);
+      e += __shfl_xor_sync(group_mask, upper ? ss[1] : ss[3], 8);
+      float own = odd ? e : a;
+      own += __shfl_xor_sync(group_mask, odd ? a : e, 4);
+      own += __shfl_xor_sync(group_mask, own, 2);
+      own += __shfl_xor_sync(group_mask, own, 1);
+      own = rsqrtf(own * (1.0f / kD) + P.eps);
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) inv[r] = __shfl_sync(group_mask, own, 4 * r, 16);
+    } else {
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) ss[0] += __shfl_xor_sync(group_mask, ss[0], o);
+      inv[0] = rsqrtf(ss[0] * (1.0f / kD) + P.eps);
+    }
+  }
+  T* out = static_cast<T*>(S.out) + b * S.out_b + t * S.out_t + h0 * S.out_h + 4 * lane;
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
-    const int h = h0 + r;
-    if (h >= heads) break;  // uniform in the group
-    const RopeSide& S = h < P.hq ? P.q : P.k;
-    float lo[4], hi[4];
+    if (r >= n) break;  // uniform in the group
+    float lo[4], hi[4], x[4], y[4];  // x, y: the pairs' first and second channels
     raw[r][0].get(lo);
     raw[r][1].get(hi);
-    if (r == 0 || h == P.hq) {
-      out = static_cast<T*>(S.out) + b * S.out_b + t * S.out_t + (h < P.hq ? h : h - P.hq) * S.out_h + 4 * lane;
-      float wl[4] = {1.f, 1.f, 1.f, 1.f}, wh[4] = {1.f, 1.f, 1.f, 1.f};
-      if (S.weight) {
-        load_small<4>(S.weight, 4 * lane, P.weight_dtype, P.weight_words, wl);
-        load_small<4>(S.weight, 64 + 4 * lane, P.weight_dtype, P.weight_words, wh);
-      }
+    const uint64_t inv2 = pair_of(inv[r], inv[r]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        // Pair i of the lane: channels (lo[i], hi[i]), or with adjacent pairs (lo[2i], lo[2i + 1]), then of hi.
-        const float wa = kInterleaved ? (i < 2 ? wl[2 * i] : wh[2 * i - 4]) : wl[i];
-        const float wb = kInterleaved ? (i < 2 ? wl[2 * i + 1] : wh[2 * i - 3]) : wh[i];
-        ac[i] = wa * c[i], bs[i] = wb * s[i], bc[i] = wb * c[i], as[i] = wa * s[i];
-      }
-    } else {
-      out += S.out_h;
-    }
-    float inv = 1.0f;
-    if (S.weight) {
-      float ss = 0.f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) ss = fmaf(lo[i], lo[i], fmaf(hi[i], hi[i], ss));
-#pragma unroll
-      for (int o = 8; o > 0; o >>= 1) ss += __shfl_xor_sync(group_mask, ss, o);
-      inv = rsqrtf(ss * (1.0f / kD) + P.eps);
-    }
-    float a[4], e[4];  // the pairs' first and second channels
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      a[i] = kInterleaved ? (i < 2 ? lo[2 * i] : hi[2 * i - 4]) : lo[i];
-      e[i] = kInterleaved ? (i < 2 ? lo[2 * i + 1] : hi[2 * i - 3]) : hi[i];
-      const float x = (a[i] * ac[i] - e[i] * bs[i]) * inv, y = (e[i] * bc[i] + a[i] * as[i]) * inv;
-      a[i] = x, e[i] = y;
+    for (int i = 0; i < 2; ++i) {
+      const uint64_t a = pair_of(first_of(lo, hi, 2 * i), first_of(lo, hi, 2 * i + 1));
+      const uint64_t e = pair_of(second_of(lo, hi, 2 * i), second_of(lo, hi, 2 * i + 1));
+      split_pair(mul_pair(fma_pair(a, ac[i], mul_pair(e, bs[i])), inv2), x[2 * i], x[2 * i + 1]);
+      split_pair(mul_pair(fma_pair(e, bc[i], mul_pair(a, as[i])), inv2), y[2 * i], y[2 * i + 1]);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      lo[i] = kInterleaved ? (i & 1 ? e[i >> 1] : a[i >> 1]) : a[i];
-      hi[i] = kInterleaved ? (i & 1 ? e[2 + (i >> 1)] : a[2 + (i >> 1)]) : e[i];
+      lo[i] = kInterleaved ? (i & 1 ? y[i >> 1] : x[i >> 1]) : x[i];
+      hi[i] = kInterleaved ? (i & 1 ? y[2 + (i >> 1)] : x[2 + (i >> 1)]) : y[i];
     }
     Pack4<T> p;
     p.set(lo);
-    store_row<kRows>(out, p);
+    store_row<kRows>(out + r * S.out_h, p);
     p.set(hi);
-    store_row<kRows>(out + 64, p);
+    store_row<kRows>(out + r * S.out_h + 64, p);
   }
 }
 
@@ -226,15 +262,17 @@ constexpr int kRopeRows = 4;
 template <typename T>
 static void launch_rope(RopeParams& P, cudaStream_t s) {
   const int64_t rows = int64_t(P.batch) * P.tokens;
-  const int heads = P.hq + P.hkv;
-  const int64_t wide = rows * ((heads + kRopeRows - 1) / kRopeRows);
+  P.q_groups = (P.hq + kRopeRows - 1) / kRopeRows;
+  P.groups = P.q_groups + (P.hkv + kRopeRows - 1) / kRopeRows;
+  const int64_t wide = rows * P.groups;
   if (wide >= 148 * 16) {
     P.n_units = uint32_t(wide);
     const unsigned grid = unsigned((wide + 7) / 8);
     if (P.interleaved) norm_rope_kernel<T, kRopeRows, true><<<grid, 128, 0, s>>>(P);
     else norm_rope_kernel<T, kRopeRows, false><<<grid, 128, 0, s>>>(P);
   } else {
-    P.n_units = uint32_t(rows * heads);
+    P.q_groups = P.hq, P.groups = P.hq + P.hkv;
+    P.n_units = uint32_t(rows * P.groups);
     const unsigned grid = (P.n_units + 3) / 4;
     if (P.interleaved) norm_rope_kernel<T, 1, true><<<grid, 64, 0, s>>>(P);
     else norm_rope_kernel<T, 1, false><<<grid, 64, 0, s>>>(P);
