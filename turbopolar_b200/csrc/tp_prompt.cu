@@ -23,8 +23,8 @@
 // 1,040; what is left is the latency of scores, weights and products after one another.  Keys in units of 64
 // with two score buffers per tile took 4,500 (products with 64 columns wait for shared memory), two issuing
 // warps and a share of the exponentials as polynomials on the FMA pipe were slower too.
-// Bound, packed requests (12 of 1 to 2,500 tokens, 156 us): an item has 7 key tiles in the mean, and its
-// start and end, about 8 us, stand beside 12 us of tiles.  CTAs that stay and take items in turn,
+// Bound, packed requests (12 of 1 to 2,500 tokens, 153 us): an item has 7 key tiles in the mean, and its
+// start and end, 7 to 8 us, stand beside 12 us of tiles.  CTAs that stay and take items in turn,
 // with the next item's loads and first scores under the last one's end, gained that back for items of one or
 // two key tiles only (9.1 instead of 9.9 us each) and lost a ring stage: 162 us.
 // Bound, single tokens: memory (100 MB; the floor is 15.3 us), launch, the first loads and the merge.
@@ -263,58 +263,71 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
       const int rec_row = (kPair ? t * kTile : 0) + r;
       const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
       uint8_t* dst = valid ? reinterpret_cast<uint8_t*>(P.out + (q_row * P.hq + head) * kD) : nullptr;
-      // The query tile has been read: its memory carries the rows out.
-      uint8_t* buf = smem + (kPair ? t * kTileBytes + (warp & 3) * kStageRows : warp * kStageRows);
-      const int c_begin = kPair ? 0 : 64 * t, c_end = kPair ? kD : 64 * t + 64;
-#pragma unroll 1
-      for (int c = c_begin; c < c_end; c += 32) {
-        float o[32];
-        if (here) {
-          tmem_ld32(o_addr + c, o);
-          tmem_wait_ld<32>(o);
-        } else {
+      // All of the row's channels at once (without pairs, this warpgroup's half of them): the loads and the
+      // stages of shared memory wait for one another once, not every 32 channels (packed prompts 156 -> 153 us).
+      constexpr int kC = kPair ? kD : kD / 2;
+      const int c0 = kPair ? 0 : kC * t;
+      float o[kC];
+      if (here) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = 0.0f;
+        for (int c = 0; c < kC; c += 32) tmem_ld32(o_addr + c0 + c, o + c);
+        tmem_wait_ld<kC>(o);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kC; ++i) o[i] = 0.0f;
+      }
+      if (!kPair) {
+#pragma unroll
+        for (int i = 0; i < kC; ++i) o[i] *= mine;
+        if (there) {
+          float x[kC];
+#pragma unroll
+          for (int c = 0; c < kC; c += 32) tmem_ld32(kOutCol + 128 * (t ^ 1) + lanes + c0 + c, x + c);
+          tmem_wait_ld<kC>(x);
+#pragma unroll
+          for (int i = 0; i < kC; ++i) o[i] = fmaf(others, x[i], o[i]);
         }
-        if (!kPair) {
+      }
+      if (marked && valid) {  // keys with non-finite values that this row sees
+        for (int e = 0; e < kPartial * kKeys; ++e) {
+          if (partial * kKeys + e >= limit) break;
+          const int key = k_begin + partial * kKeys + e;
+          if (!(late[e >> 5] >> (e & 31) & 1)) continue;
+          const uint16_t* qr = P.q + q_row * P.q_t + head * P.q_h;
+          const uint16_t* kr = P.k + (int64_t(k_row) + key) * P.k_t + kvh * P.k_h;
+          const uint16_t* vr = P.v + (int64_t(k_row) + key) * P.v_t + kvh * P.v_h + c0;
+          float dot = 0.0f;
+          for (int d = 0; d < kD; ++d) dot = fmaf(widen<kBf16>(qr[d]), widen<kBf16>(kr[d]), dot);
+          const float p = exp2_approx(fmaf(dot, P.scale_log2, -base));
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] *= mine;
-          if (there) {
-            float x[32];
-            tmem_ld32(kOutCol + 128 * (t ^ 1) + lanes + c, x);
-            tmem_wait_ld<32>(x);
+          for (int i = 0; i < kC; ++i) o[i] = fmaf(p, widen<kBf16>(vr[i]), o[i]);
+        }
+      }
+      __syncwarp();
+      if (merged) {
+        float4* to = reinterpret_cast<float4*>(P.rec_o) + (rec * 32 + c0 / 4) * kRecordRows + rec_row;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = fmaf(others, x[i], o[i]);
+        for (int i = 0; i < kC / 4; ++i)
+          if (valid) to[i * kRecordRows] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+      } else {
+        // The query tile has been read: its memory carries the rows out, 64 bytes of 32 rows in each 2 KB.
+        uint8_t* buf = smem + (kPair ? t * kTileBytes + (warp & 3) * (kTileBytes / 4) : warp * (kTileBytes / 8));
+#pragma unroll
+        for (int c = 0; c < kC; c += 8)
+          *staged(buf + (c >> 5) * kStageRows, lane, c >> 3 & 3) =
+              make_uint4(pack2<kBf16>(o[c] * inv, o[c + 1] * inv), pack2<kBf16>(o[c + 2] * inv, o[c + 3] * inv),
+                         pack2<kBf16>(o[c + 4] * inv, o[c + 5] * inv), pack2<kBf16>(o[c + 6] * inv, o[c + 7] * inv));
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int from = 8 * i + (lane >> 2);  // four lanes to a row
+          uint8_t* to = reinterpret_cast<uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), from));
+          if (to) {
+#pragma unroll
+            for (int c = 0; c < kC; c += 32)
+              *reinterpret_cast<uint4*>(to + 2 * (c0 + c) + 16 * (lane & 3)) = *staged(buf + (c >> 5) * kStageRows, from, lane & 3);
           }
         }
-        if (marked && valid) {  // keys with non-finite values that this row sees
-          for (int e = 0; e < kPartial * kKeys; ++e) {
-            if (partial * kKeys + e >= limit) break;
-            const int key = k_begin + partial * kKeys + e;
-            if (!(late[e >> 5] >> (e & 31) & 1)) continue;
-            const uint16_t* qr = P.q + q_row * P.q_t + head * P.q_h;
-            const uint16_t* kr = P.k + (int64_t(k_row) + key) * P.k_t + kvh * P.k_h;
-            const uint16_t* vr = P.v + (int64_t(k_row) + key) * P.v_t + kvh * P.v_h;
-            float dot = 0.0f;
-            for (int d = 0; d < kD; ++d) dot = fmaf(widen<kBf16>(qr[d]), widen<kBf16>(kr[d]), dot);
-            const float p = exp2_approx(fmaf(dot, P.scale_log2, -base));
-#pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = fmaf(p, widen<kBf16>(vr[c + i]), o[i]);
-          }
-        }
-        __syncwarp();
-        if (merged) {
-          float4* to = reinterpret_cast<float4*>(P.rec_o) + (rec * 32 + c / 4) * kRecordRows + rec_row;
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (valid) to[i * kRecordRows] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-        } else {
-          uint32_t w[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) w[i] = pack2<kBf16>(o[2 * i] * inv, o[2 * i + 1] * inv);
-          store_rows64(buf, w, dst ? dst + 2 * c : nullptr);
-        }
-        __syncwarp();
       }
       if (merged && valid && (kPair || t == 0)) P.rec_ml[rec * kRecordRows + rec_row] = make_float2(top, sum);
     }
