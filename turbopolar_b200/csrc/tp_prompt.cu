@@ -93,10 +93,10 @@ template <bool kBf16>
 __device__ __forceinline__ float widen(uint16_t u) {
   return kBf16 ? __uint_as_float(uint32_t(u) << 16) : __half2float(__ushort_as_half(u));
 }
+// Bit 15 or 31 is set where that 16-bit number of w has an exponent of all ones: one more carries into it.
 template <bool kBf16>
-__device__ __forceinline__ bool not_finite(uint32_t w) {  // either 16-bit number of w
-  const uint32_t e = kBf16 ? 0x7f807f80u : 0x7c007c00u, x = w & e;
-  return (x & 0xffff0000u) == (e & 0xffff0000u) || (x & 0xffffu) == (e & 0xffffu);
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+  return kBf16 ? (w & 0x7f807f80u) + 0x00800080u : (w & 0x7c007c00u) + 0x04000400u;
 }
 
 // Rows [first, 128) of a value tile: clear those from `valid` (at most 128) on and those with a non-finite value,
@@ -116,11 +116,17 @@ __device__ void clean_values(uint8_t* tile, int first, int valid, int which, uin
       if (row < valid) x[i] = *reinterpret_cast<const uint4*>(at + row * 128);
       else if (row < kKeys) *reinterpret_cast<uint4*>(at + row * 128) = zero;
     }
+    uint32_t bad = 0;  // bit i: x[i] holds a non-finite value
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const bool hit = not_finite<kBf16>(x[i].x) || not_finite<kBf16>(x[i].y) || not_finite<kBf16>(x[i].z) ||
-                       not_finite<kBf16>(x[i].w);
-      const uint32_t hits = __ballot_sync(0xffffffffu, hit) >> (lane & 16) & 0xffffu;  // of this lane's row
+      const uint32_t any = not_finite<kBf16>(x[i].x) | not_finite<kBf16>(x[i].y) | not_finite<kBf16>(x[i].z) |
+                           not_finite<kBf16>(x[i].w);
+      if (any & 0x80008000u) bad |= 1u << i;
+    }
+    if (!__any_sync(0xffffffffu, bad)) continue;
+#pragma unroll 1
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t hits = __ballot_sync(0xffffffffu, bad >> i & 1) >> (lane & 16) & 0xffffu;  // of this lane's row
       if (hits) {
         const int row = r0 + 4 * i + (lane >> 4);
         *reinterpret_cast<uint4*>(at + row * 128) = zero;
