@@ -233,33 +233,33 @@ __device__ __forceinline__ uint4 dense_chunk(const void* p, int64_t at, int f32)
   const float4 b = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + at + 4);
   return make_uint4(pack_h2(a.x, a.y), pack_h2(a.z, a.w), pack_h2(b.x, b.y), pack_h2(b.z, b.w));
 }
-__device__ __forceinline__ bool chunk_not_finite(uint4 x) {
-  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-  bool bad = false;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t e = w[i] & 0x7c007c00u;
-    bad |= (e & 0xffff0000u) == 0x7c000000u || (e & 0xffffu) == 0x7c00u;
-  }
-  return bad;
+__device__ __forceinline__ bool chunk_not_finite(uint4 x) {  // an exponent of all ones: one more carries over
+  auto carry = [](uint32_t w) { return (w & 0x7c007c00u) + 0x04000400u; };
+  return (carry(x.x) | carry(x.y) | carry(x.z) | carry(x.w)) & 0x80008000u;
 }
 
 // Rows [0, valid) of dense keys and values (row strides kt, vt) into the stage, the rest cleared.
 // With `late`, a row with a non-finite value sets its bit there.  All 256 decode threads.
 __device__ __forceinline__ void dense_step(uint32_t stage, const void* k, const void* v, int64_t kt, int64_t vt, int f32,
                                            int valid, uint32_t* late, int tid) {
+  const int c = tid & 15;
+  uint4 x[4], y[4];  // all loads in flight before the first is looked at
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int row = i * 16 + (tid >> 4), c = tid & 15;
-    uint4 x = make_uint4(0, 0, 0, 0), y = x;
+    const int row = i * 16 + (tid >> 4);
+    x[i] = y[i] = make_uint4(0, 0, 0, 0);
     if (row < valid) {
-      x = dense_chunk(k, row * kt + 8 * c, f32);
-      y = dense_chunk(v, row * vt + 8 * c, f32);
-      if (late && chunk_not_finite(y)) atomicOr(late + (row >> 5), 1u << (row & 31));
+      x[i] = dense_chunk(k, row * kt + 8 * c, f32);
+      y[i] = dense_chunk(v, row * vt + 8 * c, f32);
     }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = i * 16 + (tid >> 4);
     const uint32_t at = stage + tile_chunk(row, c, kTreeKeys);
-    st16(at, x.x, x.y, x.z, x.w);
-    st16(at + 2 * kKvHalf, y.x, y.y, y.z, y.w);
+    st16(at, x[i].x, x[i].y, x[i].z, x[i].w);
+    st16(at + 2 * kKvHalf, y[i].x, y[i].y, y[i].z, y[i].w);
+    if (late && chunk_not_finite(y[i])) atomicOr(late + (row >> 5), 1u << (row & 31));
   }
 }
 
