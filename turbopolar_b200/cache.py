@@ -388,7 +388,7 @@ class TurboPolarKVCacheRuntime:
         tree (or a chain) of drafts in one call.  Nothing is appended.
 
         ``q`` is ``(B, H_q, T, 128)``, ``k_draft`` and ``v_draft`` ``(B, H_kv, T, 128)``, all rotated
-        to the drafts' positions, float16 or float32 (rounded to float16); ``T`` is 1 to 256.
+        to the drafts' positions, float16 or float32; ``T`` is 1 to 256.
         ``mask`` is ``(T, T)`` or ``(B, T, T)`` bool: draft ``t`` sees draft ``d`` where
         ``mask[t, d]``, usually its ancestors and itself.  Every draft sees the whole cache.
         A draft that is masked has no influence on a row, whatever it holds.

@@ -23,10 +23,10 @@
 // 1,040; what is left is the latency of scores, weights and products after one another.  Keys in units of 64
 // with two score buffers per tile took 4,500 (products with 64 columns wait for shared memory), two issuing
 // warps and a share of the exponentials as polynomials on the FMA pipe were slower too.
-// Bound, packed requests (12 of 1 to 2,500 tokens, 153 us): an item has 7 key tiles in the mean, and its
-// start and end, 7 to 8 us, stand beside 12 us of tiles.  CTAs that stay and take items in turn,
+// Bound, packed requests (12 of 1 to 2,500 tokens, 146 us): an item has 7 key tiles in the mean, and its
+// start and end, about 7 us, stand beside 12 us of tiles.  CTAs that stay and take items in turn,
 // with the next item's loads and first scores under the last one's end, gained that back for items of one or
-// two key tiles only (9.1 instead of 9.9 us each) and lost a ring stage: 162 us.
+// two key tiles only (9.1 instead of 9.9 us each) and lost a ring stage: 162 us where these took 155.
 // Bound, single tokens: memory (100 MB; the floor is 15.3 us), launch, the first loads and the merge.
 //
 // Values that no row may see: keys past the item's range in its last tile belong to another

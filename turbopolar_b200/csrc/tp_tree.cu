@@ -24,6 +24,10 @@
 // With more than 128 rows the softmax warpgroups have a tile each; with fewer they take
 // alternate steps of the one tile, each with its own running maximum, sum and accumulator, and
 // merge at the segment's end.
+//
+// Float32 queries, tails and drafts are split into two float16 parts (22 bits), so only the weights and the output are
+// rounded to float16; rounded inputs had twice the error of a float32 computation on contexts of few tokens.
+// The queries' second part takes the tensor memory of a second tile, a key's second part a row of its own.
 #include <algorithm>
 #include <cmath>
 #include <string>
@@ -42,7 +46,7 @@ constexpr int kPageCopiers = 4;
 constexpr int kMaxDrafts = 256;
 // Up to so many steps a CTA takes a whole segment: a second kernel costs about what four steps do.
 constexpr int kWholeSteps = 4;
-constexpr int kGroupRows = 2 * kTile;                 // rows that share a decoded page
+constexpr int kGroupRows = 2 * kTile;                 // rows that share a decoded page, at most
 constexpr int kLateRing = 16;                         // segments whose lists may be alive
 constexpr int kTreeThreads = 640;
 // Five warpgroups at 96 registers: 480, of which the softmax threads take 128, decode 88, issue 48.
@@ -66,6 +70,7 @@ struct TreeParams {
   const void *tail_k, *tail_v;
   int tail_f32, q_f32, kv_f32;
   int heads, hkv, hq, group, drafts, rows;  // heads: batch * hkv; rows: drafts * group
+  int group_rows;                           // kGroupRows, or one tile
   int row_groups, n_page_steps, tail_len, n_tail_steps, n_steps, visible;
   int total, grid;                          // segments * n_steps; CTAs
   int merged;                               // merge_pieces_kernel follows
@@ -238,6 +243,23 @@ __device__ __forceinline__ bool chunk_not_finite(uint4 x) {  // an exponent of a
   return (carry(x.x) | carry(x.y) | carry(x.z) | carry(x.w)) & 0x80008000u;
 }
 
+// Eight float32 channels in two float16 parts: what the first part rounds away is the second (nothing where the first
+// is not finite).  Together they hold 22 bits.
+__device__ __forceinline__ void split_chunk(const void* p, int64_t at, uint4& hi, uint4& lo) {
+  const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + at);
+  const float4 b = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + at + 4);
+  auto rest = [](uint32_t h, float x, float y) {
+    const float2 f = __half22float2(u32_as_h2(h));
+    return pack_h2(isfinite(f.x) ? x - f.x : 0.0f, isfinite(f.y) ? y - f.y : 0.0f);
+  };
+  hi = make_uint4(pack_h2(a.x, a.y), pack_h2(a.z, a.w), pack_h2(b.x, b.y), pack_h2(b.z, b.w));
+  lo = make_uint4(rest(hi.x, a.x, a.y), rest(hi.y, a.z, a.w), rest(hi.z, b.x, b.y), rest(hi.w, b.z, b.w));
+}
+
+// Float32 keys and values take two rows of the stage each, r and r + 32 (see split_chunk), so a step holds 32:
+// scores of both rows are added, and the weight is written for both.
+__host__ __device__ __forceinline__ int dense_keys(int f32) { return f32 ? kTreeKeys / 2 : kTreeKeys; }
+
 // Rows [0, valid) of dense keys and values (row strides kt, vt) into the stage, the rest cleared.
 // With `late`, a row with a non-finite value sets its bit there.  All 256 decode threads.
 __device__ __forceinline__ void dense_step(uint32_t stage, const void* k, const void* v, int64_t kt, int64_t vt, int f32,
@@ -245,12 +267,24 @@ __device__ __forceinline__ void dense_step(uint32_t stage, const void* k, const 
   const int c = tid & 15;
   uint4 x[4], y[4];  // all loads in flight before the first is looked at
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = i * 16 + (tid >> 4);
-    x[i] = y[i] = make_uint4(0, 0, 0, 0);
-    if (row < valid) {
-      x[i] = dense_chunk(k, row * kt + 8 * c, f32);
-      y[i] = dense_chunk(v, row * vt + 8 * c, f32);
+  for (int i = 0; i < 4; ++i) x[i] = y[i] = make_uint4(0, 0, 0, 0);
+  if (f32) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int row = i * 16 + (tid >> 4);
+      if (row < valid) {
+        split_chunk(k, row * kt + 8 * c, x[i], x[i + 2]);
+        split_chunk(v, row * vt + 8 * c, y[i], y[i + 2]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = i * 16 + (tid >> 4);
+      if (row < valid) {
+        x[i] = *reinterpret_cast<const uint4*>(static_cast<const __half*>(k) + row * kt + 8 * c);
+        y[i] = *reinterpret_cast<const uint4*>(static_cast<const __half*>(v) + row * vt + 8 * c);
+      }
     }
   }
 #pragma unroll
@@ -268,10 +302,12 @@ __device__ __forceinline__ float load_any(const void* p, int64_t i, int f32) {
 }
 
 // kPair: a tile per softmax warpgroup (more than 128 rows).
-template <int kMode, bool kPair>
+// kF32: the query, the tail or the drafts are float32 (an instance of its own: float16 calls were 4% slower in one).
+template <int kMode, bool kPair, bool kF32>
 __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const __grid_constant__ TreeParams P,
                                                                           const __grid_constant__ TreeAngles<kMode> A) {
   extern __shared__ __align__(1024) uint8_t smem[];
+  const int q_f32 = kF32 ? P.q_f32 : 0, kv_f32 = kF32 ? P.kv_f32 : 0, tail_f32 = kF32 ? P.tail_f32 : 0;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   float2* tab = reinterpret_cast<float2*>(smem + kOffTab);
   uint32_t* late_ring = reinterpret_cast<uint32_t*>(smem + kOffLate);
@@ -342,7 +378,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
       const int b = min(P.n_steps, a + count - done);
       const int head = seg / P.row_groups, rg = seg - head * P.row_groups;
       const int batch = head / P.hkv, kvh = head - batch * P.hkv;
-      const int r = rg * kGroupRows + (kPair ? w * kTile : 0) + r0;
+      const int r = rg * P.group_rows + (kPair ? w * kTile : 0) + r0;
       const bool valid = r < P.rows;
       const int g = valid ? r / P.drafts : 0, t = valid ? r - g * P.drafts : 0;
       const int64_t q_at = batch * P.q_b + (int64_t(kvh) * P.group + g) * P.q_h + t * P.q_t;
@@ -356,7 +392,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
           const bool there = __shfl_sync(0xffffffffu, int(valid), from);
 #pragma unroll
           for (int p = 0; p < 4; ++p)
-            x[i][p] = there ? dense_chunk(P.q, at + 32 * p + 8 * (lane & 3), P.q_f32) : make_uint4(0, 0, 0, 0);
+            x[i][p] = there ? dense_chunk(P.q, at + 32 * p + 8 * (lane & 3), q_f32) : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
@@ -371,6 +407,27 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
           }
           __syncwarp();
           tmem_st16(64 * w + lanes + 16 * p, y);
+        }
+        if (!kPair && q_f32) {  // what the rounding left, in the columns of the second tile's queries
+          for (int p = 0; p < 4; ++p) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int from = 8 * i + (lane >> 2);
+              const int64_t at = __shfl_sync(0xffffffffu, q_at, from);
+              uint4 hi, lo = make_uint4(0, 0, 0, 0);
+              if (__shfl_sync(0xffffffffu, int(valid), from)) split_chunk(P.q, at + 32 * p + 8 * (lane & 3), hi, lo);
+              *staged(buf, from, lane & 3) = lo;
+            }
+            __syncwarp();
+            uint32_t y[16];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint4 v = *staged(buf, lane, i);
+              y[4 * i] = v.x, y[4 * i + 1] = v.y, y[4 * i + 2] = v.z, y[4 * i + 3] = v.w;
+            }
+            __syncwarp();
+            tmem_st16(64 + lanes + 16 * p, y);
+          }
         }
         tmem_wait_st();
       }
@@ -407,14 +464,21 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
         if (ok && live) {
           tmem_fence_after();
           uint64_t sees = ~uint64_t(0);
+          const bool twice = s >= draft0 ? kv_f32 : s >= P.n_page_steps && tail_f32;
           if (s >= draft0) {
-            sees = bits[s - draft0];
+            const int j = s - draft0;
+            sees = twice ? bits[j >> 1] >> (32 * (j & 1)) | ~uint64_t(0) << 32 : bits[j];
           } else {
-            const int n = s < P.n_page_steps ? P.visible - s * kTreeKeys : P.tail_len;
-            if (n < kTreeKeys) sees = (uint64_t(1) << n) - 1;
+            const int n = s < P.n_page_steps ? P.visible - s * kTreeKeys
+                                             : P.tail_len - (s - P.n_page_steps) * dense_keys(tail_f32);
+            if (n < (twice ? 32 : kTreeKeys)) sees = ((uint64_t(1) << n) - 1) | (twice ? ~uint64_t(0) << 32 : 0);
           }
-          ok = softmax_tile<kTreeKeys, false>(row, s_addr, kTreeOutCol + 128 * w + lanes, Bits64{sees}, P.scale_log2, !any,
-                                              [&] { return wait_bar(o_done + w, (units - 1) & 1, stop); });
+          const uint32_t o_addr = kTreeOutCol + 128 * w + lanes;
+          auto before = [&] { return wait_bar(o_done + w, (units - 1) & 1, stop); };
+          if (twice)
+            ok = softmax_tile<kTreeKeys / 2, false, true>(row, s_addr, o_addr, Bits64{sees}, P.scale_log2, !any, before);
+          else
+            ok = softmax_tile<kTreeKeys, false>(row, s_addr, o_addr, Bits64{sees}, P.scale_log2, !any, before);
           tmem_fence_before();
         }
         __syncwarp();
@@ -449,7 +513,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
         const bool whole = a == 0 && b == P.n_steps;
         const float inv = !whole ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
         const int64_t rec = int64_t(blockIdx.x) + seg;
-        const int in_rec = r - rg * kGroupRows;
+        const int in_rec = r - rg * P.group_rows;
         const int64_t out_at = ((int64_t(batch) * P.drafts + t) * P.hq + int64_t(kvh) * P.group + g) * kD;
         uint8_t* dst = valid ? reinterpret_cast<uint8_t*>(P.out + out_at) : nullptr;
         const uint32_t* late = late_ring + (draft_pieces & (kLateRing - 1)) * 8;
@@ -483,10 +547,10 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
                 if (!(late[d >> 5] >> (d & 31) & 1) || !(bits[d >> 6] >> (d & 63) & 1)) continue;
                 const int64_t k_at = batch * P.k_b + kvh * P.k_h + d * P.k_t, v_at = batch * P.v_b + kvh * P.v_h + d * P.v_t;
                 float dot = 0.0f;
-                for (int i = 0; i < kD; ++i) dot = fmaf(load_any(P.q, q_at + i, P.q_f32), load_any(P.k, k_at + i, P.kv_f32), dot);
+                for (int i = 0; i < kD; ++i) dot = fmaf(load_any(P.q, q_at + i, q_f32), load_any(P.k, k_at + i, kv_f32), dot);
                 const float p = exp2_approx(fmaf(dot, P.scale_log2, -base));
 #pragma unroll
-                for (int i = 0; i < 32; ++i) o[i] = fmaf(p, load_any(P.v, v_at + c + i, P.kv_f32), o[i]);
+                for (int i = 0; i < 32; ++i) o[i] = fmaf(p, load_any(P.v, v_at + c + i, kv_f32), o[i]);
               }
             }
           }
@@ -546,26 +610,27 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
         if (lane == 0) mbar_arrive(page_empty + slot);
         if (++slot == kPageRing) slot = 0, slot_ph ^= 1;
       } else if (at < draft0) {
-        const int64_t row0 = int64_t(h) * kPage * kD * (P.tail_f32 ? 4 : 2);
+        const int t0 = (at - P.n_page_steps) * dense_keys(tail_f32);
+        const int64_t row0 = (int64_t(h) * kPage + t0) * kD * (tail_f32 ? 4 : 2);
         dense_step(stage, static_cast<const uint8_t*>(P.tail_k) + row0, static_cast<const uint8_t*>(P.tail_v) + row0, kD, kD,
-                   P.tail_f32, P.tail_len, nullptr, tid);
+                   tail_f32, min(dense_keys(tail_f32), P.tail_len - t0), nullptr, tid);
       } else {
-        const int batch = h / P.hkv, kvh = h - batch * P.hkv, d0 = (at - draft0) * kTreeKeys;
-        const int size = P.kv_f32 ? 4 : 2;
+        const int batch = h / P.hkv, kvh = h - batch * P.hkv, d0 = (at - draft0) * dense_keys(kv_f32);
+        const int size = kv_f32 ? 4 : 2;
         uint32_t* late = late_ring + (draft_pieces & (kLateRing - 1)) * 8;
         if (tid < 8 && (at == draft0 || i == 0)) late_ring[((draft_pieces + kLateRing / 2) & (kLateRing - 1)) * 8 + tid] = 0;
-        const int n = min(kTreeKeys, P.drafts - d0);
+        const int n = min(dense_keys(kv_f32), P.drafts - d0);
         dense_step(stage, static_cast<const uint8_t*>(P.k) + (batch * P.k_b + kvh * P.k_h + d0 * P.k_t) * size,
                    static_cast<const uint8_t*>(P.v) + (batch * P.v_b + kvh * P.v_h + d0 * P.v_t) * size, P.k_t, P.v_t,
-                   P.kv_f32, n, late + (d0 >> 5), tid);
+                   kv_f32, n, late + (d0 >> 5), tid);
         __syncwarp();
         if (lane == 0) mbar_arrive(scanned);
         ok = warp_wait(scanned, scans & 1, stop);
         if (!ok) break;
         ++scans;
         for (int q = 0; q < 4; ++q) {
-          const int row = q * 16 + (tid >> 4);
-          if (late[(d0 >> 5) + (row >> 5)] >> (row & 31) & 1)
+          const int row = q * 16 + (tid >> 4), key = row & (dense_keys(kv_f32) - 1);
+          if (late[(d0 >> 5) + (key >> 5)] >> (key & 31) & 1)
             st16(stage + 2 * kKvHalf + tile_chunk(row, tid & 15, kTreeKeys), 0, 0, 0, 0);
         }
         if (at == P.n_steps - 1) ++draft_pieces;
@@ -599,6 +664,11 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
           for (int ks = 0; ks < kD / 16; ++ks)
             mma_ts(kTreeScoreCol + 64 * t, (kPair ? 64 * t : 0) + ks * 8, k_lo + (((ks >> 2) * kKvHalf + (ks & 3) * 32) >> 4),
                    kScores, ks > 0);
+          if (!kPair && q_f32) {
+#pragma unroll
+            for (int ks = 0; ks < kD / 16; ++ks)
+              mma_ts(kTreeScoreCol + 64 * t, 64 + ks * 8, k_lo + (((ks >> 2) * kKvHalf + (ks & 3) * 32) >> 4), kScores, true);
+          }
           mbar_arrive(s_full + t);  // makes what this warp has acquired from the decode warps visible
           mma_commit(s_full + t);
         }
@@ -670,7 +740,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
 template <bool kFew>
 __global__ void __launch_bounds__(kMergeThreads, kFew ? 2 : 4) merge_pieces_kernel(const __grid_constant__ TreeParams P) {
   const int seg = blockIdx.x, head = seg / P.row_groups, rg = seg - head * P.row_groups;
-  const int i0 = blockIdx.y * 32, rows = min(32, min(kGroupRows, P.rows - rg * kGroupRows) - i0);
+  const int i0 = blockIdx.y * 32, rows = min(32, min(P.group_rows, P.rows - rg * P.group_rows) - i0);
   const int part = kFew ? blockIdx.z * (kMergeThreads / 32) + (threadIdx.x >> 5) : blockIdx.z;  // channels 8 part ..
   const int lane = threadIdx.x & 31;
   // CTAs whose ranges meet the segment's steps.
@@ -684,7 +754,7 @@ __global__ void __launch_bounds__(kMergeThreads, kFew ? 2 : 4) merge_pieces_kern
                            int64_t(32) * P.rec_rows, P.rec_rows, last - first + 1, rows) ||
       lane >= rows)
     return;
-  const int r = rg * kGroupRows + i0 + lane;
+  const int r = rg * P.group_rows + i0 + lane;
   const int batch = head / P.hkv, kvh = head - batch * P.hkv, g = r / P.drafts, t = r - g * P.drafts;
   *reinterpret_cast<uint4*>(P.out + ((int64_t(batch) * P.drafts + t) * P.hq + int64_t(kvh) * P.group + g) * kD + 8 * part) =
       make_uint4(pack_h2(p.acc[0], p.acc[1]), pack_h2(p.acc[2], p.acc[3]), pack_h2(p.acc[4], p.acc[5]),
@@ -711,13 +781,13 @@ static void copy_angles(float2* cs, int bits) {
   std::copy_n(table[bits], 1 << bits, cs);
 }
 
-template <int kMode, bool kPair>
+template <int kMode, bool kPair, bool kF32>
 static int launch_tree(const TreeParams& P, const tp_format& fmt, int segments, cudaStream_t s) {
   static bool allowed[64] = {};  // the attribute belongs to a device's copy of the kernel
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess && (dev >= 64 || !allowed[dev])) {
-    const int st = allow_kernel(reinterpret_cast<const void*>(tree_attention_kernel<kMode, kPair>), kTreeSmem, kTreeThreads,
+    const int st = allow_kernel(reinterpret_cast<const void*>(tree_attention_kernel<kMode, kPair, kF32>), kTreeSmem, kTreeThreads,
                                 2 * kTreeSoftmaxRegs + 2 * kTreeDecodeRegs + kTreeIssueRegs, "tp_tree_attention");
     if (st != TP_OK) return st;
     if (dev < 64) allowed[dev] = true;
@@ -726,7 +796,7 @@ static int launch_tree(const TreeParams& P, const tp_format& fmt, int segments, 
   TreeAngles<kMode> A;
   copy_angles(A.cs, fmt.l1_bits);
   if constexpr (kMode != kTreeDefault) copy_angles(A.cs + 256, fmt.deep_bits);
-  tree_attention_kernel<kMode, kPair><<<P.grid, kTreeThreads, kTreeSmem, s>>>(P, A);
+  tree_attention_kernel<kMode, kPair, kF32><<<P.grid, kTreeThreads, kTreeSmem, s>>>(P, A);
   if (P.merged) {
     const int blocks = (P.rec_rows + 31) / 32;
     const bool few = P.n_steps / (P.total / P.grid) + 2 <= kFewRecords;  // CTAs that can share a segment
@@ -739,14 +809,21 @@ static int launch_tree(const TreeParams& P, const tp_format& fmt, int segments, 
 
 template <int kMode>
 static int launch_tree_rows(const TreeParams& P, const tp_format& fmt, int segments, cudaStream_t s) {
-  return P.rows > kTile ? launch_tree<kMode, true>(P, fmt, segments, s) : launch_tree<kMode, false>(P, fmt, segments, s);
+  const bool pair = P.rows > kTile && P.group_rows > kTile;
+  if (P.q_f32 || P.kv_f32 || (P.tail_f32 && P.tail_len > 0))
+    return pair ? launch_tree<kMode, true, true>(P, fmt, segments, s) : launch_tree<kMode, false, true>(P, fmt, segments, s);
+  return pair ? launch_tree<kMode, true, false>(P, fmt, segments, s) : launch_tree<kMode, false, false>(P, fmt, segments, s);
 }
 
-static int row_groups_of(int64_t rows) { return int((rows + kGroupRows - 1) / kGroupRows); }
+static int row_groups_of(int64_t rows, int group_rows) { return int((rows + group_rows - 1) / group_rows); }
 
 static size_t tree_workspace(int64_t heads, int64_t rows) {
-  const int64_t slots = heads * row_groups_of(rows) + device_sms();
-  return 256 + size_t(slots) * std::min<int64_t>(rows, kGroupRows) * (kD * sizeof(float) + sizeof(float2));
+  size_t need = 0;
+  for (int group : {kTile, kGroupRows}) {  // by the queries' type
+    const int64_t slots = heads * row_groups_of(rows, group) + device_sms();
+    need = std::max(need, size_t(slots) * std::min<int64_t>(rows, group) * (kD * sizeof(float) + sizeof(float2)));
+  }
+  return 256 + need;
 }
 
 static bool rows_ok(const void* p, const int64_t* st, const int* n, int f32) {
@@ -819,12 +896,15 @@ int tp_tree_attention(const tp_page_pool* pool, const tp_tail* tail, tp_state st
   P.group = group;
   P.drafts = D.n_drafts;
   P.rows = int(rows);
-  P.row_groups = row_groups_of(rows);
+  // Float32 queries take two parts of tensor memory, so one tile of rows instead of two shares a page.
+  P.group_rows = P.q_f32 ? kTile : kGroupRows;
+  P.row_groups = row_groups_of(rows, P.group_rows);
   P.visible = int(std::min<int64_t>(state.seq_len, int64_t(state.n_pages) * kPage));
   P.n_page_steps = (P.visible + kPage - 1) / kPage;
   P.tail_len = int(std::max<int64_t>(0, state.seq_len - int64_t(state.n_pages) * kPage));
-  P.n_tail_steps = P.tail_len > 0;
-  P.n_steps = P.n_page_steps + P.n_tail_steps + (D.n_drafts + kTreeKeys - 1) / kTreeKeys;
+  auto steps_of = [](int keys, int f32) { return (keys + kTreeKeys / (f32 ? 2 : 1) - 1) / (kTreeKeys / (f32 ? 2 : 1)); };
+  P.n_tail_steps = steps_of(P.tail_len, P.tail_f32);
+  P.n_steps = P.n_page_steps + P.n_tail_steps + steps_of(D.n_drafts, P.kv_f32);
   const int64_t segments = int64_t(heads) * P.row_groups;
   const int64_t total = segments * P.n_steps;
   if (segments > (1 << 24) || total > (1 << 30))
@@ -842,7 +922,7 @@ int tp_tree_attention(const tp_page_pool* pool, const tp_tail* tail, tp_state st
   P.mask_b = D.mask[0], P.mask_t = D.mask[1];
   P.out = static_cast<__half*>(out);
   P.error = static_cast<int*>(workspace);
-  P.rec_rows = int(std::min<int64_t>(rows, kGroupRows));
+  P.rec_rows = int(std::min<int64_t>(rows, P.group_rows));
   P.rec_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + 256);
   P.rec_ml = reinterpret_cast<float2*>(P.rec_o + (segments + device_sms()) * P.rec_rows * kD);
   cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -280,13 +280,26 @@ struct Bits64 {
 // The weights are made with the reference as it is while the maximum is found on another pipe, and
 // made again in the few tiles that move the reference: the special-function unit, which needs 8 cycles
 // for a warp's exponential (1,024 for 128 columns), does not wait for the maximum.
-template <int kCols, bool kBf16, class Sees, class Wait>
+//
+// kTwice: the scores of column c are the sum of columns c and c + kCols (a key in two parts), and its weight
+// is written to both.
+template <int kCols, bool kBf16, bool kTwice = false, class Sees, class Wait>
 __device__ __forceinline__ bool softmax_tile(SoftmaxRow& row, uint32_t s_addr, uint32_t o_addr, Sees sees,
                                              float scale_log2, bool first, Wait before_rescale) {
   float s[kCols];
 #pragma unroll
   for (int c = 0; c < kCols; c += 32) tmem_ld32(s_addr + c, s + c);
-  tmem_wait_ld<kCols>(s);
+  if constexpr (kTwice) {
+    float rest[kCols];
+#pragma unroll
+    for (int c = 0; c < kCols; c += 32) tmem_ld32(s_addr + kCols + c, rest + c);
+    tmem_wait_ld<kCols>(s);
+    tmem_wait_ld<kCols>(rest);
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) s[c] += rest[c];
+  } else {
+    tmem_wait_ld<kCols>(s);
+  }
   if (!__all_sync(0xffffffffu, sees.template all<kCols>())) {
 #pragma unroll
     for (int c = 0; c < kCols; ++c) s[c] = sees(c) ? s[c] : -INFINITY;
@@ -319,6 +332,7 @@ __device__ __forceinline__ bool softmax_tile(SoftmaxRow& row, uint32_t s_addr, u
         w[i] = pack2<kBf16>(e0, e1);
       }
       tmem_st16(s_addr + c / 2, w);
+      if (kTwice) tmem_st16(s_addr + kCols / 2 + c / 2, w);
     }
     const float m = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * scale_log2;
     const bool moves = m > row.ref + kRefSlack;
