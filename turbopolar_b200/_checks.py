@@ -17,10 +17,14 @@ def refuse_gradients(*tensors) -> None:
                 raise NotImplementedError("TurboPolar kernels have no backward pass; call them under torch.no_grad()")
 
 
+def raw_stream(device: torch.device) -> int:
+    """The handle of ``device``'s current stream."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 def launch(device: torch.device, fn, *args) -> int:
     """``fn(*args, stream)`` on ``device`` and its current stream."""
-    i = device.index
-    stream = torch._C._cuda_getCurrentRawStream(i)
+    i, stream = device.index, raw_stream(device)
     if i == torch.cuda.current_device():
         return fn(*args, stream)
     with torch.cuda.device(device):

@@ -29,7 +29,7 @@ from typing import Any, Dict, Optional, Tuple
 import torch
 
 from . import _lib, guard
-from ._checks import check_out, disjoint, launch, refuse_gradients
+from ._checks import check_out, disjoint, launch, raw_stream, refuse_gradients
 from .codec import encode_pages, _stream
 from .config import TurboPolarConfig
 from .pages import PAGE, PagePool, page_bytes
@@ -61,6 +61,10 @@ class TurboPolarKVCacheRuntime:
         self._device_arg = device
         # Sequence shard: absolute index of local page 0 (tokens before it live on other ranks).
         self.first_page = int(first_page)
+        # Scratch of tree_attention by (device, stream): calls on two streams may run at the same time.  A
+        # captured call keeps its scratch's address, so replaced ones are held as long as the runtime, past reset().
+        self._tree_scratch: Dict[Tuple[Optional[int], int], torch.Tensor] = {}
+        self._tree_replaced: list = []
         self.reset()
 
     # ------------------------------------------------------------------ state
@@ -72,8 +76,7 @@ class TurboPolarKVCacheRuntime:
         self._tail: Optional[_lib.Tail] = None
         self.d_state: Optional[torch.Tensor] = None
         self._workspace: Optional[torch.Tensor] = None
-        self._tree_workspace: Optional[torch.Tensor] = None
-        self._tree_room = 0
+        self._tree_workspace: Optional[torch.Tensor] = None  # scratch of the last tree_attention
         self._tree_layouts: dict = {}  # checked layouts of tree_attention calls, by shapes, strides and types
         self.n_pages = 0
         self.tail_len = 0
@@ -380,7 +383,20 @@ class TurboPolarKVCacheRuntime:
         code = lambda x: _lib.TP_F16 if x.dtype == torch.float16 else _lib.TP_F32
         layout = _lib.Drafts(B, Hq, T, code(q), code(k), strides(q), strides(k), strides(v),
                              (ctypes.c_int64 * 2)(mask.stride(0) if mask.dim() == 3 else 0, mask.stride(-2)))
-        return layout, _lib.lib().tp_tree_attention_workspace_size(self.heads, B * Hq, T)
+        # Sizes in powers of two of the drafts: scratch is replaced (and the old one held) a few times at most.
+        return layout, _lib.lib().tp_tree_attention_workspace_size(self.heads, B * Hq, max(8, 1 << (T - 1).bit_length()))
+
+    def _tree_scratch_for(self, need: int) -> torch.Tensor:
+        key = (self.device.index, raw_stream(self.device))
+        scratch = self._tree_scratch.get(key)
+        if scratch is None or scratch.numel() < need:
+            if scratch is not None:
+                self._tree_replaced.append(scratch)
+            scratch = torch.empty(need, dtype=torch.uint8, device=self.device)
+            scratch[:256].zero_()  # the error word
+            self._tree_scratch[key] = scratch
+        self._tree_workspace = scratch
+        return scratch
 
     def tree_attention(self, q: torch.Tensor, k_draft: torch.Tensor, v_draft: torch.Tensor, mask: torch.Tensor,
                        scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -396,6 +412,10 @@ class TurboPolarKVCacheRuntime:
         Returns float16 ``(B, H_q, T, 128)``, a view of a ``(B, T, H_q, 128)`` buffer (``out`` if
         given), so that ``.transpose(1, 2).reshape(B, T, -1)`` copies nothing.  After verification,
         ``append(k_draft[:, :, path], v_draft[:, :, path])`` stores the accepted path.
+
+        Scratch belongs to the runtime, one piece per stream, and a piece that a larger call replaced is
+        kept, so a CUDA graph that captured a call stays valid while the runtime exists.  Graphs captured
+        on one stream share a piece: they must not be replayed at the same time.
         """
         if not self._initialized or (self.n_pages == 0 and self.tail_len == 0):
             raise RuntimeError("TurboPolar cache returned no blocks after append")
@@ -427,13 +447,11 @@ class TurboPolarKVCacheRuntime:
                 raise ValueError("out must be contiguous and 16-byte aligned")
             if not all(disjoint(out, x) for x in (q, k_draft, v_draft)):
                 raise ValueError("out shares memory with an input")
-        if self._tree_room < need:
-            self._tree_workspace = torch.zeros(need, dtype=torch.uint8, device=self.device)
-            self._tree_room = need
+        scratch = self._tree_scratch_for(need)
         status = launch(self.device, _lib.lib().tp_tree_attention, self.pool_struct(), self.tail_struct(),
                         _lib.State(self.n_pages, self.tail_len, self.actual_seq_len, 0), layout, qp, kp, vp,
                         mask.data_ptr(), self.config.attention_scale if scale is None else scale, out.data_ptr(),
-                        self._tree_workspace.data_ptr(), self._tree_room)
+                        scratch.data_ptr(), scratch.numel())
         if status:
             _lib.check(status)
         return out.transpose(1, 2)
