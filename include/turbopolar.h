@@ -373,6 +373,7 @@ typedef struct tp_drafts {
   int32_t batch, num_q_heads, n_drafts; /* query heads of one sequence; drafts 1..256 */
   int32_t q_dtype, kv_dtype;            /* TP_F16 or TP_F32 (kept to 22 bits) */
   int64_t q[3], k[3], v[3], mask[2];
+  int32_t* d_state; /* the cache's state words on the device, or NULL */
 } tp_drafts;
 
 /* Workspace bytes of tp_tree_attention; num_q_heads over num_kv_heads as the pool counts them (all
@@ -386,7 +387,10 @@ size_t tp_tree_attention_workspace_size(int32_t num_kv_heads, int32_t num_q_head
  * ancestors and itself.  A row that sees nothing gives 0, and a masked draft has no influence,
  * whatever it holds.  Nothing is appended: tp_append takes the accepted drafts.  The reference has
  * no counterpart (its fused call takes one query token, benchmarks/turbopolar_fast_attention.py:
- * 106-131).  The pool's heads are batch x KV heads; state.first_page must be 0.  workspace: not
+ * 106-131).  The pool's heads are batch x KV heads; state.first_page must be 0.
+ * The sizes are `state`'s, also in a captured call.  With drafts->d_state, a call that finds other
+ * counters there (a graph replayed after an append) reads nothing of the cache, gives NaN rows and
+ * sets state word 4 to 4.  workspace: not
  * shared by calls that may overlap; word 0 is set to 1 when a wait ran out (the output is then
  * unusable) and never cleared. */
 int tp_tree_attention(const tp_page_pool* pool, const tp_tail* tail, tp_state state, const tp_drafts* drafts,

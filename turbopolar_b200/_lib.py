@@ -100,7 +100,7 @@ class Drafts(ctypes.Structure):
     """tp_drafts: sizes, types and strides of a tp_tree_attention call."""
     _fields_ = [("batch", ctypes.c_int32), ("num_q_heads", ctypes.c_int32), ("n_drafts", ctypes.c_int32),
                 ("q_dtype", ctypes.c_int32), ("kv_dtype", ctypes.c_int32), ("q", ctypes.c_int64 * 3),
-                ("k", ctypes.c_int64 * 3), ("v", ctypes.c_int64 * 3), ("mask", ctypes.c_int64 * 2)]
+                ("k", ctypes.c_int64 * 3), ("v", ctypes.c_int64 * 3), ("mask", ctypes.c_int64 * 2), ("d_state", ctypes.c_void_p)]
 
 
 _lib = None

@@ -65,11 +65,17 @@ class TurboPolarKVCacheRuntime:
         # captured call keeps its scratch's address, so replaced ones are held as long as the runtime, past reset().
         self._tree_scratch: Dict[Tuple[Optional[int], int], torch.Tensor] = {}
         self._tree_replaced: list = []
+        self._old_states: list = []  # state words of before a reset, read by captured tree_attention calls
+        self.d_state: Optional[torch.Tensor] = None
+        self._tree_layouts: dict = {}
         self.reset()
 
     # ------------------------------------------------------------------ state
     def reset(self):
         """Clear all cache state and persistent invariants (``turbo_polar_cache.py:379-395``)."""
+        if self.d_state is not None and self._tree_layouts:
+            self.d_state[:3] = -1  # no cache: captured calls that are replayed give NaN rows
+            self._old_states.append(self.d_state)
         self.pool: Optional[PagePool] = None
         self.tail_k: Optional[torch.Tensor] = None
         self.tail_v: Optional[torch.Tensor] = None
@@ -382,7 +388,8 @@ class TurboPolarKVCacheRuntime:
         strides = lambda x: (ctypes.c_int64 * 3)(*(s if n > 1 else 0 for s, n in zip(x.stride(), x.shape[:3])))
         code = lambda x: _lib.TP_F16 if x.dtype == torch.float16 else _lib.TP_F32
         layout = _lib.Drafts(B, Hq, T, code(q), code(k), strides(q), strides(k), strides(v),
-                             (ctypes.c_int64 * 2)(mask.stride(0) if mask.dim() == 3 else 0, mask.stride(-2)))
+                             (ctypes.c_int64 * 2)(mask.stride(0) if mask.dim() == 3 else 0, mask.stride(-2)),
+                             self.d_state.data_ptr())
         # Sizes in powers of two of the drafts: scratch is replaced (and the old one held) a few times at most.
         return layout, _lib.lib().tp_tree_attention_workspace_size(self.heads, B * Hq, max(8, 1 << (T - 1).bit_length()))
 
@@ -415,7 +422,9 @@ class TurboPolarKVCacheRuntime:
 
         Scratch belongs to the runtime, one piece per stream, and a piece that a larger call replaced is
         kept, so a CUDA graph that captured a call stays valid while the runtime exists.  Graphs captured
-        on one stream share a piece: they must not be replayed at the same time.
+        on one stream share a piece: they must not be replayed at the same time.  A captured call is valid for
+        the cache as it was: replayed after an append or a reset it gives NaN rows and sets
+        :meth:`read_device_error` to 4.
         """
         if not self._initialized or (self.n_pages == 0 and self.tail_len == 0):
             raise RuntimeError("TurboPolar cache returned no blocks after append")
@@ -619,7 +628,8 @@ class TurboPolarKVCacheRuntime:
         }
 
     def read_device_error(self) -> int:
-        """The append kernel's error word (0 ok, 1 tail overflow, 2 pool full); synchronises."""
+        """The cache's error word: 0 ok; an append found 1 the tail or 2 the pool full; 4 a captured
+        tree_attention was replayed on a cache that had changed.  Synchronises."""
         return int(self.d_state[4].item()) if self.d_state is not None else 0
 
     def compressed_bytes_per_token(self) -> int:
