@@ -390,7 +390,7 @@ size_t tp_tree_attention_workspace_size(int32_t num_kv_heads, int32_t num_q_head
  * 106-131).  The pool's heads are batch x KV heads; state.first_page must be 0.
  * The sizes are `state`'s, also in a captured call.  With drafts->d_state, a call that finds other
  * counters there (a graph replayed after an append) reads nothing of the cache, gives NaN rows and
- * sets state word 4 to 4.  workspace: not
+ * sets state word 4 to 4; a wait that ran out sets it to 3.  workspace: not
  * shared by calls that may overlap; word 0 is set to 1 when a wait ran out (the output is then
  * unusable) and never cleared. */
 int tp_tree_attention(const tp_page_pool* pool, const tp_tail* tail, tp_state state, const tp_drafts* drafts,

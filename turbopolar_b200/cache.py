@@ -628,8 +628,9 @@ class TurboPolarKVCacheRuntime:
         }
 
     def read_device_error(self) -> int:
-        """The cache's error word: 0 ok; an append found 1 the tail or 2 the pool full; 4 a captured
-        tree_attention was replayed on a cache that had changed.  Synchronises."""
+        """The cache's error word: 0 ok; an append found 1 the tail or 2 the pool full; 3 a wait of a
+        tree_attention ran out (its output is unusable); 4 a captured tree_attention was replayed on a
+        cache that had changed.  Kept until :meth:`reset`.  Synchronises."""
         return int(self.d_state[4].item()) if self.d_state is not None else 0
 
     def compressed_bytes_per_token(self) -> int:

@@ -753,7 +753,10 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
     tmem_fence_after();
     tmem_free(tmem, 512);
   }
-  if (threadIdx.x == 0 && *stop) *P.error = 1;
+  if (threadIdx.x == 0 && *stop) {
+    *P.error = 1;
+    if (P.d_state) P.d_state[4] = 3;
+  }
   if (!*current) refuse_rows(P);
 }
 

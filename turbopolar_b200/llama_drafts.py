@@ -10,8 +10,9 @@ with the head norms of models that have them), then
   afterwards.
 
 :class:`DraftDecoder` runs a model that way: :meth:`~DraftDecoder.prefill`,
-:meth:`~DraftDecoder.verify` (logits of every draft), :meth:`~DraftDecoder.accept`, and
-:meth:`~DraftDecoder.generate`, greedy decoding whose tokens are those of one-token steps.
+:meth:`~DraftDecoder.verify` (logits of every draft), :meth:`~DraftDecoder.accept`,
+:meth:`~DraftDecoder.check` (error words of the kernels), and :meth:`~DraftDecoder.generate`, greedy
+decoding whose tokens are those of one-token steps.
 
 ``python -m turbopolar_b200.llama_drafts`` decodes with a random-init model.
 """
@@ -58,10 +59,19 @@ class DraftDecoder:
             cfg.num_hidden_layers, self.hq, self.hkv, head_dim, device=self.device, max_seq_len=max_seq_len,
             check_finite=check_finite)
         self._drafts: List[Tuple[torch.Tensor, torch.Tensor]] = []
+        self._prompt_error = torch.zeros(1, dtype=torch.int32, device=self.device)  # of all prompts so far
 
     @property
     def offset(self) -> int:
         return self.cache[0].offset
+
+    def check(self) -> None:
+        """Raise ``RuntimeError`` where a kernel of a prompt, a verification or an append has reported that its
+        results are unusable.  Synchronises; :meth:`accept` calls it before it appends."""
+        words = torch.cat([self._prompt_error, *(layer.runtime.d_state[4:5] for layer in self.cache
+                                                 if layer.runtime.d_state is not None)]).tolist()
+        if any(words):
+            raise RuntimeError(f"TurboPolar kernels reported errors (prompt attention {words[0]}, layers {words[1:]})")
 
     def _qkv(self, attn, x, cos, sin):
         t = x.shape[1]
@@ -96,7 +106,9 @@ class DraftDecoder:
             return prompt_attention(q, *(y[0].transpose(0, 1) for y in hist), plan, scale=attn.scaling)
 
         positions = torch.arange(start, start + n, device=self.device)
-        return self.model.lm_head(self._layers(tokens, positions, attend)[-1]).float()
+        logits = self.model.lm_head(self._layers(tokens, positions, attend)[-1]).float()
+        self._prompt_error |= plan.device_error
+        return logits
 
     @torch.no_grad()
     def verify(self, tokens: torch.Tensor, parents: Sequence[int]) -> torch.Tensor:
@@ -120,6 +132,7 @@ class DraftDecoder:
         """Append the drafts ``path`` (a root and its descendants) of the last :meth:`verify`."""
         if not self._drafts:
             raise RuntimeError("accept() follows verify()")
+        self.check()
         index = torch.as_tensor(list(path), device=self.device)
         for layer, (k, v) in zip(self.cache, self._drafts):
             layer.runtime.append(k[:, :, index].to(torch.float16), v[:, :, index].to(torch.float16))

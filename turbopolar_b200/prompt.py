@@ -56,9 +56,14 @@ class PromptPlan:
         self._ptrs = (self._words.data_ptr(), self._workspace.data_ptr(), self._workspace.numel())
         self._layouts: dict = {}  # checked row layouts, by strides and types
 
+    @property
+    def device_error(self) -> torch.Tensor:
+        """The error word on the device, an int32 tensor ``(1,)``."""
+        return self._workspace[:4].view(torch.int32)
+
     def read_device_error(self) -> int:
         """0, or 1 when a wait in a kernel of this plan ran out (outputs unusable); synchronises."""
-        return int(self._workspace[:4].view(torch.int32).item())
+        return int(self.device_error.item())
 
     def _layout(self, q, k, v) -> _lib.PromptRows:
         for name, x, tokens, heads in (("q", q, self.struct.q_tokens, self.num_q_heads),
