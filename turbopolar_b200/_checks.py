@@ -39,11 +39,17 @@ def extent(x: torch.Tensor) -> Tuple[int, int]:
 
 def _share_rows(a: torch.Tensor, b: torch.Tensor) -> bool:
     """True when ``a`` and ``b`` ``(..., T, H, 128)`` are slices of the same token rows with no common
-    element: equal strides and, within a row, disjoint runs of heads (a fused projection's q and k)."""
+    element: equal strides and, within a row, disjoint runs of heads (a fused projection's q and k).  Rows
+    are ``row`` elements apart and every leading stride is a multiple of that, so an element's place within
+    its row says which run it belongs to."""
     if a.dim() != b.dim() or a.stride() != b.stride() or a.shape[:-2] != b.shape[:-2]:
         return False
-    row = a.stride(-3)
-    off = (b.data_ptr() - a.data_ptr()) // a.element_size()
+    leading = [s for s, n in zip(a.stride()[:-2], a.shape[:-2]) if n > 1]
+    row = min(leading, default=0)  # none: one row, whose run is the extent
+    size = a.element_size()
+    if not row or size != b.element_size() or (b.data_ptr() - a.data_ptr()) % size or any(s % row for s in leading):
+        return False
+    off = (b.data_ptr() - a.data_ptr()) // size
     run_a, run_b = (a.shape[-2] - 1) * a.stride(-2) + HEAD_DIM, (b.shape[-2] - 1) * b.stride(-2) + HEAD_DIM
     return (run_a <= off and off + run_b <= row) or (run_b <= -off and -off + run_a <= row)
 
