@@ -454,8 +454,11 @@ class TurboPolarKVCacheRuntime:
             check_out(out, (B, T, Hq, 128), torch.float16, self.device, "out")
             if not out.is_contiguous() or out.data_ptr() & 15:
                 raise ValueError("out must be contiguous and 16-byte aligned")
-            if not all(disjoint(out, x) for x in (q, k_draft, v_draft)):
-                raise ValueError("out shares memory with an input")
+            inputs = [q, k_draft, v_draft, mask, self.tail_k, self.tail_v]
+            if self.pool is not None:
+                inputs += [x for x in (self.pool.pages, self.pool.radii_scales) if x is not None]
+            if not all(disjoint(out, x) for x in inputs):
+                raise ValueError("out shares memory with an input or the cache")
         scratch = self._tree_scratch_for(need)
         status = launch(self.device, _lib.lib().tp_tree_attention, self.pool_struct(), self.tail_struct(),
                         _lib.State(self.n_pages, self.tail_len, self.actual_seq_len, 0), layout, qp, kp, vp,

@@ -33,12 +33,12 @@ def _aligned(x: torch.Tensor) -> bool:
         and not x.data_ptr() & (4 * x.element_size() - 1)
 
 
-def _check_rows_out(out, x, other, what: str) -> None:
+def _check_rows_out(out, x, others, what: str) -> None:
     check_out(out, x.shape, x.dtype, x.device, what)
     if not _aligned(out):
         raise ValueError(f"{what} needs contiguous channels and strides that are multiples of 4 elements")
     same = out.data_ptr() == x.data_ptr() and out.stride() == x.stride()
-    if not (same or disjoint(out, x)) or not disjoint(out, other):
+    if not (same or disjoint(out, x)) or not all(disjoint(out, y) for y in others if y is not None):
         raise ValueError(f"{what} overlaps an input; it may only be its own input, whole")
 
 
@@ -154,11 +154,11 @@ def norm_rope(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Te
     if q_out is None:
         q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
-        _check_rows_out(q_out, q, k, "q_out")
+        _check_rows_out(q_out, q, (k, cos, sin, positions, q_weight, k_weight), "q_out")
     if k_out is None:
         k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
     else:
-        _check_rows_out(k_out, k, q, "k_out")
+        _check_rows_out(k_out, k, (q, cos, sin, positions, q_weight, k_weight), "k_out")
     struct = layout[0]
     if given:
         if not disjoint(q_out, k_out):
