@@ -5,16 +5,21 @@ from __future__ import annotations
 from typing import Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 HEAD_DIM = 128
 
 
 def refuse_gradients(*tensors) -> None:
-    """The kernels have no backward pass: say so rather than return outputs without a gradient."""
+    """The kernels have no derivatives: say so rather than return outputs without a gradient or a tangent."""
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise NotImplementedError("TurboPolar kernels have no backward pass; call them under torch.no_grad()")
+    if getattr(forward_ad, "_current_level", 0) >= 0:  # inside dual_level(), also under no_grad()
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError("TurboPolar kernels have no forward-mode derivative; pass the primal tensors")
 
 
 def raw_stream(device: torch.device) -> int:

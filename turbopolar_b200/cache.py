@@ -430,8 +430,7 @@ class TurboPolarKVCacheRuntime:
             raise RuntimeError("TurboPolar cache returned no blocks after append")
         if self.first_page or self.later_tokens:
             raise NotImplementedError("tree_attention works on whole sequences, not on sequence shards")
-        if torch.is_grad_enabled():
-            refuse_gradients(q, k_draft, v_draft)
+        refuse_gradients(q, k_draft, v_draft)
         key = (q.shape, q.stride(), q.dtype, q.device, k_draft.shape, k_draft.stride(), k_draft.dtype, k_draft.device,
                v_draft.shape, v_draft.stride(), v_draft.dtype, v_draft.device, mask.shape, mask.stride(), mask.dtype,
                mask.device)
