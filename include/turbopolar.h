@@ -368,7 +368,7 @@ int tp_prompt_attention(const tp_prompt_plan* plan, const int32_t* words, const 
 
 /* Layout of a tp_tree_attention call: queries (batch, head, draft) at b * q[0] + h * q[1] + t * q[2]
  * elements, drafted keys and values alike, 128 contiguous channels, rows on 16-byte boundaries;
- * mask bytes (0 or 1) at b * mask[0] + row * mask[1] + column. */
+ * mask bytes (0: not seen) at b * mask[0] + row * mask[1] + column. */
 typedef struct tp_drafts {
   int32_t batch, num_q_heads, n_drafts; /* query heads of one sequence; drafts 1..256 */
   int32_t q_dtype, kv_dtype;            /* TP_F16 or TP_F32 (kept to 22 bits) */

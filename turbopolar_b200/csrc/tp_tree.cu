@@ -458,17 +458,20 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
           uint64_t x = 0;
           const int n = min(64, P.drafts - d0);
           if ((uintptr_t(m) & 3) == 0) {
-            // Four bytes of 0 or 1 at a time: the product moves byte i to bit 28 + i.
+            // Four bytes at a time: bit 0 of a byte says whether it is not 0, and the product moves byte i to bit 28 + i.
             uint32_t word[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i)
               word[i] = 4 * i + 3 < n ? *reinterpret_cast<const uint32_t*>(m + d0 + 4 * i) : 0;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) x |= uint64_t((word[i] & 0x01010101u) * 0x10204080u >> 28) << (4 * i);
-            for (int d = n & ~3; d < n; ++d) x |= uint64_t(m[d0 + d] & 1) << d;
+            for (int i = 0; i < 16; ++i) {
+              const uint32_t set = (((word[i] & 0x7f7f7f7fu) + 0x7f7f7f7fu) | word[i]) >> 7 & 0x01010101u;
+              x |= uint64_t(set * 0x10204080u >> 28) << (4 * i);
+            }
+            for (int d = n & ~3; d < n; ++d) x |= uint64_t(m[d0 + d] != 0) << d;
           } else {
 #pragma unroll 16
-            for (int d = 0; d < n; ++d) x |= uint64_t(m[d0 + d] & 1) << d;
+            for (int d = 0; d < n; ++d) x |= uint64_t(m[d0 + d] != 0) << d;
           }
           bits[d0 >> 6] = x;
         }
