@@ -249,11 +249,13 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
-// The running softmax of a row: weights are 2^(s * scale_log2 - ref) with a reference that is at
-// least the row's maximum so far minus 8.  It moves only when a maximum exceeds it by more than 8:
-// weights up to 2^8 lose nothing in 16 bits, and the output accumulator, which lives in tensor
-// memory, is rescaled a few times per row instead of once per tile.
-constexpr float kRefSlack = 8.0f;
+// The running softmax of a row: weights are 2^(s * scale_log2 - ref) with a reference 7 below the maximum that set
+// it.  It moves only when a maximum exceeds that one by more than 8: weights up to 2^15 fit float16, sums and
+// accumulators are float32, and the output accumulator, which lives in tensor memory, is rescaled a few times per row
+// instead of once per tile.  The 7 are for small weights: float16 ends at 2^-24, so weights vanish from the product
+// (not from the sum) under 2^-32 of the largest, where a reference at the maximum lost those under 2^-25: the whole
+// of a flat background of keys behind one strong one.
+constexpr float kRefBelow = 7.0f, kRefSlack = kRefBelow + 8.0f;
 struct SoftmaxRow {
   float ref = -INFINITY;  // nothing seen yet
   float sum = 0.0f;
@@ -308,7 +310,7 @@ __device__ __forceinline__ bool softmax_tile(SoftmaxRow& row, uint32_t s_addr, u
     float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
     for (int c = 0; c < kCols; c += 2) top[c >> 1 & 3] = max3(top[c >> 1 & 3], s[c], s[c + 1]);
-    row.ref = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * scale_log2;
+    row.ref = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * scale_log2 - kRefBelow;
   }
   const uint64_t scale2 = pair_of(scale_log2, scale_log2);
   uint64_t add[2];
@@ -337,7 +339,7 @@ __device__ __forceinline__ bool softmax_tile(SoftmaxRow& row, uint32_t s_addr, u
     const float m = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * scale_log2;
     const bool moves = m > row.ref + kRefSlack;
     if (!__any_sync(0xffffffffu, moves)) break;
-    const float to = moves ? m : row.ref;
+    const float to = moves ? m - kRefBelow : row.ref;
     const float f = moves ? exp2_approx(row.ref - to) : 1.0f;
     row.ref = to;
     row.sum *= f;
