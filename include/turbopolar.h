@@ -371,7 +371,7 @@ int tp_prompt_attention(const tp_prompt_plan* plan, const int32_t* words, const 
  * mask bytes (0: not seen) at b * mask[0] + row * mask[1] + column. */
 typedef struct tp_drafts {
   int32_t batch, num_q_heads, n_drafts; /* query heads of one sequence; drafts 1..256 */
-  int32_t q_dtype, kv_dtype;            /* TP_F16 or TP_F32 (kept to 22 bits) */
+  int32_t q_dtype, kv_dtype;            /* TP_F16 or TP_F32 (of any size; two float16 parts) */
   int64_t q[3], k[3], v[3], mask[2];
   int32_t* d_state; /* the cache's state words on the device, or NULL */
 } tp_drafts;

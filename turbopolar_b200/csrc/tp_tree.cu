@@ -27,7 +27,11 @@
 //
 // Float32 queries, tails and drafts are split into two float16 parts (22 bits), so only the weights and the output are
 // rounded to float16; rounded inputs had twice the error of a float32 computation on contexts of few tokens.
-// The queries' second part takes the tensor memory of a second tile, a key's second part a row of its own.
+// The queries' second part takes the tensor memory of a second tile, a key's second part a row of its own.  A row of
+// queries or keys is first brought into float16's range by a power of two of its own, taken out again of its scores
+// (of a query row what lies under 2^-39 of its largest is lost); scores of keys beyond 2^16 are made in float32.
+// Values keep their size (under 1/4 their two parts are exact to 2^-25, as fine as the output's own last bit); rows with
+// values beyond float16 stay out of the product and are added in float32 at the end, as rows of infinities are.
 #include <algorithm>
 #include <cmath>
 #include <string>
@@ -48,6 +52,7 @@ constexpr int kMaxDrafts = 256;
 constexpr int kWholeSteps = 4;
 constexpr int kGroupRows = 2 * kTile;                 // rows that share a decoded page, at most
 constexpr int kLateRing = 16;                         // segments whose lists may be alive
+constexpr int kLateWords = 10;                        // a bit per draft, then per row of the tail
 constexpr int kTreeThreads = 640;
 // Five warpgroups at 96 registers: 480, of which the softmax threads take 128, decode 88, issue 48.
 constexpr int kTreeSoftmaxRegs = 128, kTreeDecodeRegs = 88, kTreeIssueRegs = 48;
@@ -56,8 +61,9 @@ constexpr int kOffBits = kOffPages + kPageRing * kPageSlot;  // [2][128][4] uint
 constexpr int kOffTab = kOffBits + 2 * 128 * 4 * 8;   // float2[512]
 constexpr int kOffMl = kOffTab + 512 * 8;             // [2 pieces][2 warpgroups][128] float2
 constexpr int kOffBuf = kOffMl + 2 * 2 * 128 * 8;     // 2 KB per softmax warp: rows on their way in and out
-constexpr int kOffLate = kOffBuf + 8 * kStageRows;    // [kLateRing][8] words
-constexpr int kOffTreeBars = kOffLate + kLateRing * 32;
+constexpr int kOffLate = kOffBuf + 8 * kStageRows;    // [kLateRing][kLateWords]
+constexpr int kOffFactors = kOffLate + kLateRing * kLateWords * 4;  // [kTreeStages][32] float: of float32 keys
+constexpr int kOffTreeBars = kOffFactors + kTreeStages * 32 * 4;
 constexpr int kTreeSmem = kOffTreeBars + 256;
 
 // Tensor memory (a CTA holds all of it): queries of tile t at 64 t, accumulator and scores t at
@@ -250,22 +256,41 @@ __device__ __forceinline__ void decode_step(const uint8_t* pg, const PoolArgs& L
   }
 }
 
-__device__ __forceinline__ uint4 dense_chunk(const void* p, int64_t at, int f32) {  // 8 channels as float16
-  if (!f32) return *reinterpret_cast<const uint4*>(static_cast<const __half*>(p) + at);
-  const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + at);
-  const float4 b = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + at + 4);
-  return make_uint4(pack_h2(a.x, a.y), pack_h2(a.z, a.w), pack_h2(b.x, b.y), pack_h2(b.z, b.w));
-}
 __device__ __forceinline__ bool chunk_not_finite(uint4 x) {  // an exponent of all ones: one more carries over
   auto carry = [](uint32_t w) { return (w & 0x7c007c00u) + 0x04000400u; };
   return (carry(x.x) | carry(x.y) | carry(x.z) | carry(x.w)) & 0x80008000u;
 }
 
-// Eight float32 channels in two float16 parts: what the first part rounds away is the second (nothing where the first
-// is not finite).  Together they hold 22 bits.
-__device__ __forceinline__ void split_chunk(const void* p, int64_t at, uint4& hi, uint4& lo) {
-  const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + at);
-  const float4 b = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + at + 4);
+// Eight float32 channels of a row.
+struct Chunk32 {
+  float4 a, b;
+  __device__ __forceinline__ Chunk32() : a(make_float4(0.f, 0.f, 0.f, 0.f)), b(a) {}
+  __device__ __forceinline__ Chunk32(const void* p, int64_t at)
+      : a(*reinterpret_cast<const float4*>(static_cast<const float*>(p) + at)),
+        b(*reinterpret_cast<const float4*>(static_cast<const float*>(p) + at + 4)) {}
+  __device__ __forceinline__ void scale(float f) {
+    a.x *= f, a.y *= f, a.z *= f, a.w *= f, b.x *= f, b.y *= f, b.z *= f, b.w *= f;
+  }
+  __device__ __forceinline__ uint32_t top() const {  // bits of the largest finite magnitude, which order as numbers do
+    auto finite = [](float x) {
+      const uint32_t u = __float_as_uint(x) & 0x7fffffffu;
+      return u < 0x7f800000u ? u : 0u;
+    };
+    return max(max(max(finite(a.x), finite(a.y)), max(finite(a.z), finite(a.w))),
+               max(max(finite(b.x), finite(b.y)), max(finite(b.z), finite(b.w))));
+  }
+};
+// The power of two that brings a row whose largest magnitude has the bits `top` to [2^14, 2^15), at most 2^24: a row
+// of at least 2^-27 keeps 22 bits, a smaller one 2^-49.  And its inverse.
+__device__ __forceinline__ float row_factor(uint32_t top) {
+  return top ? __uint_as_float(uint32_t(127 + min(24, 14 + 127 - int(top >> 23))) << 23) : 1.0f;
+}
+constexpr uint32_t kBeyondHalf = 0x47800000u;  // 2^16
+__device__ __forceinline__ float inverse_factor(float f) { return __uint_as_float((254u << 23) - __float_as_uint(f)); }
+
+// Two float16 parts: what the first rounds away is the second (nothing where the first is not finite).
+__device__ __forceinline__ void split_chunk(const Chunk32& x, uint4& hi, uint4& lo) {
+  const float4 &a = x.a, &b = x.b;
   auto rest = [](uint32_t h, float x, float y) {
     const float2 f = __half22float2(u32_as_h2(h));
     return pack_h2(isfinite(f.x) ? x - f.x : 0.0f, isfinite(f.y) ? y - f.y : 0.0f);
@@ -279,20 +304,43 @@ __device__ __forceinline__ void split_chunk(const void* p, int64_t at, uint4& hi
 __host__ __device__ __forceinline__ int dense_keys(int f32) { return f32 ? kTreeKeys / 2 : kTreeKeys; }
 
 // Rows [0, valid) of dense keys and values (row strides kt, vt) into the stage, the rest cleared.
-// With `late`, a row with a non-finite value sets its bit there.  All 256 decode threads.
+// With `late`, a row with a value that is not finite as float16 sets its bit there; of float32 it is cleared, too.
+// `factors`: where the scores' factors of float32 keys go, 0 for a key beyond float16.  All 256 decode threads.
 __device__ __forceinline__ void dense_step(uint32_t stage, const void* k, const void* v, int64_t kt, int64_t vt, int f32,
-                                           int valid, uint32_t* late, int tid) {
+                                           int valid, uint32_t* late, float* factors, int tid) {
   const int c = tid & 15;
   uint4 x[4], y[4];  // all loads in flight before the first is looked at
 #pragma unroll
   for (int i = 0; i < 4; ++i) x[i] = y[i] = make_uint4(0, 0, 0, 0);
   if (f32) {
+    Chunk32 key[2], value[2];
+    uint32_t top[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int row = i * 16 + (tid >> 4);
-      if (row < valid) {
-        split_chunk(k, row * kt + 8 * c, x[i], x[i + 2]);
-        split_chunk(v, row * vt + 8 * c, y[i], y[i + 2]);
+      if (row < valid) key[i] = Chunk32(k, row * kt + 8 * c), value[i] = Chunk32(v, row * vt + 8 * c);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) top[i] = key[i].top();
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) {  // 16 lanes to a row
+#pragma unroll
+      for (int i = 0; i < 2; ++i) top[i] = max(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int row = i * 16 + (tid >> 4);
+      const bool beyond = top[i] >= kBeyondHalf;
+      if (beyond) key[i] = Chunk32();
+      const float f = row_factor(top[i]);
+      key[i].scale(f);
+      split_chunk(key[i], x[i], x[i + 2]);
+      split_chunk(value[i], y[i], y[i + 2]);
+      const uint32_t listed = __ballot_sync(0xffffffffu, chunk_not_finite(y[i])) >> (tid & 16) & 0xffffu;
+      if (listed) y[i] = y[i + 2] = make_uint4(0, 0, 0, 0);
+      if (c == 0) {
+        factors[row] = beyond ? 0.0f : inverse_factor(f);
+        if (listed) atomicOr(late, 1u << row);
       }
     }
   } else {
@@ -311,12 +359,12 @@ __device__ __forceinline__ void dense_step(uint32_t stage, const void* k, const 
     const uint32_t at = stage + tile_chunk(row, c, kTreeKeys);
     st16(at, x[i].x, x[i].y, x[i].z, x[i].w);
     st16(at + 2 * kKvHalf, y[i].x, y[i].y, y[i].z, y[i].w);
-    if (late && chunk_not_finite(y[i])) atomicOr(late + (row >> 5), 1u << (row & 31));
+    if (!f32 && late && chunk_not_finite(y[i])) atomicOr(late + (row >> 5), 1u << (row & 31));
   }
 }
 
 __device__ __forceinline__ float load_any(const void* p, int64_t i, int f32) {
-  return f32 ? __half2float(__float2half_rn(static_cast<const float*>(p)[i])) : __half2float(static_cast<const __half*>(p)[i]);
+  return f32 ? static_cast<const float*>(p)[i] : __half2float(static_cast<const __half*>(p)[i]);
 }
 
 // kPair: a tile per softmax warpgroup (more than 128 rows).
@@ -350,7 +398,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
       tab[i] = cs;
     }
   }
-  for (int i = threadIdx.x; i < kLateRing * 8; i += kTreeThreads) late_ring[i] = 0;
+  for (int i = threadIdx.x; i < kLateRing * kLateWords; i += kTreeThreads) late_ring[i] = 0;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kTreeStages; ++i) {
       mbar_init(kv_full + i, 8);
@@ -403,7 +451,55 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
       const bool valid = r < P.rows;
       const int g = valid ? r / P.drafts : 0, t = valid ? r - g * P.drafts : 0;
       const int64_t q_at = batch * P.q_b + (int64_t(kvh) * P.group + g) * P.q_h + t * P.q_t;
-      if (kPair || w == 0) {
+      float q_factor = 1.0f, row_scale = P.scale_log2;
+      if (!kPair && q_f32) {
+        // Four lanes to a row here too.  Both warpgroups need the rows' factors, the first writes the queries: its
+        // second parts to the columns of the second tile's.
+        float f[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int from = 8 * i + (lane >> 2);
+          const int64_t at = __shfl_sync(0xffffffffu, q_at, from);
+          const bool there = __shfl_sync(0xffffffffu, int(valid), from);
+          uint32_t top = 0;
+#pragma unroll
+          for (int p = 0; p < 4; ++p)
+            if (there) top = max(top, Chunk32(P.q, at + 32 * p + 8 * (lane & 3)).top());
+          top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          f[i] = row_factor(max(top, __shfl_xor_sync(0xffffffffu, top, 2)));
+          const float own = __shfl_sync(0xffffffffu, f[i], 4 * (lane & 7));
+          if (lane >> 3 == i) q_factor = own;
+        }
+        row_scale *= inverse_factor(q_factor);
+#pragma unroll 1
+        for (int p = 0; w == 0 && p < 4; ++p) {
+          uint4 parts[2][4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int from = 8 * i + (lane >> 2);
+            const int64_t at = __shfl_sync(0xffffffffu, q_at, from);
+            Chunk32 x;
+            if (__shfl_sync(0xffffffffu, int(valid), from)) x = Chunk32(P.q, at + 32 * p + 8 * (lane & 3));
+            x.scale(f[i]);
+            split_chunk(x, parts[0][i], parts[1][i]);
+          }
+#pragma unroll
+          for (int part = 0; part < 2; ++part) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) *staged(buf, 8 * i + (lane >> 2), lane & 3) = parts[part][i];
+            __syncwarp();
+            uint32_t y[16];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint4 v = *staged(buf, lane, i);
+              y[4 * i] = v.x, y[4 * i + 1] = v.y, y[4 * i + 2] = v.z, y[4 * i + 3] = v.w;
+            }
+            __syncwarp();
+            tmem_st16(64 * part + lanes + 16 * p, y);
+          }
+        }
+        tmem_wait_st();
+      } else if (kPair || w == 0) {
         // Four lanes to a row, all loads in flight, then 64 bytes of every row at a time through `buf`.
         uint4 x[4][4];
 #pragma unroll
@@ -413,7 +509,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
           const bool there = __shfl_sync(0xffffffffu, int(valid), from);
 #pragma unroll
           for (int p = 0; p < 4; ++p)
-            x[i][p] = there ? dense_chunk(P.q, at + 32 * p + 8 * (lane & 3), q_f32) : make_uint4(0, 0, 0, 0);
+            x[i][p] = there ? *reinterpret_cast<const uint4*>(static_cast<const __half*>(P.q) + at + 32 * p + 8 * (lane & 3))
+                            : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
@@ -428,27 +525,6 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
           }
           __syncwarp();
           tmem_st16(64 * w + lanes + 16 * p, y);
-        }
-        if (!kPair && q_f32) {  // what the rounding left, in the columns of the second tile's queries
-          for (int p = 0; p < 4; ++p) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int from = 8 * i + (lane >> 2);
-              const int64_t at = __shfl_sync(0xffffffffu, q_at, from);
-              uint4 hi, lo = make_uint4(0, 0, 0, 0);
-              if (__shfl_sync(0xffffffffu, int(valid), from)) split_chunk(P.q, at + 32 * p + 8 * (lane & 3), hi, lo);
-              *staged(buf, from, lane & 3) = lo;
-            }
-            __syncwarp();
-            uint32_t y[16];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint4 v = *staged(buf, lane, i);
-              y[4 * i] = v.x, y[4 * i + 1] = v.y, y[4 * i + 2] = v.z, y[4 * i + 3] = v.w;
-            }
-            __syncwarp();
-            tmem_st16(64 + lanes + 16 * p, y);
-          }
         }
         tmem_wait_st();
       }
@@ -500,9 +576,18 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
           const uint32_t o_addr = kTreeOutCol + 128 * w + lanes;
           auto before = [&] { return wait_bar(o_done + w, (units - 1) & 1, stop); };
           if (twice)
-            ok = softmax_tile<kTreeKeys / 2, false, true>(row, s_addr, o_addr, Bits64{sees}, P.scale_log2, !any, before);
+            ok = softmax_tile<kTreeKeys / 2, false, true>(
+                row, s_addr, o_addr, Bits64{sees}, row_scale, !any, before,
+                reinterpret_cast<const float*>(smem + kOffFactors) + 32 * ((done + s - a) & (kTreeStages - 1)), [&](int c) {
+                  const bool draft = s >= draft0;
+                  const float* k = draft ? static_cast<const float*>(P.k) + batch * P.k_b + kvh * P.k_h + (32 * (s - draft0) + c) * P.k_t
+                                         : static_cast<const float*>(P.tail_k) + (int64_t(head) * kPage + 32 * (s - P.n_page_steps) + c) * kD;
+                  float dot = 0.0f;
+                  for (int i = 0; i < kD; ++i) dot = fmaf(load_any(P.q, q_at + i, q_f32), k[i], dot);
+                  return dot * q_factor;
+                });
           else
-            ok = softmax_tile<kTreeKeys, false>(row, s_addr, o_addr, Bits64{sees}, P.scale_log2, !any, before);
+            ok = softmax_tile<kTreeKeys, false>(row, s_addr, o_addr, Bits64{sees}, row_scale, !any, before);
           tmem_fence_before();
         }
         __syncwarp();
@@ -540,10 +625,11 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
         const int in_rec = r - rg * P.group_rows;
         const int64_t out_at = ((int64_t(batch) * P.drafts + t) * P.hq + int64_t(kvh) * P.group + g) * kD;
         uint8_t* dst = valid ? reinterpret_cast<uint8_t*>(P.out + out_at) : nullptr;
-        const uint32_t* late = late_ring + (draft_pieces & (kLateRing - 1)) * 8;
+        const uint32_t* late = late_ring + (draft_pieces & (kLateRing - 1)) * kLateWords;
         bool listed = false;
         if (b > draft0)
           for (int i = 0; i < (P.drafts + 31) >> 5; ++i) listed |= late[i] != 0;
+        const bool tail_listed = tail_f32 && b > P.n_page_steps && (late[8] | late[9]);
         const int c_begin = kPair ? 0 : 64 * w, c_end = kPair ? kD : 64 * w + 64;
         const uint32_t o0 = kTreeOutCol + (kPair ? 128 * w : 0) + lanes, o1 = kTreeOutCol + 128 + lanes;
 #pragma unroll 1
@@ -577,6 +663,18 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
                 for (int i = 0; i < 32; ++i) o[i] = fmaf(p, load_any(P.v, v_at + c + i, kv_f32), o[i]);
               }
             }
+            if (tail_listed) {  // and rows of the tail, which every row sees
+              for (int d = 0; d < P.tail_len; ++d) {
+                if (!(late[8 + (d >> 5)] >> (d & 31) & 1)) continue;
+                const int64_t at = (int64_t(head) * kPage + d) * kD;
+                const float *k = static_cast<const float*>(P.tail_k) + at, *v = static_cast<const float*>(P.tail_v) + at + c;
+                float dot = 0.0f;
+                for (int i = 0; i < kD; ++i) dot = fmaf(load_any(P.q, q_at + i, q_f32), k[i], dot);
+                const float p = exp2_approx(fmaf(dot, P.scale_log2, -base));
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = fmaf(p, v[i], o[i]);
+              }
+            }
           }
           __syncwarp();
           if (whole) {
@@ -596,7 +694,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
           P.rec_ml[rec * P.rec_rows + in_rec] = make_float2(kPair ? row.ref : top, sum);
       }
       tmem_fence_before();
-      if (b > draft0) ++draft_pieces;
+      ++draft_pieces;
       done += b - a;
     }
   } else if (warp < 16) {
@@ -624,6 +722,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
         if (i + 1 < count && s < P.n_page_steps) rscale_next = radius_scale(head, s);
       }
       const uint32_t stage = stages + st * kTreeStage;
+      float* factors = reinterpret_cast<float*>(smem + kOffFactors) + 32 * st;
       ok = i < kTreeStages || warp_wait(kv_empty + st, ph, stop);
       if (!ok) break;
       if (at < P.n_page_steps) {
@@ -637,16 +736,18 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
         const int t0 = (at - P.n_page_steps) * dense_keys(tail_f32);
         const int64_t row0 = (int64_t(h) * kPage + t0) * kD * (tail_f32 ? 4 : 2);
         dense_step(stage, static_cast<const uint8_t*>(P.tail_k) + row0, static_cast<const uint8_t*>(P.tail_v) + row0, kD, kD,
-                   tail_f32, min(dense_keys(tail_f32), P.tail_len - t0), nullptr, tid);
+                   tail_f32, min(dense_keys(tail_f32), P.tail_len - t0),
+                   tail_f32 ? late_ring + (draft_pieces & (kLateRing - 1)) * kLateWords + 8 + (t0 >> 5) : nullptr, factors, tid);
       } else {
         const int batch = h / P.hkv, kvh = h - batch * P.hkv, d0 = (at - draft0) * dense_keys(kv_f32);
         const int size = kv_f32 ? 4 : 2;
-        uint32_t* late = late_ring + (draft_pieces & (kLateRing - 1)) * 8;
-        if (tid < 8 && (at == draft0 || i == 0)) late_ring[((draft_pieces + kLateRing / 2) & (kLateRing - 1)) * 8 + tid] = 0;
+        uint32_t* late = late_ring + (draft_pieces & (kLateRing - 1)) * kLateWords;
+        if (tid < kLateWords && (at == draft0 || i == 0))
+          late_ring[((draft_pieces + kLateRing / 2) & (kLateRing - 1)) * kLateWords + tid] = 0;
         const int n = min(dense_keys(kv_f32), P.drafts - d0);
         dense_step(stage, static_cast<const uint8_t*>(P.k) + (batch * P.k_b + kvh * P.k_h + d0 * P.k_t) * size,
                    static_cast<const uint8_t*>(P.v) + (batch * P.v_b + kvh * P.v_h + d0 * P.v_t) * size, P.k_t, P.v_t,
-                   kv_f32, n, late + (d0 >> 5), tid);
+                   kv_f32, n, late + (d0 >> 5), factors, tid);
         __syncwarp();
         if (lane == 0) mbar_arrive(scanned);
         ok = warp_wait(scanned, scans & 1, stop);

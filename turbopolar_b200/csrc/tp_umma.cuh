@@ -283,11 +283,15 @@ struct Bits64 {
 // made again in the few tiles that move the reference: the special-function unit, which needs 8 cycles
 // for a warp's exponential (1,024 for 128 columns), does not wait for the maximum.
 //
-// kTwice: the scores of column c are the sum of columns c and c + kCols (a key in two parts), and its weight
-// is written to both.
-template <int kCols, bool kBf16, bool kTwice = false, class Sees, class Wait>
+// kTwice: the scores of column c are the sum of columns c and c + kCols (a key in two parts) times `factors[c]` in
+// shared memory, and its weight is written to both.  Where the factor is 0 the score is exact(c) instead.
+struct NoExact {
+  __device__ __forceinline__ float operator()(int) const { return 0.0f; }
+};
+template <int kCols, bool kBf16, bool kTwice = false, class Sees, class Wait, class Exact = NoExact>
 __device__ __forceinline__ bool softmax_tile(SoftmaxRow& row, uint32_t s_addr, uint32_t o_addr, Sees sees,
-                                             float scale_log2, bool first, Wait before_rescale) {
+                                             float scale_log2, bool first, Wait before_rescale,
+                                             const float* factors = nullptr, Exact exact = Exact()) {
   float s[kCols];
 #pragma unroll
   for (int c = 0; c < kCols; c += 32) tmem_ld32(s_addr + c, s + c);
@@ -297,8 +301,23 @@ __device__ __forceinline__ bool softmax_tile(SoftmaxRow& row, uint32_t s_addr, u
     for (int c = 0; c < kCols; c += 32) tmem_ld32(s_addr + kCols + c, rest + c);
     tmem_wait_ld<kCols>(s);
     tmem_wait_ld<kCols>(rest);
+    float least = 1.0f;
 #pragma unroll
-    for (int c = 0; c < kCols; ++c) s[c] += rest[c];
+    for (int c = 0; c < kCols; c += 4) {
+      const float4 f = *reinterpret_cast<const float4*>(factors + c);
+      s[c] = (s[c] + rest[c]) * f.x, s[c + 1] = (s[c + 1] + rest[c + 1]) * f.y;
+      s[c + 2] = (s[c + 2] + rest[c + 2]) * f.z, s[c + 3] = (s[c + 3] + rest[c + 3]) * f.w;
+      least = fminf(fminf(fminf(least, f.x), fminf(f.y, f.z)), f.w);
+    }
+    if (least == 0.0f) {  // the same for all threads
+#pragma unroll 1
+      for (int i = 0; i < kCols; ++i) {
+        if (factors[i] != 0.0f) continue;
+        const float x = exact(i);
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) s[c] = c == i ? x : s[c];
+      }
+    }
   } else {
     tmem_wait_ld<kCols>(s);
   }
