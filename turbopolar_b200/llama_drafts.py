@@ -58,7 +58,10 @@ class DraftDecoder:
         self.cache = cache if cache is not None else make_turbo_caches(
             cfg.num_hidden_layers, self.hq, self.hkv, head_dim, device=self.device, max_seq_len=max_seq_len,
             check_finite=check_finite)
+        # Of the last verify(): per layer the drafts' keys and values; their parents; the offset they follow.
         self._drafts: List[Tuple[torch.Tensor, torch.Tensor]] = []
+        self._parents: List[int] = []
+        self._verified_at = 0
         self._prompt_error = torch.zeros(1, dtype=torch.int32, device=self.device)  # of all prompts so far
 
     @property
@@ -97,6 +100,7 @@ class DraftDecoder:
     @torch.no_grad()
     def prefill(self, tokens: torch.Tensor) -> torch.Tensor:
         """Append a prompt or a further chunk of it ``(T,)``; float32 logits of its last token."""
+        self._drafts = []  # drafts of an earlier verify() are rotated for another offset
         start, n = self.offset, len(tokens)
         plan = PromptPlan([n], [start + n], num_q_heads=self.hq, num_kv_heads=self.hkv, device=self.device)
 
@@ -117,23 +121,35 @@ class DraftDecoder:
             raise ValueError(f"{len(tokens)} drafts and {len(parents)} parents")
         mask = tree_mask(parents, self.device)
         depth = mask.sum(1) - 1
-        self._drafts = []
+        self._drafts, drafts = [], []
 
         def attend(i, attn, q, k, v):
             heads_first = lambda y: y.transpose(0, 1)[None]
             k, v = heads_first(k), heads_first(v)
-            self._drafts.append((k, v))
+            drafts.append((k, v))
             return self.cache[i].tree_attention(heads_first(q), k, v, mask, attn.scaling).transpose(1, 2)
 
-        return self.model.lm_head(self._layers(tokens, self.offset + depth, attend)).float()
+        logits = self.model.lm_head(self._layers(tokens, self.offset + depth, attend)).float()
+        self._drafts, self._parents, self._verified_at = drafts, list(parents), self.offset
+        return logits
 
     @torch.no_grad()
     def accept(self, path: Sequence[int]) -> None:
-        """Append the drafts ``path`` (a root and its descendants) of the last :meth:`verify`."""
+        """Append the drafts ``path`` of the last :meth:`verify`: a root, one of its children, and so on.  An
+        empty path accepts none."""
         if not self._drafts:
             raise RuntimeError("accept() follows verify()")
+        path = [int(i) for i in path]
+        for parent, i in zip([-1, *path], path):
+            if not 0 <= i < len(self._parents) or self._parents[i] != parent:
+                raise ValueError(f"path {path} is not a root of the verified drafts with its descendants")
+        if any(layer.offset != self._verified_at for layer in self.cache):
+            raise RuntimeError("the caches have changed since verify()")
+        if not path:
+            self._drafts = []
+            return
         self.check()
-        index = torch.as_tensor(list(path), device=self.device)
+        index = torch.tensor(path, device=self.device)
         for layer, (k, v) in zip(self.cache, self._drafts):
             layer.runtime.append(k[:, :, index].to(torch.float16), v[:, :, index].to(torch.float16))
         self._drafts = []
