@@ -44,19 +44,38 @@ def tree_mask(parents: Sequence[int], device=None) -> torch.Tensor:
     return mask.to(device)
 
 
+def _check_model(model) -> None:
+    """Refuse models whose attention is not causal attention over the whole history with heads of 128 channels,
+    in a type that ``prompt_attention`` takes."""
+    cfg = model.config
+    head_dim = getattr(cfg, "head_dim", None) or cfg.hidden_size // cfg.num_attention_heads
+    if head_dim != 128:
+        raise NotImplementedError("TurboPolar only supports head_dim == 128")
+    layers = [layer.self_attn for layer in model.model.layers]
+    windows = [getattr(cfg, "sliding_window", None) if getattr(cfg, "use_sliding_window", True) else None]
+    windows += [getattr(a, "sliding_window", None) for a in layers]
+    kinds = set(getattr(cfg, "layer_types", None) or ["full_attention"])
+    if any(w is not None for w in windows) or kinds != {"full_attention"}:
+        raise NotImplementedError("DraftDecoder attends the whole history; this model has layers of other attention")
+    if getattr(cfg, "attn_logit_softcapping", None) is not None or any(getattr(a, "sinks", None) is not None for a in layers):
+        raise NotImplementedError("DraftDecoder knows plain softmax attention only")
+    dtype = model.model.embed_tokens.weight.dtype
+    if dtype not in (torch.float16, torch.bfloat16):
+        raise NotImplementedError(f"DraftDecoder needs a float16 or bfloat16 model, got {dtype}")
+
+
 class DraftDecoder:
-    """A Hugging Face Llama model (batch 1, head_dim 128) over per-layer TurboPolar caches."""
+    """A Hugging Face Llama model (batch 1, head_dim 128, float16 or bfloat16, attention over the whole history)
+    over per-layer TurboPolar caches."""
 
     def __init__(self, model, cache: Optional[TurboPolarCache] = None, max_seq_len: Optional[int] = None,
                  check_finite: bool = False):
+        _check_model(model)
         cfg = model.config
         self.model, self.device = model, next(model.parameters()).device
         self.hq, self.hkv = cfg.num_attention_heads, cfg.num_key_value_heads
-        head_dim = getattr(cfg, "head_dim", None) or cfg.hidden_size // cfg.num_attention_heads
-        if head_dim != 128:
-            raise NotImplementedError("TurboPolar only supports head_dim == 128")
         self.cache = cache if cache is not None else make_turbo_caches(
-            cfg.num_hidden_layers, self.hq, self.hkv, head_dim, device=self.device, max_seq_len=max_seq_len,
+            cfg.num_hidden_layers, self.hq, self.hkv, 128, device=self.device, max_seq_len=max_seq_len,
             check_finite=check_finite)
         # Of the last verify(): per layer the drafts' keys and values; their parents; the offset they follow.
         self._drafts: List[Tuple[torch.Tensor, torch.Tensor]] = []
@@ -89,7 +108,10 @@ class DraftDecoder:
         """Final hidden states of ``tokens`` ``(T,)``; ``attend(layer, attn, q, k, v)`` is the attention."""
         base = self.model.model
         x = base.embed_tokens(tokens[None])
-        cos, sin = (r[0, :, :64] for r in base.rotary_emb(x, positions[None]))
+        tables = base.rotary_emb(x, positions[None])
+        if any(r.shape[-1] != 128 for r in tables):
+            raise NotImplementedError("norm_rope rotates whole heads; this model rotates a part of each")
+        cos, sin = (r[0, :, :64] for r in tables)
         for i, layer in enumerate(base.layers):
             h = layer.input_layernorm(x)
             o = attend(i, layer.self_attn, *self._qkv(layer.self_attn, h, cos, sin))
