@@ -39,6 +39,7 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <exception>
 #include <string>
 #include <vector>
 
@@ -591,14 +592,8 @@ static int launch_prompt(const PromptParams& P, const tp_prompt_plan& plan, cuda
   return check_launch("tp_prompt_attention");
 }
 
-}  // namespace tp
-
-using namespace tp;
-
-extern "C" {
-
-int tp_prompt_plan_make(const int64_t* q_lens, const int64_t* k_lens, int32_t n_seqs, int32_t num_q_heads,
-                        int32_t num_kv_heads, tp_prompt_plan* plan, int32_t* words, size_t n_words) {
+static int make_plan(const int64_t* q_lens, const int64_t* k_lens, int32_t n_seqs, int32_t num_q_heads, int32_t num_kv_heads,
+                     tp_prompt_plan* plan, int32_t* words, size_t n_words) {
   if (!plan || n_seqs < 0 || (n_seqs && (!q_lens || !k_lens)))
     return fail(TP_ERR_INVALID, "tp_prompt_plan_make: NULL argument");
   if (num_kv_heads < 1 || num_q_heads < 1 || num_q_heads % num_kv_heads)
@@ -687,6 +682,21 @@ int tp_prompt_plan_make(const int64_t* q_lens, const int64_t* k_lens, int32_t n_
   std::copy_n(reinterpret_cast<const int32_t*>(merges.data()), merges.size() * (sizeof(PromptMerge) / 4),
               words + items.size() * (sizeof(PromptItem) / 4));
   return TP_OK;
+}
+
+}  // namespace tp
+
+using namespace tp;
+
+extern "C" {
+
+int tp_prompt_plan_make(const int64_t* q_lens, const int64_t* k_lens, int32_t n_seqs, int32_t num_q_heads,
+                        int32_t num_kv_heads, tp_prompt_plan* plan, int32_t* words, size_t n_words) {
+  try {
+    return make_plan(q_lens, k_lens, n_seqs, num_q_heads, num_kv_heads, plan, words, n_words);
+  } catch (const std::exception&) {  // the lists of a batch that asks for more items than the host has memory for
+    return fail(TP_ERR_CUDA, "tp_prompt_plan_make: out of host memory");
+  }
 }
 
 int tp_prompt_attention(const tp_prompt_plan* plan, const int32_t* words, const tp_prompt_rows* rows, const void* q,
