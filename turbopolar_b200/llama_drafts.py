@@ -64,6 +64,16 @@ def _check_model(model) -> None:
         raise NotImplementedError(f"DraftDecoder needs a float16 or bfloat16 model, got {dtype}")
 
 
+def _norm_eps(attn) -> float:
+    """The epsilon of an attention's head norms.  Only norms as Llama's own (``x * rsqrt(mean(x^2) +
+    variance_epsilon) * weight``) are known; others have an ``eps`` or another use of the weight."""
+    norms = [n for n in (getattr(attn, "q_norm", None), getattr(attn, "k_norm", None)) if n is not None]
+    eps = {getattr(n, "variance_epsilon", None) for n in norms}
+    if None in eps or len(eps) > 1:
+        raise NotImplementedError("head norms need one variance_epsilon, as Llama's RMSNorm has")
+    return eps.pop() if eps else 0.0
+
+
 class DraftDecoder:
     """A Hugging Face Llama model (batch 1, head_dim 128, float16 or bfloat16, attention over the whole history)
     over per-layer TurboPolar caches."""
@@ -99,9 +109,8 @@ class DraftDecoder:
         t = x.shape[1]
         q, k, v = (p(x)[0].view(t, -1, 128) for p in (attn.q_proj, attn.k_proj, attn.v_proj))
         norms = [getattr(attn, name, None) for name in ("q_norm", "k_norm")]
-        eps = getattr(norms[0], "variance_epsilon", 1e-6)
         q, k = norm_rope(q, k, cos, sin, q_weight=getattr(norms[0], "weight", None),
-                         k_weight=getattr(norms[1], "weight", None), eps=eps)
+                         k_weight=getattr(norms[1], "weight", None), eps=_norm_eps(attn))
         return q, k, v
 
     def _layers(self, tokens: torch.Tensor, positions: torch.Tensor, attend: Callable) -> torch.Tensor:
