@@ -414,7 +414,9 @@ class TurboPolarKVCacheRuntime:
         to the drafts' positions, float16 or float32; ``T`` is 1 to 256.
         ``mask`` is ``(T, T)`` or ``(B, T, T)`` bool: draft ``t`` sees draft ``d`` where
         ``mask[t, d]``, usually its ancestors and itself.  Every draft sees the whole cache.
-        A draft that is masked has no influence on a row, whatever it holds.
+        A draft that is masked has no influence on a row, whatever it holds.  Scores, maxima, sums and
+        accumulators are float32, of float32 inputs of any size too; softmax weights are rounded to float16 for
+        the product with the values (keys beyond 2^16 and values beyond float16 are multiplied in float32).
 
         Returns float16 ``(B, H_q, T, 128)``, a view of a ``(B, T, H_q, 128)`` buffer (``out`` if
         given), so that ``.transpose(1, 2).reshape(B, T, -1)`` copies nothing.  After verification,

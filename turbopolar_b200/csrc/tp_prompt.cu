@@ -17,12 +17,13 @@
 //   warp 9           loads tiles (TMA) into a ring of five or six 32 KB stages: K0 V0 K1 V1 ...
 //   warps 10, 11     clean value tiles that some row does not see whole
 //
-// Bound, one 16K prompt of 32 + 8 heads (1.85 to 1.95 ms by the clock that the power limit leaves, about
-// 1,150 TFLOP/s of the causal half's products): exponentials and the chain around them.  128 keys for both tiles
-// take about 3,170 cycles, of which the two softmaxes' special-function work is 2,048 and the products
-// 1,040; what is left is the latency of scores, weights and products after one another.  Keys in units of 64
-// with two score buffers per tile took 4,500 (products with 64 columns wait for shared memory), two issuing
-// warps and a share of the exponentials as polynomials on the FMA pipe were slower too.
+// Bound, one 16K prompt of 32 + 8 heads (1.82 to 1.92 ms by the clock that the power limit leaves, about
+// 1,150 to 1,200 TFLOP/s of the causal half's products): tensor cores and special-function units alike, neither
+// hidden under the other.  128 keys for both tiles take about 3,170 cycles, of which the four products need 2,050 (8.4 M
+// multiply-adds at 4,096 a cycle) and the exponentials 2,048 (32,768 at 16 a cycle); counters: 54% and 57%.  The rest
+// is the latency of scores, weights and products after one another: a tile's weights are handed over whole.  Keys in
+// units of 64 with two score buffers per tile took 4,500 (products with 64 columns wait for shared memory), two
+// issuing warps and a share of the exponentials as polynomials on the FMA pipe were slower too.
 // Bound, packed requests (12 of 1 to 2,500 tokens, 146 us): an item has 7 key tiles in the mean, and its
 // start and end, about 7 us, stand beside 12 us of tiles.  CTAs that stay and take items in turn,
 // with the next item's loads and first scores under the last one's end, gained that back for items of one or

@@ -16,16 +16,19 @@
 //   warp 17          copies pages as they are stored into a ring of three (bulk copies)
 //   warps 18, 19     complete the warpgroup (registers are moved per warpgroup)
 //
-// Bound, 32 drafts x 4 heads over 32K tokens (39.4 us; the pages' bytes take 12.1): a step's decode, about 1,700
-// cycles of latency and 1,090 shared-memory wavefronts, where its bytes take 814.  Eight decode warps with four
-// stages hide part of it; sixteen gained nothing.  64 drafts over 128K: 182 us, of which the products take 84.
-// Short contexts (100 tokens, 5 drafts: 10.0 us) are one CTA's chain of copy, decode, scores, weights and rows.
+// Time, 32 drafts x 4 heads over 32K tokens: 40.3 us, where the pages' bytes take 12.1.  No pipe is busy (issue slots
+// 48%, shared memory 31%, special functions 26%, tensor 19%): a step is a chain of latencies of about 1,700 cycles
+// (page wait, stage wait, loads, decode, proxy fence, arrival), which all eight decode warps go through for an eighth
+// of the page each.  Sixteen warps on the same chain gained nothing; no other arrangement of eight was tried.
+// 64 drafts over 128K: 186 us, of which the products take 84.
+// Short contexts (100 tokens, 5 drafts: 10.2 us) are one CTA's chain of copy, decode, scores, weights and rows.
 //
 // With more than 128 rows the softmax warpgroups have a tile each; with fewer they take
 // alternate steps of the one tile, each with its own running maximum, sum and accumulator, and
 // merge at the segment's end.
 //
-// Float32 queries, tails and drafts are split into two float16 parts (22 bits), so only the weights and the output are
+// Float32 queries, tails and drafts (100 tokens, 5 drafts: 15.4 us; 32K x 32: 52.5 us, a page for one tile of rows instead
+// of two) are split into two float16 parts (22 bits), so only the weights and the output are
 // rounded to float16; rounded inputs had twice the error of a float32 computation on contexts of few tokens.
 // The queries' second part takes the tensor memory of a second tile, a key's second part a row of its own.  A row of
 // queries or keys is first brought into float16's range by a power of two of its own, taken out again of its scores

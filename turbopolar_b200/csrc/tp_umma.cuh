@@ -283,6 +283,10 @@ struct Bits64 {
 // made again in the few tiles that move the reference: the special-function unit, which needs 8 cycles
 // for a warp's exponential (1,024 for 128 columns), does not wait for the maximum.
 //
+// Weights are rounded to the 16-bit input type (float16 for trees) for the product, the sum is of the unrounded ones:
+// 0.00021 to 0.00027 of the norm from the 64-bit result where rounding the output alone gives 0.00021 (bfloat16 0.0020
+// and 0.0016).  A second part of each would halve what the weights add and double the second product.
+//
 // kTwice: the scores of column c are the sum of columns c and c + kCols (a key in two parts) times `factors[c]` in
 // shared memory, and its weight is written to both.  Where the factor is 0 the score is exact(c) instead.
 struct NoExact {
