@@ -711,7 +711,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_kernel(const _
     auto radius_scale = [&](int h, int page) {
       return P.pool.int8_radii ? __half2float(P.pool.radii_scales[int64_t(h) * P.pool.page_capacity + page]) : 0.0f;
     };
-    if (kMode != kTreeDefault && s < P.n_page_steps) rscale_next = radius_scale(head, s);
+    if (kMode != kTreeDefault && count && s < P.n_page_steps) rscale_next = radius_scale(head, s);
     bool ok = true;
     for (int i = 0; i < count && ok; ++i) {
       const int at = s, h = head;
